@@ -33,6 +33,7 @@ ACTIVATIONS = {"none": ACT_NONE, "relu": ACT_RELU, "gelu": ACT_GELU}
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ROUTER_BLOCK_TOKENS = 128
 MAX_EXPERTS = 128
+KV4_PAGE_TOKENS = 64
 NOALLOC_MAX_TOKENS = 131072
 NOALLOC_MAX_EXPERTS = 128
 
@@ -90,6 +91,21 @@ SIGNATURES = {
     "cti_add_layernorm": (
         _I,
         [_P, _P, _P, _P, _I64, _I, ctypes.c_float, _P, _P, _P],
+    ),
+    "cti_kv4_page_bytes": (_SZ, [_I, _I]),
+    "cti_kv4_append": (
+        _I,
+        [_P, _P, _I64, _I64, _I, _P, _P, _P, _I64, _I, _I, _I64, _I, _I, _P, _I64, _P, _P],
+    ),
+    "cti_kv4_read": (
+        _I,
+        [_P, _I64, _I, _P, _P, _P, _I64, _I, _I, _I64, _I, _I, _P, _P, _I64, _I64, _P, _P],
+    ),
+    "cti_kv4_attention_workspace_bytes": (_SZ, [_I, _I64, _I, _I64, _I, _I, _I]),
+    "cti_kv4_attention": (
+        _I,
+        [_P, _I64, _I, _P, _P, _P, _I64, _I, _I, _I64, _I, _I64, _I, _I, _I, ctypes.c_float, _I,
+         _P, _I64, _P, _P, _SZ, _P, _P],
     ),
 }
 

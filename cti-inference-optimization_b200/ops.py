@@ -7,12 +7,14 @@ tensors.  They are the building blocks of :class:`SMoE` and
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
 from ._lib import check, lib, ptr, require_cuda, stream_handle, status_word
+from .kv_cache import PAGE_TOKENS, KV4Cache
 
 
 @dataclass
@@ -354,3 +356,158 @@ def ctr_head(h: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tens
         "cti_ctr_head",
     )
     return logits, probs
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device for a launch (no switch where it is)."""
+    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _kv4_rows(t: torch.Tensor, name: str, cache: KV4Cache, heads: int) -> None:
+    """A [tokens, heads, head_dim] view with contiguous heads in the cache's type."""
+    if not t.is_cuda or t.dtype != cache.dtype:
+        raise TypeError(f"{name} must be a {cache.dtype} CUDA tensor")
+    if t.device != cache.device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    hd = cache.head_dim
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd:
+        raise ValueError(f"{name} must be [tokens, {heads}, {hd}], got {tuple(t.shape)}")
+    if t.shape[0] and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd)):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous heads")
+
+
+def _kv4_stride(t: torch.Tensor, row: int) -> int:
+    """Token stride as the C entry points take it (a single token has any)."""
+    return t.stride(0) if t.shape[0] > 1 else row
+
+
+def _kv4_index(cache: KV4Cache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
+               page_table: torch.Tensor) -> int:
+    """Checks the index tensors; returns the number of sequences."""
+    dev = cache.device
+    for name, t in (("cu_seqlens", cu_seqlens), ("kv_lens", kv_lens)):
+        require_cuda(t, name, torch.int32)
+        if t.dim() != 1:
+            raise ValueError(f"{name} must have one dimension")
+    if not page_table.is_cuda or page_table.dtype != torch.int32:
+        raise TypeError("page_table must be an int32 CUDA tensor")
+    n = kv_lens.shape[0]
+    if cu_seqlens.shape[0] != n + 1:
+        raise ValueError(f"cu_seqlens must have {n + 1} entries for {n} sequences")
+    if page_table.dim() != 2 or page_table.shape[0] != n:
+        raise ValueError(f"page_table must be [{n}, pages], got {tuple(page_table.shape)}")
+    if page_table.numel() and page_table.shape[1] > 1 and page_table.stride(1) != 1:
+        raise ValueError("page_table rows must be contiguous")
+    if cu_seqlens.device != dev or kv_lens.device != dev or page_table.device != dev:
+        raise ValueError(f"cu_seqlens, kv_lens and page_table must be on {dev}")
+    return n
+
+
+def _table_stride(page_table: torch.Tensor) -> int:
+    return page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+
+
+def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+               kv_lens: torch.Tensor, page_table: torch.Tensor) -> None:
+    """Quantises keys and values into the 4-bit cache (see cti_kv4_append).
+    k, v [tokens, kv_heads, head_dim] views of the cache's dtype (any token
+    stride); cu_seqlens int32 [N+1] packs them by sequence; kv_lens int32 [N]
+    are the sequences' lengths with these tokens, which are their last;
+    page_table int32 [N, pages].  A position past the table or a page outside
+    the cache is skipped and reported in the device status word."""
+    n = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
+    H, hd, dev = cache.kv_heads, cache.head_dim, cache.device
+    _kv4_rows(k, "k", cache, H)
+    _kv4_rows(v, "v", cache, H)
+    if v.shape[0] != k.shape[0]:
+        raise ValueError("k and v must have the same number of tokens")
+    with _on(dev):
+        rc = lib.cti_kv4_append(
+            k.data_ptr(), v.data_ptr(), _kv4_stride(k, H * hd), _kv4_stride(v, H * hd),
+            _lib.DTYPE_CODES[cache.dtype], cu_seqlens.data_ptr(), kv_lens.data_ptr(),
+            page_table.data_ptr(), _table_stride(page_table), page_table.shape[1], n, k.shape[0],
+            H, hd, cache.pages.data_ptr(), cache.num_pages, status_word(dev).data_ptr(),
+            stream_handle(dev))
+    check(rc, "cti_kv4_append")
+
+
+def kv4_read(cache: KV4Cache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
+             page_table: torch.Tensor, tokens: int,
+             out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """What the cache holds for the last cu_seqlens[i+1] - cu_seqlens[i] tokens
+    of every sequence (see cti_kv4_read): (k, v), each [tokens, kv_heads,
+    head_dim] in the cache's dtype.  ``tokens`` is cu_seqlens[-1]; with
+    cu_seqlens the offsets of kv_lens, whole sequences are read.  ``out``: the
+    two tensors to write (rows of no sequence keep their contents)."""
+    n = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
+    H, hd, dev = cache.kv_heads, cache.head_dim, cache.device
+    tokens = int(tokens)
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    if out is None:
+        k = torch.empty((tokens, H, hd), dtype=cache.dtype, device=dev)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        for name, t in (("out[0]", k), ("out[1]", v)):
+            _kv4_rows(t, name, cache, H)
+            if t.shape[0] != tokens:
+                raise ValueError(f"{name} must hold {tokens} tokens")
+    with _on(dev):
+        rc = lib.cti_kv4_read(
+            cache.pages.data_ptr(), cache.num_pages, _lib.DTYPE_CODES[cache.dtype],
+            cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
+            _table_stride(page_table), page_table.shape[1], n, tokens, H, hd, k.data_ptr(),
+            v.data_ptr(), _kv4_stride(k, H * hd), _kv4_stride(v, H * hd),
+            status_word(dev).data_ptr(), stream_handle(dev))
+    check(rc, "cti_kv4_read")
+    return k, v
+
+
+def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
+                  kv_lens: torch.Tensor, page_table: torch.Tensor, max_new: int | None = None,
+                  causal: bool = True, scale: float | None = None,
+                  max_kv_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens over the 4-bit cache, which holds their own keys
+    and values already (see cti_kv4_attention).  q [tokens, heads, head_dim]
+    view of the cache's dtype, heads a multiple of the cache's kv_heads (query
+    head h reads KV head h // (heads // kv_heads)); the other arguments as in
+    kv4_append.  causal: a token sees the keys up to its own position, else all
+    of its sequence's.  scale: of the scores, 1 / sqrt(head_dim) by default.
+    max_new, max_kv_len: bounds of the new tokens of a sequence and of kv_lens
+    (defaults: from the token count and the table's width); the work is split
+    by them, results hold for any.  Returns a contiguous [tokens, heads,
+    head_dim]; a token that sees no key is zero."""
+    n = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
+    hd, dev = cache.head_dim, cache.device
+    if q.dim() != 3 or q.shape[1] <= 0 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"q must be [tokens, heads, head_dim] with heads a multiple of "
+                         f"{cache.kv_heads}, got {tuple(q.shape)}")
+    T, H, _ = q.shape
+    _kv4_rows(q, "q", cache, H)
+    cols = page_table.shape[1]
+    if max_new is None:
+        max_new = 1 if T <= n else T
+    if max_kv_len is None:
+        max_kv_len = cols * PAGE_TOKENS
+    if scale is None:
+        scale = hd ** -0.5
+    if out is None:
+        out = torch.empty((T, H, hd), dtype=cache.dtype, device=dev)
+    else:
+        _kv4_rows(out, "out", cache, H)
+        if out.shape[0] != T or not out.is_contiguous():
+            raise ValueError("out must be contiguous, of q's shape")
+    with _on(dev):
+        need = lib.cti_kv4_attention_workspace_bytes(n, T, int(max_new), int(max_kv_len), H,
+                                                     cache.kv_heads, hd)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        rc = lib.cti_kv4_attention(
+            q.data_ptr(), _kv4_stride(q, H * hd), _lib.DTYPE_CODES[cache.dtype],
+            cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
+            _table_stride(page_table), cols, n, T, int(max_new), int(max_kv_len), H,
+            cache.kv_heads, hd, float(scale), int(bool(causal)), cache.pages.data_ptr(),
+            cache.num_pages, out.data_ptr(), ptr(ws), need, status_word(dev).data_ptr(),
+            stream_handle(dev))
+    check(rc, "cti_kv4_attention")
+    return out

@@ -352,6 +352,71 @@ int cti_ctr_head(const void* h_bf16, const void* W1_bf16, const float* b1, const
                  const float* b2, int64_t T, int D, int Hd, float limit, float* logits,
                  float* probs, int32_t* status, void* stream);
 
+/* ----------------------------------------------------------------------
+ * The 4-bit key/value cache: a user's history is held per layer, and a
+ * forward runs the new tokens only (the reference recomputes every token of
+ * every sequence, baseline/infer.py:388-409).
+ *
+ * Each 32 consecutive head dims of a token's key or value are held as 32
+ * codes n with a scale s and a base b of the tensors' type T
+ * (dtype CTI_DTYPE_BF16 or CTI_DTYPE_F16):
+ *   s = T((max - min) / 15),  b = T(min - 16 s),
+ *   n = clamp(round((x - b) / s) - 16, 0, 15)   (ties to even; 0 where s = 0)
+ * and stand for (16 + n) s + b.  A group with a value that is not finite (or
+ * whose b is not: magnitudes above 20,000 in fp16) stands for NaN as a whole.
+ * head_dim 32, 64 or 128 (CTI_ERR_UNSUPPORTED otherwise).
+ *
+ * pages: num_pages pages of cti_kv4_page_bytes(kv_heads, head_dim) bytes,
+ * 16-byte aligned; a page holds CTI_KV4_PAGE_TOKENS tokens of every KV head.
+ * page_table int32 [num_seqs][table_cols], rows table_stride elements apart:
+ * token p of sequence s is token p % 64 of page page_table[s][p / 64].
+ * cu_seqlens int32 [num_seqs+1] (non-decreasing): the packed tokens of
+ * sequence s are cu[s] .. cu[s+1] - 1; they are the LAST ones of its
+ * kv_lens[s] (int32) tokens, so packed token t has position
+ * kv_lens[s] - cu[s+1] + t.  Sequences may share pages that no call writes.
+ * A position or page outside its buffer raises CTI_ERR_BOUNDS in `status`
+ * (detail: the sequence) and is left out: not written, read as zeros, or not
+ * attended to.  Rows of no sequence are left as they were.
+ * ---------------------------------------------------------------------- */
+#define CTI_KV4_PAGE_TOKENS 64
+size_t cti_kv4_page_bytes(int kv_heads, int head_dim);
+
+/* Writes the packed tokens' keys and values (views [tokens][kv_heads][head_dim]
+ * with token strides in elements, multiples of 8, 16-byte aligned bases). */
+int cti_kv4_append(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int dtype,
+                   const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* page_table,
+                   int64_t table_stride, int table_cols, int num_seqs, int64_t tokens,
+                   int kv_heads, int head_dim, void* pages, int64_t num_pages, int32_t* status,
+                   void* stream);
+
+/* The inverse: k, v (as above) = what the cache holds for the packed tokens,
+ * rounded to T; with cu_seqlens the offsets of kv_lens, whole sequences. */
+int cti_kv4_read(const void* pages, int64_t num_pages, int dtype, const int32_t* cu_seqlens,
+                 const int32_t* kv_lens, const int32_t* page_table, int64_t table_stride,
+                 int table_cols, int num_seqs, int64_t tokens, int kv_heads, int head_dim, void* k,
+                 void* v, int64_t k_stride, int64_t v_stride, int32_t* status, void* stream);
+
+/* Attention of the packed tokens' queries over the cache, which holds their
+ * own keys and values already (append first):
+ *   out[t, h, :] = sum_j softmax_j(scale q[t, h, :] . k_j) v_j
+ * over the keys j <= position of t of its sequence (causal = 1) or all
+ * kv_lens[s] of them (causal = 0: candidates scored side by side).  Query
+ * head h reads KV head h / (heads / kv_heads).  q [tokens][heads][head_dim]
+ * with a token stride as above; out the same, contiguous.  A row that sees
+ * no key is zero.  max_new and max_kv_len: the caller's bounds of the new
+ * tokens and of kv_lens; the work is split by them, results hold for any.
+ * workspace: cti_kv4_attention_workspace_bytes(...) bytes, 256-byte aligned
+ * (may be NULL where that is 0); contents do not outlive the call. */
+size_t cti_kv4_attention_workspace_bytes(int num_seqs, int64_t tokens, int max_new,
+                                         int64_t max_kv_len, int heads, int kv_heads,
+                                         int head_dim);
+int cti_kv4_attention(const void* q, int64_t q_stride, int dtype, const int32_t* cu_seqlens,
+                      const int32_t* kv_lens, const int32_t* page_table, int64_t table_stride,
+                      int table_cols, int num_seqs, int64_t tokens, int max_new,
+                      int64_t max_kv_len, int heads, int kv_heads, int head_dim, float scale,
+                      int causal, const void* pages, int64_t num_pages, void* out,
+                      void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
