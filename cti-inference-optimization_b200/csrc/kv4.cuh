@@ -8,9 +8,10 @@
 // and stand for (16 + n) s + b.  The 16 makes a number out of a code without
 // arithmetic: a T with the exponent of 16 and the code in its top four
 // mantissa bits is 16 + n, so unpacking is a shift and one three-input logic
-// operation, and a value is one fused multiply-add away.  b is rounded after
-// the 16 s has been taken off it; that moves the grid by at most 1/20 of a
-// step (bf16).  A constant group has s = 0 and is held exactly.  A group with
+// operation, and a value is one fused multiply-add away.  b is rounded with
+// the 16 s already taken off; that moves the grid by half a unit of T in b at
+// most, as much as the group's values were rounded by when they became T's.
+// A constant group has s = 0 and is held exactly.  A group with
 // a value that is not finite, or whose b is not, has s = b = NaN: all of it
 // reads back as NaN.
 //
@@ -87,14 +88,52 @@ struct Type16<__half> {
   }
 };
 
+// a b + c of both halves in T, rounded once.
+template <typename T>
+CTI_DEVICE uint32_t fma2(uint32_t a, uint32_t b, uint32_t c);
+template <>
+CTI_DEVICE uint32_t fma2<__nv_bfloat16>(uint32_t a, uint32_t b, uint32_t c) {
+  __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&a),
+                             *reinterpret_cast<__nv_bfloat162*>(&b),
+                             *reinterpret_cast<__nv_bfloat162*>(&c));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+template <>
+CTI_DEVICE uint32_t fma2<__half>(uint32_t a, uint32_t b, uint32_t c) {
+  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
+                      *reinterpret_cast<__half2*>(&c));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// 16 + n twice from nibble j of both halves of a K word (rotated left by 3)
+// or a V word.
+template <typename T>
+CTI_DEVICE uint32_t k_pair(uint32_t w, int j) {
+  constexpr int s = Type16<T>::kShift;
+  const int r = 3 + 4 * j - s;  // right shift that brings the nibble to bits s..s+3
+  const uint32_t x = r < 0 ? w << -r : j == 3 ? __funnelshift_r(w, w, r) : w >> r;
+  return (x & (0x000f000fu << s)) | Type16<T>::kMagic;
+}
+template <typename T>
+CTI_DEVICE uint32_t v_pair(uint32_t w, int j) {
+  constexpr int s = Type16<T>::kShift;
+  const int r = 4 * j - s;
+  const uint32_t x = r < 0 ? w << -r : w >> r;
+  return (x & (0x000f000fu << s)) | Type16<T>::kMagic;
+}
+
 // Where a packed token's key and value live.
 struct Place {
   int64_t page;  // -1: nowhere (an index outside its buffer; the status word says so)
   int slot;
 };
 
-// Largest s in [0, n) with cu[s] <= t (cu[0] <= t < cu[n]).
-CTI_DEVICE int sequence_of(const int32_t* __restrict__ cu, int n, int t) {
+// Largest s in [0, n) with cu[s] <= t (cu[0] <= t < cu[n]).  Tried first: the
+// sequence that t lies in if all are equally long, at once right for batches
+// of single tokens.
+CTI_DEVICE int sequence_of(const int32_t* __restrict__ cu, int n, int tokens, int t) {
+  const int guess = (int)((int64_t)t * n / tokens);
+  if (__ldg(cu + guess) <= t && t < __ldg(cu + guess + 1)) return guess;
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -104,25 +143,27 @@ CTI_DEVICE int sequence_of(const int32_t* __restrict__ cu, int n, int t) {
   return lo;
 }
 
+// The page of position p of sequence s, or -1.
+CTI_DEVICE int64_t page_of(const int32_t* __restrict__ table, int64_t table_stride, int table_cols,
+                           int64_t num_pages, int s, int64_t p, int32_t* status) {
+  if (p >= 0 && p / kPage < table_cols) {
+    const int64_t page = __ldg(table + s * table_stride + p / kPage);
+    if (page >= 0 && page < num_pages) return page;
+  }
+  raise_status(status, CTI_ERR_BOUNDS, s);
+  return -1;
+}
+
 // The place of packed new token t: the last cu[s+1] - cu[s] of sequence s's
 // kv_lens[s] tokens are the new ones.
 CTI_DEVICE Place place_of(const int32_t* __restrict__ cu, const int32_t* __restrict__ kv_lens,
                           const int32_t* __restrict__ table, int64_t table_stride, int table_cols,
-                          int num_seqs, int64_t num_pages, int t, int32_t* status) {
-  const int s = sequence_of(cu, num_seqs, t);
+                          int num_seqs, int tokens, int64_t num_pages, int t,
+                          int32_t* status) {
+  const int s = sequence_of(cu, num_seqs, tokens, t);
   const int64_t p = (int64_t)__ldg(kv_lens + s) - __ldg(cu + s + 1) + t;
-  Place at = {-1, (int)(p & (kPage - 1))};
-  if (p < 0 || p / kPage >= table_cols) {
-    raise_status(status, CTI_ERR_BOUNDS, s);
-    return at;
-  }
-  const int64_t page = __ldg(table + s * table_stride + p / kPage);
-  if (page < 0 || page >= num_pages) {
-    raise_status(status, CTI_ERR_BOUNDS, s);
-    return at;
-  }
-  at.page = page;
-  return at;
+  return {page_of(table, table_stride, table_cols, num_pages, s, p, status),
+          (int)(p & (kPage - 1))};
 }
 
 }  // namespace kv4

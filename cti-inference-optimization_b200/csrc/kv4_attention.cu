@@ -76,12 +76,6 @@ struct Mma<__nv_bfloat16> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  CTI_DEVICE static uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-    __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&a),
-                               *reinterpret_cast<__nv_bfloat162*>(&b),
-                               *reinterpret_cast<__nv_bfloat162*>(&c));
-    return *reinterpret_cast<uint32_t*>(&r);
-  }
   static constexpr uint32_t kInf = 0x7f80u;
 };
 template <>
@@ -93,30 +87,8 @@ struct Mma<__half> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  CTI_DEVICE static uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-    __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
-                        *reinterpret_cast<__half2*>(&c));
-    return *reinterpret_cast<uint32_t*>(&r);
-  }
   static constexpr uint32_t kInf = 0x7c00u;
 };
-
-// 16 + n twice from nibble j of both halves of a K word (rotated left by 3)
-// or a V word.
-template <typename T>
-CTI_DEVICE uint32_t k_pair(uint32_t w, int j) {
-  constexpr int s = Type16<T>::kShift;
-  const int r = 3 + 4 * j - s;  // right shift that brings the nibble to bits s..s+3
-  const uint32_t x = r < 0 ? w << -r : j == 3 ? __funnelshift_r(w, w, r) : w >> r;
-  return (x & (0x000f000fu << s)) | Type16<T>::kMagic;
-}
-template <typename T>
-CTI_DEVICE uint32_t v_pair(uint32_t w, int j) {
-  constexpr int s = Type16<T>::kShift;
-  const int r = 4 * j - s;
-  const uint32_t x = r < 0 ? w << -r : w >> r;
-  return (x & (0x000f000fu << s)) | Type16<T>::kMagic;
-}
 
 CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
@@ -395,8 +367,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G))
               blk + v_codes_at(G) + ((i1 >> 2) * 32 + lane) * 16 + (i1 & 3) * 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            M::run(o[4 * g + j], pa, M::fma2(v_pair<T>(w0, j), m0.x, m0.y),
-                   M::fma2(v_pair<T>(w1, j), m1.x, m1.y));
+            M::run(o[4 * g + j], pa, fma2<T>(v_pair<T>(w0, j), m0.x, m0.y),
+                   fma2<T>(v_pair<T>(w1, j), m1.x, m1.y));
         }
       }
       __syncwarp();

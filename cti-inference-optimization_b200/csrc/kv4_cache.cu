@@ -1,11 +1,16 @@
 // Writing tokens into the 4-bit key/value cache and reading them back
 // (format: kv4.cuh).
 //
-// A block takes 32 packed tokens: its first warp finds their pages and
-// slots, then every thread takes 8 dims of a token's key and value at a
-// time: one 16-byte load each, the four threads of a group share minimum and
-// maximum, and each packs its 8 codes.  HBM-bound: 4 + 1.25 bytes per
-// element pair (a key's and a value's) either way.
+// Two ways, by the tokens that a sequence has in the call:
+//   runs    a block takes 64 packed tokens and cuts them into runs that lie
+//           side by side in one page; a warp takes a run's keys or values in
+//           one head.  Its lanes are those of the page's layout, so it moves
+//           whole 16-byte vectors of codes.
+//   tokens  a block takes 8 packed tokens, every thread 8 dims of a token's
+//           key and value.  For calls with a few tokens per sequence, whose
+//           runs would leave most lanes of a warp idle.
+// HBM-bound: 4 + 1.25 bytes per element pair (a key's and a value's) either
+// way.
 #include <cfloat>
 
 #include "kv4.cuh"
@@ -15,8 +20,13 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kTokens = 32;    // packed tokens of a block
+constexpr int kSMs = 148;
 constexpr int kThreads = 256;
+constexpr int kTokens = 8;      // packed tokens of a block, by tokens
+constexpr int kRunTokens = 128;  // and by runs, at most
+constexpr int64_t kMaxStride = (int64_t)1 << 24;
+// A sequence's tokens in a call, on average, from which runs are used.
+constexpr int kRunsFrom = 8;
 
 struct Args {
   const int32_t* cu;
@@ -30,6 +40,7 @@ struct Args {
   int64_t num_pages;
   int64_t k_stride, v_stride;
   int32_t* status;
+  int tile;  // packed tokens of a block
 };
 
 CTI_DEVICE float min_nan(float a, float b) {
@@ -42,59 +53,103 @@ CTI_DEVICE float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-
-// The code of x in the group with base b and scale s (inv = 1 / s), exactly:
-// k = rint(x / s - b / s) from the reciprocal is at most one off, and only
-// where x is within rounding of the border between two codes.  The remainder
-// r = (x - b) - (16 + k) s is exact (it is a small difference of numbers on
-// the scale's grid), so |r| < s / 2 proves k; else the border decides, with
-// the rounding error of x - b taken into account.
-CTI_DEVICE int code_of(float x, float b, float s, float inv) {
-  const float a = x - b;
-  float k = rintf(fmaf(a, inv, -16.0f));
-  const float h = 0.5f * s;
-  const float r = fmaf(-s, 16.0f + k, a);
-  if (fabsf(r) >= h) {
-    const float z = a - x;
-    const float err = (x - (a - z)) + (-b - z);  // x - b = a + err
-    const bool odd = ((int)k & 1) != 0;
-    if (r > 0.0f) {
-      const float over = (r - h) + err;
-      if (over > 0.0f || (over == 0.0f && odd)) k += 1.0f;
-    } else {
-      const float over = (r + h) + err;
-      if (over < 0.0f || (over == 0.0f && odd)) k -= 1.0f;
-    }
-  }
-  return min(max((int)k, 0), 15);
+CTI_DEVICE float min3_nan(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+CTI_DEVICE float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
-// Codes of the 8 values that this thread has of a group of 32 (its quad has
-// the others), and the group's scale and base as 16 bits each.
+// Codes are exact, whatever fp32 rounds.  With a = x - b, the quotient a / s
+// is rounded to nearest by one correction of its estimate's remainder
+// (Markstein), and then to a whole number, ties to even, by adding 1.5 2^23,
+// which leaves k = 16 + n in the low bits.  Rounding twice is right: a has 24
+// bits and lies in [16 s, 32 s), so a / s is either a border k + 1/2 itself
+// or at least 2^-19 away from it, one unit of the quotient.  Two cases are
+// looked at again, out of line:
+//   - an end of the group comes out below code 0 or above 15, because b's or
+//     s's rounding moved the grid;
+//   - a was rounded, which takes an |x| far below |b|, where a is -b, and -b
+//     lies on a border: then x's sign decides.
+constexpr float kRound = 12582912.0f;  // 1.5 2^23
+constexpr uint32_t kRoundBits = 0x4b400000u;
+
+enum Order { kKeys, kValues };  // dims 2 j at 4 j, 2 j + 1 at 16 + 4 j; or dim j at 4 j
+__host__ __device__ constexpr int dim_at(Order order, int nibble) {
+  return order == kValues ? nibble : nibble < 4 ? 2 * nibble : 2 * nibble - 7;
+}
+
 template <typename T>
-CTI_DEVICE void quantise8(const uint4& raw, uint32_t (&n)[8], uint32_t& s_bits, uint32_t& b_bits) {
+CTI_DEVICE void unpack(const uint4& raw, float (&x)[8]) {
   using Y = Type16<T>;
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     x[2 * i] = Y::low(w[i]);
     x[2 * i + 1] = Y::high(w[i]);
   }
-  float lo = x[0], hi = x[0];
+}
+
+// The nibbles of the 8 t (kRoundBits + 16 + n as bits): a chain of shift-adds
+// less what is not n.
+template <Order ORDER>
+CTI_DEVICE uint32_t pack_codes(const float (&t)[8]) {
+  uint32_t word = 0, less = 0;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
+  for (int i = 7; i >= 0; --i) {
+    word = word * 16 + __float_as_uint(t[dim_at(ORDER, i)]);
+    less = less * 16 + kRoundBits + 16;
   }
+  return word - less;
+}
+
+// The cases above, one value at a time: k is at most one off, the remainder
+// r = a - k s is exact, and where it reaches s / 2 the rounding error of a
+// decides.
+template <typename T, Order ORDER>
+__device__ __noinline__ uint32_t codes_again(uint4 raw, float s, float b, float inv) {
+  float x[8], t[8];
+  unpack<T>(raw, x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = x[i] - b, z = a - x[i];
+    const float err = (x[i] - (a - z)) + (-b - z);  // x - b = a + err
+    float k = rintf(a * inv);
+    const float r = fmaf(-s, k, a);
+    const float over = (fabsf(r) - 0.5f * s) + (r > 0.0f ? err : -err);
+    if (fabsf(r) >= 0.5f * s && (over > 0.0f || (over == 0.0f && ((int)k & 1) != 0)))
+      k += r > 0.0f ? 1.0f : -1.0f;
+    t[i] = kRound + fminf(fmaxf(k, 16.0f), 31.0f);
+  }
+  return pack_codes<ORDER>(t);
+}
+
+// Packs 8 values of a group of 32 (the lanes of the quad have the others)
+// into a word of codes.  Also the group's scale and base, 16 bits each.
+// Bound by instructions: about 80 with the group's part, the element's
+// arithmetic two at a time.
+template <typename T, Order ORDER>
+CTI_DEVICE uint32_t quantise(const uint4& raw, uint32_t& s_bits, uint32_t& b_bits) {
+  using Y = Type16<T>;
+  float x[8];
+  unpack<T>(raw, x);
+  float lo = min3_nan(min3_nan(min3_nan(x[0], x[1], x[2]), x[3], x[4]), x[5], min_nan(x[6], x[7]));
+  float hi = max3_nan(max3_nan(max3_nan(x[0], x[1], x[2]), x[3], x[4]), x[5], max_nan(x[6], x[7]));
 #pragma unroll
   for (int o = 1; o <= 2; o <<= 1) {
     lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  // The scale is rounded to T from fp32; max - min and the quotient are
-  // nearer to the true value than any T border that they could cross.
-  s_bits = Y::bits((hi - lo) / 15.0f);
+  // (hi - lo) / 15 in the same way; its rounding on to T is right too: the
+  // quotient is nearer to the true value than to any border of T that it does
+  // not lie on.
+  const float range = hi - lo;
+  const float q = range * (1.0f / 15.0f);
+  s_bits = Y::bits(fmaf(fmaf(-15.0f, q, range), 1.0f / 15.0f, q));
   float s = Y::to_float(s_bits);
   if (s < FLT_MIN) {  // below the smallest normal fp32 number: a constant group
     s = 0.0f;
@@ -102,38 +157,79 @@ CTI_DEVICE void quantise8(const uint4& raw, uint32_t (&n)[8], uint32_t& s_bits, 
   }
   b_bits = Y::bits(fmaf(-16.0f, s, lo));
   const float b = Y::to_float(b_bits);
-  if (!(fabsf(b) <= FLT_MAX) || !(s <= FLT_MAX)) {
-    s_bits = b_bits = 0x7fffu;  // NaN in both types
-#pragma unroll
-    for (int i = 0; i < 8; ++i) n[i] = 0;
-    return;
+  if (!(fabsf(b) <= FLT_MAX) || !(s <= FLT_MAX)) s_bits = b_bits = 0x7fffu;  // NaN in both types
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  float add = kRound;
+  if (s == 0.0f) {
+    inv = 0.0f;
+    add = kRound + 16.0f;
   }
-  const float inv = s > 0.0f ? 1.0f / s : 0.0f;
+  // a / s for two values at once
+  const uint64_t ns2 = f2_pack(-s, -s), nb2 = f2_pack(-b, -b), inv2 = f2_pack(inv, inv);
+  const uint64_t add2 = f2_pack(add, add);
+  auto k_of = [&](float x0, float x1, float& t0, float& t1) {
+    const uint64_t a = f2_add(f2_pack(x0, x1), nb2);
+    const uint64_t e = f2_mul(a, inv2);
+    f2_unpack(f2_add(f2_fma(f2_fma(ns2, e, a), inv2, e), add2), t0, t1);
+  };
+  float t[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = s > 0.0f ? (uint32_t)code_of(x[i], b, s, inv) : 0u;
+  for (int i = 0; i < 8; i += 2) k_of(x[i], x[i + 1], t[i], t[i + 1]);
+  float t_lo, t_hi;
+  k_of(lo, hi, t_lo, t_hi);
+  bool again = t_lo < kRound + 16.0f || t_hi > kRound + 31.0f;
+  // -b on a border: -b / s = a whole number and a half
+  const float e0 = -b * inv, e1 = fmaf(fmaf(-s, e0, -b), inv, e0);
+  if (fabsf(e1 - rintf(e1)) == 0.5f) {
+    float least = INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) least = fminf(least, x[i] == 0.0f ? INFINITY : fabsf(x[i]));
+    again = again || least < fabsf(b) * 0x1p-12f;
+  }
+  if (again) return codes_again<T, ORDER>(raw, s, b, inv);
+  return pack_codes<ORDER>(t);
 }
 
-CTI_DEVICE void find_places(const Args& a, int t0, Place (&places)[kTokens]) {
-  if (threadIdx.x < kTokens) {
-    const int t = t0 + threadIdx.x;
-    Place at = {-1, 0};
-    if (t < a.tokens && a.num_seqs > 0 && t >= __ldg(a.cu) && t < __ldg(a.cu + a.num_seqs))
-      at = place_of(a.cu, a.kv_lens, a.table, a.table_stride, a.table_cols, a.num_seqs,
-                    a.num_pages, t, a.status);
-    else
-      at.page = -2;  // of no sequence
-    places[threadIdx.x] = at;
-  }
-  __syncthreads();
+CTI_DEVICE uint32_t twice(uint32_t h) { return __byte_perm(h, h, 0x1010); }
+
+// What a K word stands for in T.
+template <typename T>
+CTI_DEVICE uint4 k_values(uint32_t w, uint32_t meta) {
+  const uint32_t s = __byte_perm(meta, 0, 0x1010), b = __byte_perm(meta, 0, 0x3232);
+  return make_uint4(fma2<T>(k_pair<T>(w, 0), s, b), fma2<T>(k_pair<T>(w, 1), s, b),
+                    fma2<T>(k_pair<T>(w, 2), s, b), fma2<T>(k_pair<T>(w, 3), s, b));
+}
+// What a V word stands for: its even token's 4 values, and its odd one's.
+template <typename T>
+CTI_DEVICE void v_values(uint32_t w, uint32_t s, uint32_t b, uint2& even, uint2& odd) {
+  uint32_t x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = fma2<T>(v_pair<T>(w, j), s, b);
+  even = make_uint2(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410));
+  odd = make_uint2(__byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
 }
 
+// Place of packed token t, page -2 where it is of no sequence.
+CTI_DEVICE Place find_place(const Args& a, int t) {
+  Place at = {-2, 0};
+  if (t < a.tokens && t >= __ldg(a.cu) && t < __ldg(a.cu + a.num_seqs))
+    at = place_of(a.cu, a.kv_lens, a.table, a.table_stride, a.table_cols, a.num_seqs, a.tokens,
+                  a.num_pages, t, a.status);
+  return at;
+}
+
+// ---------------------------------------------------------------------------
+// By tokens.
+// ---------------------------------------------------------------------------
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads)
-    kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, Args a,
-                      uint8_t* __restrict__ pages) {
+    kv4_append_tokens_kernel(const T* __restrict__ k, const T* __restrict__ v, Args a,
+                             uint8_t* __restrict__ pages) {
   __shared__ Place places[kTokens];
   const int t0 = blockIdx.x * kTokens;
-  find_places(a, t0, places);
+  if (threadIdx.x < kTokens) places[threadIdx.x] = find_place(a, t0 + threadIdx.x);
+  __syncthreads();
   const int per = a.kv_heads * G * 4;  // 8-dim pieces of a token
   const int total = kTokens * per;     // a multiple of 32
   for (int i = threadIdx.x; i < total; i += kThreads) {
@@ -146,21 +242,17 @@ __global__ void __launch_bounds__(kThreads)
       rk = __ldg(reinterpret_cast<const uint4*>(k + (t0 + tok) * a.k_stride + piece * 8));
       rv = __ldg(reinterpret_cast<const uint4*>(v + (t0 + tok) * a.v_stride + piece * 8));
     }
-    uint32_t nk[8], nv[8], ks, kb, vs, vb;
-    quantise8<T>(rk, nk, ks, kb);
-    quantise8<T>(rv, nv, vs, vb);
+    uint32_t ks, kb, vs, vb;
+    uint32_t wk = quantise<T, kKeys>(rk, ks, kb);
+    wk = __funnelshift_l(wk, wk, 3);
+    const uint32_t wv = quantise<T, kValues>(rv, vs, vb);
     if (!live) continue;  // the loop's bound is the same for a whole warp
     uint8_t* block = pages + (at.page * a.kv_heads + head) * (int64_t)block_bytes(G);
-    uint32_t wk = 0;
+    *reinterpret_cast<uint32_t*>(block + k_word_at(at.slot, g, t, G)) = wk;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) wk |= nk[2 * j] << (4 * j) | nk[2 * j + 1] << (16 + 4 * j);
-    *reinterpret_cast<uint32_t*>(block + k_word_at(at.slot, g, t, G)) = __funnelshift_l(wk, wk, 3);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const uint32_t hv = nv[4 * c] | nv[4 * c + 1] << 4 | nv[4 * c + 2] << 8 | nv[4 * c + 3] << 12;
+    for (int c = 0; c < 2; ++c)
       *reinterpret_cast<uint16_t*>(block + v_codes_at(G) + v_half_at(at.slot, g, 2 * t + c, G)) =
-          (uint16_t)hv;
-    }
+          (uint16_t)(wv >> (16 * c));
     if (t == 0) {
       *reinterpret_cast<uint32_t*>(block + k_meta_at(G) + k_meta_word_at(at.slot, g, G)) =
           ks | kb << 16;
@@ -173,12 +265,13 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads)
-    kv4_read_kernel(const uint8_t* __restrict__ pages, Args a, T* __restrict__ k,
-                    T* __restrict__ v) {
-  using Y = Type16<T>;
+    kv4_read_tokens_kernel(const uint8_t* __restrict__ pages, Args a, T* __restrict__ k,
+                           T* __restrict__ v) {
   __shared__ Place places[kTokens];
   const int t0 = blockIdx.x * kTokens;
-  find_places(a, t0, places);
+  grid_dependency_wait();
+  if (threadIdx.x < kTokens) places[threadIdx.x] = find_place(a, t0 + threadIdx.x);
+  __syncthreads();
   const int per = a.kv_heads * G * 4;
   const int total = kTokens * per;
   for (int i = threadIdx.x; i < total; i += kThreads) {
@@ -189,33 +282,305 @@ __global__ void __launch_bounds__(kThreads)
     uint4 ok = make_uint4(0, 0, 0, 0), ov = ok;
     if (at.page >= 0) {
       const uint8_t* block = pages + (at.page * a.kv_heads + head) * (int64_t)block_bytes(G);
-      uint32_t wk = __ldg(reinterpret_cast<const uint32_t*>(block + k_word_at(at.slot, g, t, G)));
-      wk = __funnelshift_r(wk, wk, 3);
+      const uint32_t wk =
+          __ldg(reinterpret_cast<const uint32_t*>(block + k_word_at(at.slot, g, t, G)));
       const uint32_t mk = __ldg(
           reinterpret_cast<const uint32_t*>(block + k_meta_at(G) + k_meta_word_at(at.slot, g, G)));
       const uint8_t* vm = block + v_meta_at(G) + v_meta_half_at(at.slot, g, G);
-      const float ks = Y::low(mk), kb = Y::high(mk);
-      const float vs = Y::to_float(__ldg(reinterpret_cast<const uint16_t*>(vm)));
-      const float vb = Y::to_float(__ldg(reinterpret_cast<const uint16_t*>(vm + 4)));
-      uint32_t o[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = Y::pack(fmaf(16.0f + (float)((wk >> (4 * j)) & 15), ks, kb),
-                       fmaf(16.0f + (float)((wk >> (16 + 4 * j)) & 15), ks, kb));
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t hv = __ldg(reinterpret_cast<const uint16_t*>(
-            block + v_codes_at(G) + v_half_at(at.slot, g, 2 * t + c, G)));
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          o[4 + 2 * c + j] = Y::pack(fmaf(16.0f + (float)((hv >> (8 * j)) & 15), vs, vb),
-                                     fmaf(16.0f + (float)((hv >> (8 * j + 4)) & 15), vs, vb));
-      }
-      ok = make_uint4(o[0], o[1], o[2], o[3]);
-      ov = make_uint4(o[4], o[5], o[6], o[7]);
+      const uint32_t vs = __ldg(reinterpret_cast<const uint16_t*>(vm));
+      const uint32_t vb = __ldg(reinterpret_cast<const uint16_t*>(vm + 4));
+      const uint8_t* vc = block + v_codes_at(G);
+      const uint32_t h0 =
+          __ldg(reinterpret_cast<const uint16_t*>(vc + v_half_at(at.slot, g, 2 * t, G)));
+      const uint32_t h1 =
+          __ldg(reinterpret_cast<const uint16_t*>(vc + v_half_at(at.slot, g, 2 * t + 1, G)));
+      uint2 v0, v1;
+      v_values<T>(h0 | h1 << 16, twice(vs), twice(vb), v0, v1);
+      ok = k_values<T>(wk, mk);
+      ov = make_uint4(v0.x, v0.y, v1.x, v1.y);
     }
     *reinterpret_cast<uint4*>(k + (t0 + tok) * a.k_stride + piece * 8) = ok;
     *reinterpret_cast<uint4*>(v + (t0 + tok) * a.v_stride + piece * 8) = ov;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// By runs.
+// ---------------------------------------------------------------------------
+// Side by side in one page: packed tokens [start, start + count), from `slot`
+// of the page on.
+struct Run {
+  int64_t page;
+  int start, count, slot;
+};
+
+// The runs that START among the block's a.tile packed tokens from t0 on, so
+// that no run is cut at a tile's end.  All threads of the block; returns their
+// number.
+CTI_DEVICE int find_runs(const Args& a, int t0, Run (&runs)[kRunTokens]) {
+  static_assert(kRunTokens % 32 == 0 && kRunTokens <= kThreads, "a thread per token");
+  __shared__ int32_t ends[kRunTokens];  // cu[s0 + 1 + i]
+  __shared__ uint32_t starts[kRunTokens / 32];
+  __shared__ int s0_shared;
+  const int i = threadIdx.x, tile = a.tile;
+  if (i < 32) {  // the sequence of token t0, 32 borders at a time
+    int lo = 0, hi = a.num_seqs;  // cu[lo] <= t0 (or lo = 0), and t0 < cu[hi]
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, at = lo + (i + 1) * step;
+      const uint32_t le = __ballot_sync(0xffffffffu, at < hi && __ldg(a.cu + at) <= t0);
+      const int last = __popc(le);
+      hi = min(hi, lo + (last + 1) * step);
+      lo += last * step;
+    }
+    if (i == 0) s0_shared = lo;
+  }
+  __syncthreads();
+  const int s0 = s0_shared;
+  if (i < tile) ends[i] = __ldg(a.cu + min(s0 + 1 + i, a.num_seqs));
+  __syncthreads();
+  const int t = t0 + i;
+  Run run = {-2, t, 0, 0};
+  if (i < tile && t < a.tokens && t >= __ldg(a.cu) && t < __ldg(a.cu + a.num_seqs)) {
+    int s = s0;
+    if (ends[tile - 1] > t) {
+      int lo = -1, hi = tile - 1;  // ends[lo] <= t < ends[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (ends[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      s += hi;
+    } else {  // more than `tile` sequences, empty ones, lie within the tile
+      s = sequence_of(a.cu, a.num_seqs, a.tokens, t);
+    }
+    const int end = min(__ldg(a.cu + s + 1), a.tokens);
+    const int64_t pos = (int64_t)__ldg(a.kv_lens + s) - __ldg(a.cu + s + 1) + t;
+    run.slot = (int)(pos & (kPage - 1));
+    if (t == __ldg(a.cu + s) || run.slot == 0) {
+      run.count = min(kPage - run.slot, end - t);
+      run.page = page_of(a.table, a.table_stride, a.table_cols, a.num_pages, s, pos, a.status);
+    }
+  }
+  if (i < tile) {
+    const uint32_t b = __ballot_sync(0xffffffffu, run.count > 0);
+    if ((i & 31) == 0) starts[i >> 5] = b;
+  }
+  __syncthreads();
+  int count = 0, before = 0;
+  for (int w = 0; w < tile / 32; ++w) {
+    if (w == i / 32) before = count + __popc(starts[w] & ((1u << (i & 31)) - 1));
+    count += __popc(starts[w]);
+  }
+  if (run.count > 0) runs[before] = run;
+  __syncthreads();
+  return count;
+}
+
+// A run's keys (or values) of one head.  Lane 4 r + t takes dims 8 t .. + 7 of
+// every group of token 8 nt + r.
+template <typename T, int G, Order ORDER>
+CTI_DEVICE void append_run(const T* __restrict__ rows, int stride, const Run& run,
+                           uint8_t* __restrict__ block, int lane) {
+  constexpr int kOctets = 4 / G;  // of tokens, in a vector of codes
+  const int r = lane >> 2, t = lane & 3, last = run.slot + run.count - 1;
+  // The lane whose word this one has in the end: keys, its own; values, the
+  // pair of tokens r / 2 and the 4 dims 2 t + r % 2.
+  const int owner = ORDER == kKeys ? lane : (2 * t + (r & 1)) * 4 + (r >> 1);
+  const int v0 = (run.slot >> 3) / kOctets;
+  int tau0 = v0 * kOctets * 8 + r;
+  int src = (tau0 - run.slot) * stride + 8 * t;
+  uint8_t* dst = block + (ORDER == kKeys ? 0 : v_codes_at(G)) + (v0 * 32 + owner) * 16;
+  for (; tau0 - r <= last; tau0 += 8 * kOctets, src += 8 * kOctets * stride, dst += 512) {
+    uint4 raw[4];
+    bool live[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int nt = j / G, g = j % G, tau = tau0 + 8 * nt;
+      live[j] = tau >= run.slot && tau <= last;
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (live[j])
+        raw[j] = __ldg(reinterpret_cast<const uint4*>(rows + (src + 8 * nt * stride) + 32 * g));
+    }
+    uint32_t w[4];
+    bool whole = true;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int nt = j / G, g = j % G, tau = tau0 + 8 * nt;
+      const bool pair = ORDER == kKeys ? live[j]
+                                       : live[j] && (tau ^ 1) >= run.slot && (tau ^ 1) <= last;
+      whole = whole && pair;
+      if (!__any_sync(0xffffffffu, live[j])) continue;
+      uint32_t s, b;
+      const uint32_t word = quantise<T, ORDER>(raw[j], s, b);
+      if (ORDER == kKeys) {
+        w[j] = __funnelshift_l(word, word, 3);
+        if (live[j] && t == 0)
+          *reinterpret_cast<uint32_t*>(block + k_meta_at(G) + k_meta_word_at(tau, g, G)) =
+              s | b << 16;
+      } else {
+        const bool odd = r & 1;
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? word : word >> 16, 4);
+        w[j] = odd ? __byte_perm(got, word, 0x7610) : __byte_perm(word, got, 0x5410);
+        const uint32_t mine = s | b << 16, meta = __shfl_xor_sync(0xffffffffu, mine, 4);
+        uint8_t* vm = block + v_meta_at(G) + v_meta_half_at(tau, g, G);
+        if (live[j] && t == 0) {
+          if (!pair) {
+            *reinterpret_cast<uint16_t*>(vm) = (uint16_t)s;
+            *reinterpret_cast<uint16_t*>(vm + 4) = (uint16_t)b;
+          } else if (!odd) {
+            *reinterpret_cast<uint2*>(vm) =
+                make_uint2(__byte_perm(mine, meta, 0x5410), __byte_perm(mine, meta, 0x7632));
+          }
+        }
+        if (live[j] && !pair) {  // an end of the run: its own halves alone
+          uint8_t* half = block + v_codes_at(G);
+          *reinterpret_cast<uint16_t*>(half + v_half_at(tau, g, 2 * t, G)) = (uint16_t)word;
+          *reinterpret_cast<uint16_t*>(half + v_half_at(tau, g, 2 * t + 1, G)) =
+              (uint16_t)(word >> 16);
+        }
+      }
+      live[j] = pair;
+    }
+    if (whole) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (live[j]) *reinterpret_cast<uint32_t*>(dst + 4 * j) = w[j];
+    }
+  }
+}
+
+// The heads [first, end) of this block: gridDim.y blocks share a tile.
+CTI_DEVICE void head_range(const Args& a, int& first, int& end) {
+  const int per = (a.kv_heads + gridDim.y - 1) / gridDim.y;
+  first = min(a.kv_heads, per * (int)blockIdx.y);
+  end = min(a.kv_heads, first + per);
+}
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads, 4)
+    kv4_append_runs_kernel(const T* __restrict__ k, const T* __restrict__ v, Args a,
+                           uint8_t* __restrict__ pages) {
+  __shared__ Run runs[kRunTokens];
+  const int lane = lane_id();
+  int h0, h1;
+  head_range(a, h0, h1);
+  const int heads = h1 - h0, units = find_runs(a, blockIdx.x * a.tile, runs) * heads * 2;
+  for (int u = warp_id(); u < units; u += kThreads / 32) {
+    const int i = (u >> 1) / heads, head = h0 + (u >> 1) - i * heads;
+    const Run run = runs[i];
+    if (run.page < 0) continue;
+    uint8_t* block = pages + (run.page * a.kv_heads + head) * (int64_t)block_bytes(G);
+    if ((u & 1) == 0)
+      append_run<T, G, kKeys>(k + run.start * a.k_stride + head * (32 * G), (int)a.k_stride, run,
+                              block, lane);
+    else
+      append_run<T, G, kValues>(v + run.start * a.v_stride + head * (32 * G), (int)a.v_stride, run,
+                                block, lane);
+  }
+}
+
+template <typename T, int G>
+CTI_DEVICE void read_keys(const uint8_t* __restrict__ block, const Run& run, T* __restrict__ rows,
+                          int stride, int lane) {
+  constexpr int kOctets = 4 / G;
+  const int r = lane >> 2, t = lane & 3, last = run.slot + run.count - 1;
+  const int v0 = (run.slot >> 3) / kOctets;
+  int tau0 = v0 * kOctets * 8 + r;
+  int dst = (tau0 - run.slot) * stride + 8 * t;
+  const uint8_t* src = block + (v0 * 32 + lane) * 16;
+  const uint32_t* ms = reinterpret_cast<const uint32_t*>(block + k_meta_at(G)) + tau0 * G;
+  // Two vectors at a time, all loads first.
+  for (; tau0 - r <= last; tau0 += 16 * kOctets, dst += 16 * kOctets * stride, src += 1024, ms += 64) {
+    uint4 w4[2];
+    uint32_t meta[8];
+    bool live[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      w4[u] = make_uint4(0, 0, 0, 0);
+      if (tau0 - r + 8 * kOctets * u <= last) w4[u] = __ldg(reinterpret_cast<const uint4*>(src + 512 * u));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int nt = j / G, g = j % G, tau = tau0 + 8 * nt;
+      live[j] = tau >= run.slot && tau <= last;
+      if (live[j]) meta[j] = __ldg(ms + 8 * nt * G + g);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int nt = j / G, g = j % G;
+      const uint32_t w = j % 4 == 0 ? w4[j / 4].x : j % 4 == 1 ? w4[j / 4].y
+                         : j % 4 == 2 ? w4[j / 4].z : w4[j / 4].w;
+      if (live[j])
+        *reinterpret_cast<uint4*>(rows + (dst + 8 * nt * stride) + 32 * g) =
+            k_values<T>(w, meta[j]);
+    }
+  }
+}
+
+template <typename T, int G>
+CTI_DEVICE void read_values(const uint8_t* __restrict__ block, const Run& run,
+                            T* __restrict__ rows, int stride, int lane) {
+  constexpr int kOctets = 4 / G;
+  const int c = lane >> 2, t = lane & 3, last = run.slot + run.count - 1;
+  const int v0 = (run.slot >> 3) / kOctets;
+  int tau0 = v0 * kOctets * 8 + 2 * t;  // and the token after it
+  int dst = (tau0 - run.slot) * stride + 4 * c;
+  const uint8_t* src = block + v_codes_at(G) + (v0 * 32 + lane) * 16;
+  const uint2* ms = reinterpret_cast<const uint2*>(block + v_meta_at(G)) + (tau0 >> 1) * G;
+  for (; tau0 - 2 * t <= last; tau0 += 16 * kOctets, dst += 16 * kOctets * stride, src += 1024, ms += 32) {
+    uint4 w4[2];
+    uint2 meta[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      w4[u] = make_uint4(0, 0, 0, 0);
+      if (tau0 - 2 * t + 8 * kOctets * u <= last) {
+        w4[u] = __ldg(reinterpret_cast<const uint4*>(src + 512 * u));
+#pragma unroll
+        for (int j = 4 * u; j < 4 * u + 4; ++j) meta[j] = __ldg(ms + 4 * (j / G) * G + j % G);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int nt = j / G, g = j % G, tau = tau0 + 8 * nt;
+      const uint32_t w = j % 4 == 0 ? w4[j / 4].x : j % 4 == 1 ? w4[j / 4].y
+                         : j % 4 == 2 ? w4[j / 4].z : w4[j / 4].w;
+      T* to = rows + (dst + 8 * nt * stride) + 32 * g;
+      uint2 even, odd;
+      v_values<T>(w, meta[j].x, meta[j].y, even, odd);
+      if (tau >= run.slot && tau <= last) *reinterpret_cast<uint2*>(to) = even;
+      if (tau + 1 >= run.slot && tau + 1 <= last) *reinterpret_cast<uint2*>(to + stride) = odd;
+    }
+  }
+}
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads, 4)
+    kv4_read_runs_kernel(const uint8_t* __restrict__ pages, Args a, T* __restrict__ k,
+                         T* __restrict__ v) {
+  __shared__ Run runs[kRunTokens];
+  const int lane = lane_id();
+  grid_dependency_wait();
+  int h0, h1;
+  head_range(a, h0, h1);
+  const int heads = h1 - h0, units = find_runs(a, blockIdx.x * a.tile, runs) * heads * 2;
+  for (int u = warp_id(); u < units; u += kThreads / 32) {
+    const int i = (u >> 1) / heads, head = h0 + (u >> 1) - i * heads;
+    const Run run = runs[i];
+    const int64_t stride = (u & 1) == 0 ? a.k_stride : a.v_stride;
+    T* rows = ((u & 1) == 0 ? k : v) + run.start * stride + head * (32 * G);
+    if (run.page < 0) {  // every token of it is outside: zeros
+      for (int j = lane; j < run.count * 4 * G; j += 32)
+        *reinterpret_cast<uint4*>(rows + (j / (4 * G)) * stride + (j % (4 * G)) * 8) =
+            make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const uint8_t* block = pages + (run.page * a.kv_heads + head) * (int64_t)block_bytes(G);
+    if ((u & 1) == 0)
+      read_keys<T, G>(block, run, rows, (int)stride, lane);
+    else
+      read_values<T, G>(block, run, rows, (int)stride, lane);
   }
 }
 
@@ -240,24 +605,52 @@ int check_args(const void* k, const void* v, int dtype, int head_dim, const Args
   const int64_t row = (int64_t)a.kv_heads * head_dim;
   if ((a.k_stride | a.v_stride) % 8 != 0 || a.k_stride < row || a.v_stride < row)
     return CTI_ERR_INVALID_ARG;
+  // A page's tokens are within 2^31 elements of each other.
+  if (a.k_stride > kMaxStride || a.v_stride > kMaxStride) return CTI_ERR_UNSUPPORTED;
   if (a.table_stride < a.table_cols) return CTI_ERR_INVALID_ARG;
   return CTI_OK;
 }
 
+// The way, the tile and the grid of a call.
+struct Launch {
+  bool runs;
+  dim3 grid;
+};
+Launch plan(Args& a, int G) {
+  Launch l;
+  l.runs = a.tokens >= (int64_t)kRunsFrom * a.num_seqs;
+  a.tile = l.runs ? kRunTokens : kTokens;
+  const int64_t tiles = ((int64_t)a.tokens + a.tile - 1) / a.tile;
+  l.grid = dim3((unsigned)tiles);
+  if (l.runs) {
+    // Blocks that share a tile by heads: at least four for each SM in all, as
+    // long as a block's warps have a run each (two runs start in a tile at
+    // the least, with keys and values apart).
+    int64_t share = (kSMs * 4 + tiles - 1) / tiles;
+    const int64_t most = a.kv_heads * G > 2 ? (a.kv_heads + 1) / 2 : 1;
+    l.grid.y = (unsigned)(share > most ? most : share);
+  }
+  return l;
+}
+
 template <typename T, int G>
-int launch_append(const void* k, const void* v, const Args& a, void* pages, cudaStream_t s) {
-  const unsigned grid = (unsigned)((a.tokens + kTokens - 1) / kTokens);
-  kv4_append_kernel<T, G><<<grid, kThreads, 0, s>>>(
-      static_cast<const T*>(k), static_cast<const T*>(v), a, static_cast<uint8_t*>(pages));
+int launch_append(const void* k, const void* v, Args a, void* pages, cudaStream_t s) {
+  const Launch l = plan(a, G);
+  auto* kernel = l.runs ? kv4_append_runs_kernel<T, G> : kv4_append_tokens_kernel<T, G>;
+  kernel<<<l.grid, kThreads, 0, s>>>(static_cast<const T*>(k), static_cast<const T*>(v), a,
+                                     static_cast<uint8_t*>(pages));
   return cudaGetLastError() == cudaSuccess ? CTI_OK : CTI_ERR_CUDA;
 }
 
 template <typename T, int G>
-int launch_read(const void* pages, const Args& a, void* k, void* v, cudaStream_t s) {
-  const unsigned grid = (unsigned)((a.tokens + kTokens - 1) / kTokens);
-  kv4_read_kernel<T, G><<<grid, kThreads, 0, s>>>(static_cast<const uint8_t*>(pages), a,
-                                                  static_cast<T*>(k), static_cast<T*>(v));
-  return cudaGetLastError() == cudaSuccess ? CTI_OK : CTI_ERR_CUDA;
+int launch_read(const void* pages, Args a, void* k, void* v, cudaStream_t s) {
+  const Launch l = plan(a, G);
+  auto* kernel = l.runs ? kv4_read_runs_kernel<T, G> : kv4_read_tokens_kernel<T, G>;
+  return launch_dependent(kernel, l.grid, dim3(kThreads), 0, s,
+                          static_cast<const uint8_t*>(pages), a, static_cast<T*>(k),
+                          static_cast<T*>(v)) == cudaSuccess
+             ? CTI_OK
+             : CTI_ERR_CUDA;
 }
 
 }  // namespace
@@ -275,7 +668,7 @@ extern "C" int cti_kv4_append(const void* k, const void* v, int64_t k_stride, in
                               void* pages, int64_t num_pages, int32_t* status, void* stream) {
   using namespace cti;
   const Args a = {cu_seqlens, kv_lens,   page_table, table_stride, table_cols, num_seqs,
-                  (int)tokens, kv_heads, num_pages,  k_stride,     v_stride,   status};
+                  (int)tokens, kv_heads, num_pages,  k_stride,     v_stride,   status,   0};
   bool empty;
   const int rc = check_args(k, v, dtype, head_dim, a, tokens, pages, &empty);
   if (rc != CTI_OK || empty) return rc;
@@ -297,7 +690,7 @@ extern "C" int cti_kv4_read(const void* pages, int64_t num_pages, int dtype,
                             void* stream) {
   using namespace cti;
   const Args a = {cu_seqlens, kv_lens,   page_table, table_stride, table_cols, num_seqs,
-                  (int)tokens, kv_heads, num_pages,  k_stride,     v_stride,   status};
+                  (int)tokens, kv_heads, num_pages,  k_stride,     v_stride,   status,   0};
   bool empty;
   const int rc = check_args(k, v, dtype, head_dim, a, tokens, pages, &empty);
   if (rc != CTI_OK || empty) return rc;

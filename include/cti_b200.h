@@ -382,7 +382,8 @@ int cti_ctr_head(const void* h_bf16, const void* W1_bf16, const float* b1, const
 size_t cti_kv4_page_bytes(int kv_heads, int head_dim);
 
 /* Writes the packed tokens' keys and values (views [tokens][kv_heads][head_dim]
- * with token strides in elements, multiples of 8, 16-byte aligned bases). */
+ * with token strides in elements, multiples of 8, at most 2^24; 16-byte
+ * aligned bases). */
 int cti_kv4_append(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int dtype,
                    const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* page_table,
                    int64_t table_stride, int table_cols, int num_seqs, int64_t tokens,

@@ -72,6 +72,14 @@ def test_shapes_and_types_outside_the_kernels(kw):
         assert call(_lib.lib, **kw) == _lib.CTI_ERR_UNSUPPORTED
 
 
+def test_token_strides_past_the_kernels_offsets():
+    from cti_b200 import _lib
+
+    for call in (_append, _read):
+        for kw in (dict(ks=2 ** 24 + 8), dict(vs=2 ** 24 + 8)):
+            assert call(_lib.lib, **kw) == _lib.CTI_ERR_UNSUPPORTED
+
+
 def test_nothing_to_do_is_no_error():
     from cti_b200 import _lib
 
