@@ -6,21 +6,24 @@
 // kv_heads).  One pass with the running maximum and sum of the softmax in
 // fp32; a row that sees no key is zero.
 //
-// A warp takes a tile of up to 16 rows (the query heads of one KV head, token
-// by token) and a range of the sequence's pages.  One bulk copy brings a
+// A warp takes a tile of 8, 16 or 32 rows (the query heads of one KV head,
+// token by token) and a range of the sequence's pages.  One bulk copy brings a
 // page's block of the KV head (2560 G bytes) into the warp's own ring in
-// shared memory; nothing else of the cache is read.  Per page:
-//   S = Q K^T by m16n8k16 matrix instructions with fp32 sums.  A code n is
-//     turned into the 16-bit number 16 + n by a shift and a logic operation,
-//     exactly; the group's scale multiplies the 32-dim partial sums in fp32,
-//     and the bases enter as one more matrix instruction, sum_g b_g sum(q_g),
-//     with the sums of q split into two 16-bit numbers.  So a score is exact
-//     but for fp32 sums and 2^-16 of that term.
-//   P = 2^(S scale log2e - m), against the row's exponent offset m, which is
-//     raised (and O, l rescaled) only when a score exceeds it by 2^8.
-//   O += P V with V = (16 + n) s + b by one 16-bit fused multiply-add per two
-//     values; P and V are rounded to 16 bits once each, as 16-bit attention
-//     does.
+// shared memory; nothing else of the cache is read.  Per page, with keys and
+// head dims as the 16 rows of m16n8k16 matrix instructions and 8 query rows as
+// their columns (a single token has few, and the cache's side is the one that
+// must be unpacked):
+//   S^T = K Q^T with fp32 sums.  A code n is turned into the 16-bit number
+//     16 + n by a shift and a logic operation, exactly; the group's scale
+//     multiplies the 32-dim partial sums in fp32, and the bases enter as one
+//     more matrix instruction, sum_g b_g sum(q_g), with the sums of q split
+//     into two 16-bit numbers.  So a score is exact but for fp32 sums and
+//     2^-16 of that term.
+//   P^T = 2^(S^T scale log2e - m), against the row's exponent offset m, which
+//     is raised (and O, l rescaled) only when a score exceeds it by 2^8.
+//   O^T += V^T P^T with V = (16 + n) s + b by one 16-bit fused multiply-add
+//     per two values; P and V are rounded to 16 bits once each, as 16-bit
+//     attention does.  P^T becomes an operand by a transposition of 8 x 8.
 // The warps of a row tile (1, 2 or 4 of a block) join their O, m and l in
 // shared memory; where a sequence is also split over blocks, they go to the
 // workspace and a second kernel joins them.
@@ -39,8 +42,10 @@ constexpr int kSMs = 148;
 constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
-__host__ __device__ constexpr int stages(int G) { return G == 1 ? 4 : G == 2 ? 3 : 2; }
-__host__ __device__ constexpr int blocks_per_sm(int G) { return G == 1 ? 4 : G == 2 ? 3 : 2; }
+__host__ __device__ constexpr int stages(int G) { return G == 1 ? 3 : 2; }
+__host__ __device__ constexpr int blocks_per_sm(int G, int NT) {
+  return G == 4 || NT == 4 ? 2 : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 5 : 4;
+}
 __host__ __device__ constexpr size_t smem_bytes(int G) {
   return (size_t)kWarps * stages(G) * block_bytes(G) + kWarps * stages(G) * 8;
 }
@@ -60,6 +65,7 @@ struct Args {
   int64_t num_pages;
   int64_t q_stride;
   int warps_per_tile;  // 1, 2 or 4
+  int chunk;           // pages of a sequence for a block (gridDim.z > 1)
   float* ws_o;         // [splits][tokens * heads][D]; splits > 1 only
   float2* ws_ml;       // [splits][tokens * heads]
   int32_t* status;
@@ -98,16 +104,23 @@ CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* 
       : "memory");
 }
 
-template <typename T, int G, int ROWS>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(G))
+// Transposes an 8 x 8 matrix of 16-bit values, two to a register.
+CTI_DEVICE uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T, int G, int NT>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     kv4_attention_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pages, const Args a,
                          T* __restrict__ out) {
   using Y = Type16<T>;
   using M = Mma<T>;
   constexpr int D = 32 * G;
+  constexpr int ROWS = 8 * NT;
   constexpr int S = stages(G);
   constexpr int kBlock = block_bytes(G);
-  constexpr bool kTwo = ROWS == 16;  // rows 8..15 are in use
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = warp_id(), lane = lane_id();
   const int r8 = lane >> 2, t4 = lane & 3;
@@ -121,24 +134,24 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G))
   grid_dependency_wait();
 
   const int wpt = a.warps_per_tile;
-  const int64_t unit = (int64_t)blockIdx.x * (kWarps / wpt) + warp / wpt;
-  if (unit >= (int64_t)a.num_seqs * a.kv_heads) return;  // all warps of a tile alike
+  const unsigned unit = blockIdx.x * (kWarps / wpt) + warp / wpt;
+  if (unit >= (unsigned)a.num_seqs * a.kv_heads) return;  // all warps of a tile alike
   const int sub = warp & (wpt - 1);
-  const int s = (int)(unit / a.kv_heads), kvh = (int)(unit % a.kv_heads);
+  const int s = (int)(unit / (unsigned)a.kv_heads), kvh = (int)(unit - s * (unsigned)a.kv_heads);
   const int group = a.heads / a.kv_heads;
-  int64_t begin = __ldg(a.cu + s), end = __ldg(a.cu + s + 1);
-  const int64_t len = __ldg(a.kv_lens + s);
-  const int64_t n_given = end - begin;
-  const int64_t first = len - n_given;  // position of the first new token
-  if (begin < 0 || end > a.tokens || n_given < 0) {
+  const int begin = __ldg(a.cu + s), end = __ldg(a.cu + s + 1);
+  const int len = __ldg(a.kv_lens + s);
+  if (begin < 0 || end > a.tokens || end < begin) {
     if (lane == 0) raise_status(a.status, CTI_ERR_INVALID_ARG, s);
     return;
   }
-  const int64_t rows = n_given * group;
-  int64_t limit = len;  // keys that the table reaches
-  if (limit > (int64_t)a.table_cols * kPage || (limit > 0 && a.num_pages <= 0)) {
+  const int n_new = end - begin;
+  const int first = max(len, 0) - n_new;  // position of the first new token
+  const int rows = n_new * group;         // tokens * heads is below 2^31
+  int limit = max(len, 0);                // keys that the table reaches
+  if (limit > a.table_cols * kPage || (limit > 0 && a.num_pages <= 0)) {
     if (lane == 0 && rows > 0) raise_status(a.status, CTI_ERR_BOUNDS, s);
-    limit = a.num_pages <= 0 ? 0 : (int64_t)a.table_cols * kPage;
+    limit = a.num_pages <= 0 ? 0 : a.table_cols * kPage;
   }
   const int32_t* table = a.table + s * a.table_stride;
   const uint8_t* base = pages + (int64_t)kvh * kBlock;
@@ -147,84 +160,35 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G))
   uint32_t count = 0;  // pages copied so far: stage and parity
   bool dead = false;   // a copy did not arrive in time
 
-  for (int64_t tile = blockIdx.y; tile * ROWS < rows; tile += gridDim.y) {
-    // ---- rows: queries, keys that each sees ----
-    int64_t row_at[2];  // output row (token * heads + head), -1: none
-    int64_t sees[2];    // keys
-    uint32_t qa[G][2][4];
-    uint32_t off_a[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int64_t r = tile * ROWS + r8 + 8 * e;
-      const bool live = (e == 0 || kTwo) && r < rows;
-      const int64_t i = live ? r / group : 0;
-      const int h = kvh * group + (int)(r - i * group);
-      row_at[e] = live ? (begin + i) * a.heads + h : -1;
-      sees[e] = live ? (a.causal ? min(first + i + 1, limit) : limit) : 0;
-      float sum_mine = 0.0f;  // of group t4's 32 dims (G = 2: t4 & 1; G = 1: the only one)
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live)
-          v = __ldg(reinterpret_cast<const uint4*>(q + (begin + i) * a.q_stride + (int64_t)h * D +
-                                                   32 * g + 8 * t4));
-        if (a.negate) {
-          v.x ^= 0x80008000u;
-          v.y ^= 0x80008000u;
-          v.z ^= 0x80008000u;
-          v.w ^= 0x80008000u;
-        }
-        qa[g][0][e] = v.x;
-        qa[g][0][2 + e] = v.y;
-        qa[g][1][e] = v.z;
-        qa[g][1][2 + e] = v.w;
-        float sum = Y::low(v.x) + Y::high(v.x) + Y::low(v.y) + Y::high(v.y) + Y::low(v.z) +
-                    Y::high(v.z) + Y::low(v.w) + Y::high(v.w);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (g == (t4 & (G - 1))) sum_mine = sum;
-      }
-      // The bases' operand: column 2 t + 1 multiplies b of the group that the
-      // matching word of K's meta holds; column 2 t (its scale) gets 0.
-      const uint32_t hi = Y::bits(sum_mine);
-      const uint32_t lo = Y::bits(sum_mine - Y::to_float(hi));
-      if (G == 4) {
-        off_a[e] = hi << 16;
-        off_a[2 + e] = lo << 16;
-      } else {
-        off_a[e] = t4 < G ? hi << 16 : t4 < 2 * G ? lo << 16 : 0u;
-      }
-    }
+  for (int tile = blockIdx.y; tile < (rows + ROWS - 1) / ROWS; tile += gridDim.y) {
     // Keys that some row and that every row of the tile sees.
-    const int64_t r_last = min(rows, (tile + 1) * ROWS) - 1;
-    const int64_t most =
-        max(a.causal ? min(first + r_last / group + 1, limit) : limit, (int64_t)0);
-    const int64_t all = a.causal ? min(first + tile * ROWS / group + 1, limit) : limit;
-
-    float o[4 * G][4];
-#pragma unroll
-    for (int i = 0; i < 4 * G; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const int row0 = tile * ROWS, row_last = min(rows, row0 + ROWS) - 1;
+    const int most =
+        max(a.causal ? min(first + (int)((unsigned)row_last / group) + 1, limit) : limit, 0);
+    const int all = a.causal ? min(first + (int)((unsigned)row0 / group) + 1, limit) : limit;
 
     // ---- this warp's pages ----
-    const int64_t npages = (most + kPage - 1) / kPage;
-    const int workers = gridDim.z * wpt;
-    const int64_t per = (npages + workers - 1) / workers;
-    const int64_t p0 = min(npages, per * (blockIdx.z * wpt + sub));
-    const int np = dead ? 0 : (int)(min(npages, p0 + per) - p0);
+    int p0 = 0, np = (most + kPage - 1) / kPage;
+    if (gridDim.z > 1) {  // the last block takes what the caller's bound left out
+      p0 = min(np, (int)blockIdx.z * a.chunk);
+      np = (blockIdx.z == gridDim.z - 1 ? np : min(np, p0 + a.chunk)) - p0;
+    }
+    if (wpt > 1) {
+      const int per = (np + wpt - 1) / wpt, skip = min(np, sub * per);
+      p0 += skip;
+      np = min(np - skip, per);
+    }
+    if (dead) np = 0;
     int ids = -1;  // lane i: page p0 + (chunk of 32) + i
-    auto load_ids = [&](int i) {
-      ids = i + lane < np ? __ldg(table + p0 + i + lane) : 0;
-      if (ids < 0 || ids >= a.num_pages) {
-        raise_status(a.status, CTI_ERR_BOUNDS, s);
-        ids = -1;
-      }
-    };
-    uint32_t bad = 0;  // bit per page in flight (by stage): not a page, nothing of it is seen
+    uint32_t bad = 0;  // bit per stage: not a page, nothing of it is seen
     auto issue = [&](int i) {  // page i of the range into its stage
-      if ((i & 31) == 0) load_ids(i);
+      if ((i & 31) == 0) {
+        ids = i + lane < np ? __ldg(table + p0 + i + lane) : 0;
+        if (ids < 0 || ids >= a.num_pages) {
+          raise_status(a.status, CTI_ERR_BOUNDS, s);
+          ids = -1;
+        }
+      }
       int id = __shfl_sync(0xffffffffu, ids, i & 31);
       const uint32_t st = (count + i) % S;
       bad = id < 0 ? bad | 1u << st : bad & ~(1u << st);
@@ -236,6 +200,64 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G))
     };
     for (int i = 0; i < S && i < np; ++i) issue(i);
 
+    // ---- queries: lane 4 r + t has dims 8 t .. + 7 of every group of row r ----
+    uint32_t qb[NT][G][4];
+    uint32_t off_b[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + 8 * n + r8;
+      const int i = (int)((unsigned)row / group), h = kvh * group + row - i * group;
+      float sum_mine = 0.0f;  // of group t4's 32 dims (G = 2: t4 & 1; G = 1: the only one)
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < rows)
+          v = __ldg(reinterpret_cast<const uint4*>(q + (begin + i) * a.q_stride + (int64_t)h * D +
+                                                   32 * g + 8 * t4));
+        if (a.negate) {
+          v.x ^= 0x80008000u;
+          v.y ^= 0x80008000u;
+          v.z ^= 0x80008000u;
+          v.w ^= 0x80008000u;
+        }
+        qb[n][g][0] = v.x;
+        qb[n][g][1] = v.y;
+        qb[n][g][2] = v.z;
+        qb[n][g][3] = v.w;
+        float sum = Y::low(v.x) + Y::high(v.x) + Y::low(v.y) + Y::high(v.y) + Y::low(v.z) +
+                    Y::high(v.z) + Y::low(v.w) + Y::high(v.w);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (g == (t4 & (G - 1))) sum_mine = sum;
+      }
+      // The bases' operand: the row that meets b of a group is the sum of q in
+      // it, in two parts; the one that meets its scale is 0.
+      const uint32_t hi = Y::bits(sum_mine);
+      const uint32_t lo = Y::bits(sum_mine - Y::to_float(hi));
+      off_b[n][0] = G == 4 || t4 < G ? hi << 16 : t4 < 2 * G ? lo << 16 : 0u;
+      off_b[n][1] = G == 4 ? lo << 16 : 0u;
+    }
+    int sees[NT][2];  // keys that rows 2 t and 2 t + 1 see
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = min(row0 + 8 * n + 2 * t4 + e, row_last);
+        sees[n][e] = a.causal ? min(first + (int)((unsigned)row / group) + 1, limit) : limit;
+      }
+
+    float o[NT][2 * G][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
+    }
+
     int done = 0;
     for (; done < np; ++done) {
       const uint32_t st = (count + done) % S;
@@ -243,133 +265,216 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G))
                                              nullptr)))
         break;
       uint8_t* blk = ring + st * kBlock;
-      const int64_t key0 = (p0 + done) * kPage;
-      const bool is_bad = (bad >> st) & 1;
-      const bool whole = !is_bad && key0 + kPage <= all;
 
-      // ---- S = Q K^T ----
-      float sc[8][4];
+      // ---- S^T = K Q^T, 16 keys at a time ----
+      float sc[NT][4][4];
 #pragma unroll
-      for (int v = 0; v < 2 * G; ++v) {
-        const uint4 w4 = *reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      for (int mt = 0; mt < 4; ++mt) {
+        uint32_t w[2][G];  // of tokens 16 mt + r and + 8
+        uint32_t meta[2][G];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int nt = (4 * v + j) / G, g = (4 * v + j) % G;
-          if (g == 0) {
-            const uint32_t meta = *reinterpret_cast<const uint32_t*>(
-                blk + k_meta_at(G) + ((8 * nt + r8) * G + (t4 & (G - 1))) * 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[nt][e] = 0.0f;
-            M::run(sc[nt], off_a, meta, G == 4 ? meta : 0u);
+        for (int e = 0; e < 2; ++e) {
+          const int nt = 2 * mt + e;
+          const uint32_t* cw = reinterpret_cast<const uint32_t*>(
+              blk + ((nt * G >> 2) * 32 + lane) * 16 + (nt * G & 3) * 4);
+          const uint32_t* mw =
+              reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) + (8 * nt + r8) * G;
+          if (G == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(cw);
+            w[e][0] = x.x, w[e][G > 1 ? 1 : 0] = x.y, w[e][G > 2 ? 2 : 0] = x.z, w[e][G - 1] = x.w;
+            const uint4 y = *reinterpret_cast<const uint4*>(mw);
+            meta[e][0] = y.x, meta[e][G > 1 ? 1 : 0] = y.y, meta[e][G > 2 ? 2 : 0] = y.z,
+            meta[e][G - 1] = y.w;
+          } else if (G == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(cw);
+            w[e][0] = x.x, w[e][G - 1] = x.y;
+            const uint2 y = *reinterpret_cast<const uint2*>(mw);
+            meta[e][0] = y.x, meta[e][G - 1] = y.y;
+          } else {
+            w[e][0] = *cw;
+            meta[e][0] = *mw;
           }
-          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          M::run(c, qa[g][0], k_pair<T>(w[j], 0), k_pair<T>(w[j], 1));
-          M::run(c, qa[g][1], k_pair<T>(w[j], 2), k_pair<T>(w[j], 3));
-          const uint32_t* mc = reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) +
-                               (8 * nt + 2 * t4) * G + g;
-          const float s0 = Y::low(mc[0]), s1 = Y::low(mc[G]);
-          sc[nt][0] = fmaf(c[0], s0, sc[nt][0]);
-          sc[nt][1] = fmaf(c[1], s1, sc[nt][1]);
-          if (kTwo) {
-            sc[nt][2] = fmaf(c[2], s0, sc[nt][2]);
-            sc[nt][3] = fmaf(c[3], s1, sc[nt][3]);
+        }
+        // Each lane's own group of the meta for the bases.
+        uint32_t am[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          am[e] = G == 1 ? meta[e][0]
+                         : *(reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) +
+                             (16 * mt + 8 * e + r8) * G + (t4 & (G - 1)));
+        const uint32_t off_a[4] = {am[0], am[1], G == 4 ? am[0] : 0u, G == 4 ? am[1] : 0u};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[n][mt][e] = 0.0f;
+          M::run(sc[n][mt], off_a, off_b[n][0], off_b[n][1]);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint32_t a0[4] = {k_pair<T>(w[0][g], 0), k_pair<T>(w[1][g], 0),
+                                  k_pair<T>(w[0][g], 1), k_pair<T>(w[1][g], 1)};
+          const uint32_t a1[4] = {k_pair<T>(w[0][g], 2), k_pair<T>(w[1][g], 2),
+                                  k_pair<T>(w[0][g], 3), k_pair<T>(w[1][g], 3)};
+          const float s0 = Y::low(meta[0][g]), s1 = Y::low(meta[1][g]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            M::run(c, a0, qb[n][g][0], qb[n][g][1]);
+            M::run(c, a1, qb[n][g][2], qb[n][g][3]);
+            sc[n][mt][0] = fmaf(c[0], s0, sc[n][mt][0]);
+            sc[n][mt][1] = fmaf(c[1], s0, sc[n][mt][1]);
+            sc[n][mt][2] = fmaf(c[2], s1, sc[n][mt][2]);
+            sc[n][mt][3] = fmaf(c[3], s1, sc[n][mt][3]);
           }
         }
       }
 
-      if (!whole) {
-        // Keys that a row does not see count nothing, whatever they hold.  A
-        // value that is not finite must reach only the rows that see it: its
-        // scores become NaN for them, and its meta zero for all.
-        const int64_t lim0 = is_bad ? 0 : sees[0] - key0, lim1 = is_bad ? 0 : sees[1] - key0;
-        const int64_t lim_most = is_bad ? 0 : most - key0;
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-          const int tau = 8 * nt + 2 * t4;
-          uint32_t* vm = reinterpret_cast<uint32_t*>(blk + v_meta_at(G)) + (4 * nt + t4) * 2 * G;
-          bool nan0 = false, nan1 = false;
+      const int key0 = (p0 + done) * kPage;
+      const bool is_bad = (bad >> st) & 1;
+      if (is_bad || key0 + kPage > all) {
+        // Keys that a row does not see count nothing, whatever they hold: a
+        // value behind the last key gets a meta of zero.  One that is not
+        // finite and that only some rows see gets the same, and a score of NaN
+        // for those that do.
+        const int lim_most = is_bad ? 0 : most - key0;
+        uint32_t* vm = reinterpret_cast<uint32_t*>(blk + v_meta_at(G)) + lane * 2 * G;
+        bool nan0 = false, nan1 = false;  // of tokens 2 lane and 2 lane + 1
+        if (all < most) {
 #pragma unroll
           for (int i = 0; i < 2 * G; ++i) {
             nan0 |= (vm[i] & M::kInf) == M::kInf;
             nan1 |= ((vm[i] >> 16) & M::kInf) == M::kInf;
           }
-          __syncwarp();
-          if (nan0 || tau >= lim_most)
-            for (int i = 0; i < 2 * G; ++i) vm[i] &= 0xffff0000u;
-          if (nan1 || tau + 1 >= lim_most)
-            for (int i = 0; i < 2 * G; ++i) vm[i] &= 0x0000ffffu;
-          if (nan0) sc[nt][0] = sc[nt][2] = NAN;
-          if (nan1) sc[nt][1] = sc[nt][3] = NAN;
-          if (tau >= lim0) sc[nt][0] = -INFINITY;
-          if (tau + 1 >= lim0) sc[nt][1] = -INFINITY;
-          if (tau >= lim1) sc[nt][2] = -INFINITY;
-          if (tau + 1 >= lim1) sc[nt][3] = -INFINITY;
+        }
+        const uint32_t keep = (nan0 || 2 * lane >= lim_most ? 0u : 0xffffu) |
+                              (nan1 || 2 * lane + 1 >= lim_most ? 0u : 0xffff0000u);
+        if (keep != 0xffffffffu) {
+#pragma unroll
+          for (int i = 0; i < 2 * G; ++i) vm[i] &= keep;
+        }
+        const uint32_t even = __ballot_sync(0xffffffffu, nan0);
+        const uint32_t odd = __ballot_sync(0xffffffffu, nan1);
+        if (even | odd) {
+          const uint32_t mine = r8 & 1 ? odd : even;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+              if (mine >> (8 * mt + (r8 >> 1)) & 1) sc[n][mt][0] = sc[n][mt][1] = NAN;
+              if (mine >> (8 * mt + 4 + (r8 >> 1)) & 1) sc[n][mt][2] = sc[n][mt][3] = NAN;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int lim0 = (is_bad ? 0 : sees[n][0] - key0) - r8;
+          const int lim1 = (is_bad ? 0 : sees[n][1] - key0) - r8;
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            if (16 * mt >= lim0) sc[n][mt][0] = -INFINITY;
+            if (16 * mt >= lim1) sc[n][mt][1] = -INFINITY;
+            if (16 * mt + 8 >= lim0) sc[n][mt][2] = -INFINITY;
+            if (16 * mt + 8 >= lim1) sc[n][mt][3] = -INFINITY;
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
       }
 
       // ---- the rows' exponent offsets ----
-      float mx[2] = {-INFINITY, -INFINITY};
+      float mx[NT][2];
+      bool raise = false;
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        mx[0] = fmaxf(mx[0], fmaxf(sc[nt][0], sc[nt][1]));
-        if (kTwo) mx[1] = fmaxf(mx[1], fmaxf(sc[nt][2], sc[nt][3]));
-      }
-      const bool raise = (mx[0] - m[0]) * sl > kSlack || (kTwo && (mx[1] - m[1]) * sl > kSlack);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(sc[n][0][e], sc[n][0][2 + e]);
+#pragma unroll
+          for (int mt = 1; mt < 4; ++mt) x = fmaxf(x, fmaxf(sc[n][mt][e], sc[n][mt][2 + e]));
+          mx[n][e] = x;
+          raise = raise || (x - m[n][e]) * sl > kSlack;
+        }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int e = 0; e < (kTwo ? 2 : 1); ++e) {
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-          if (mx[e] > m[e]) {
-            const float corr = ex2_approx((m[e] - mx[e]) * sl);
-            m[e] = mx[e];
-            l[e] *= corr;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4 * G; ++i) {
-              o[i][2 * e] *= corr;
-              o[i][2 * e + 1] *= corr;
+          for (int e = 0; e < 2; ++e) {
+            float x = mx[n][e];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            if (x > m[n][e]) {
+              const float corr = ex2_approx((m[n][e] - x) * sl);
+              m[n][e] = x;
+              l[n][e] *= corr;
+#pragma unroll
+              for (int i = 0; i < 2 * G; ++i) {
+                o[n][i][e] *= corr;
+                o[n][i][2 + e] *= corr;
+              }
+            }
+          }
+      }
+
+      // ---- P^T, and O^T += V^T P^T, 16 keys at a time ----
+      float noff[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) noff[n][e] = m[n][e] == -INFINITY ? 0.0f : -m[n][e] * sl;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float(&x)[4] = sc[n][kk];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = ex2_approx(fmaf(x[e], sl, noff[n][e & 1]));
+          l[n][0] += x[0] + x[2];
+          l[n][1] += x[1] + x[3];
+          pb[n][0] = transpose8(Y::pack(x[0], x[1]));
+          pb[n][1] = transpose8(Y::pack(x[2], x[3]));
+        }
+        uint32_t w[2][G];
+        uint2 meta[2][G];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int nt = 2 * kk + e;
+          const uint32_t* cw = reinterpret_cast<const uint32_t*>(
+              blk + v_codes_at(G) + ((nt * G >> 2) * 32 + lane) * 16 + (nt * G & 3) * 4);
+          const uint2* mw =
+              reinterpret_cast<const uint2*>(blk + v_meta_at(G)) + (4 * nt + t4) * G;
+          if (G == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(cw);
+            w[e][0] = x.x, w[e][G > 1 ? 1 : 0] = x.y, w[e][G > 2 ? 2 : 0] = x.z, w[e][G - 1] = x.w;
+          } else if (G == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(cw);
+            w[e][0] = x.x, w[e][G - 1] = x.y;
+          } else {
+            w[e][0] = *cw;
+          }
+          if (G == 1) {
+            meta[e][0] = *mw;
+          } else {
+#pragma unroll
+            for (int g = 0; g < G; g += 2) {
+              const uint4 y = *reinterpret_cast<const uint4*>(mw + g);
+              meta[e][g] = make_uint2(y.x, y.y);
+              meta[e][g + (G > 1 ? 1 : 0)] = make_uint2(y.z, y.w);
             }
           }
         }
-      }
-      const float off0 = m[0] == -INFINITY ? 0.0f : m[0] * sl;
-      const float off1 = m[1] == -INFINITY ? 0.0f : m[1] * sl;
-
-      // ---- P, and O += P V, 16 keys at a time ----
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t pa[4] = {0, 0, 0, 0};
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          float(&x)[4] = sc[2 * kk + hh];
-          x[0] = ex2_approx(fmaf(x[0], sl, -off0));
-          x[1] = ex2_approx(fmaf(x[1], sl, -off0));
-          l[0] += x[0] + x[1];
-          pa[2 * hh] = Y::pack(x[0], x[1]);
-          if (kTwo) {
-            x[2] = ex2_approx(fmaf(x[2], sl, -off1));
-            x[3] = ex2_approx(fmaf(x[3], sl, -off1));
-            l[1] += x[2] + x[3];
-            pa[2 * hh + 1] = Y::pack(x[2], x[3]);
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t av[4] = {
+                fma2<T>(v_pair<T>(w[0][g], 2 * j), meta[0][g].x, meta[0][g].y),
+                fma2<T>(v_pair<T>(w[0][g], 2 * j + 1), meta[0][g].x, meta[0][g].y),
+                fma2<T>(v_pair<T>(w[1][g], 2 * j), meta[1][g].x, meta[1][g].y),
+                fma2<T>(v_pair<T>(w[1][g], 2 * j + 1), meta[1][g].x, meta[1][g].y)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) M::run(o[n][2 * g + j], av, pb[n][0], pb[n][1]);
           }
-        }
-        const uint2* vm = reinterpret_cast<const uint2*>(blk + v_meta_at(G)) + (8 * kk + t4) * G;
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const uint2 m0 = vm[g], m1 = vm[4 * G + g];
-          const int i0 = 2 * kk * G + g, i1 = i0 + G;
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(
-              blk + v_codes_at(G) + ((i0 >> 2) * 32 + lane) * 16 + (i0 & 3) * 4);
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(
-              blk + v_codes_at(G) + ((i1 >> 2) * 32 + lane) * 16 + (i1 & 3) * 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            M::run(o[4 * g + j], pa, fma2<T>(v_pair<T>(w0, j), m0.x, m0.y),
-                   fma2<T>(v_pair<T>(w1, j), m1.x, m1.y));
-        }
       }
       __syncwarp();
       if (done + S < np) issue(done + S);
@@ -381,95 +486,92 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G))
     }
     count += np;
 
-    // ---- join and store ----
+    // ---- join and store: lane 4 r + t has dims 4 r .. + 3 of every group ----
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+      }
     if (wpt > 1) {
       // Every warp's rows in its own ring, then the first warp adds them up.
-      const int bar = 1 + warp / wpt;
       float* mine = reinterpret_cast<float*>(ring);
-      float* ml = mine + ROWS * D;
       static_assert((ROWS * D + 2 * ROWS) * 4 <= S * kBlock, "room for the rows");
       __syncwarp();
       if (sub != 0) {
 #pragma unroll
-        for (int e = 0; e < (kTwo ? 2 : 1); ++e) {
-          float* dst = mine + (r8 + 8 * e) * D + 8 * t4;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            float4* d4 = reinterpret_cast<float4*>(dst + 32 * g);
-            d4[0] = make_float4(o[4 * g][2 * e], o[4 * g + 1][2 * e], o[4 * g + 2][2 * e],
-                                o[4 * g + 3][2 * e]);
-            d4[1] = make_float4(o[4 * g][2 * e + 1], o[4 * g + 1][2 * e + 1],
-                                o[4 * g + 2][2 * e + 1], o[4 * g + 3][2 * e + 1]);
+          for (int e = 0; e < 2; ++e) {
+            const int row = 8 * n + 2 * t4 + e;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+              *reinterpret_cast<float4*>(mine + row * D + 32 * g + 4 * r8) =
+                  make_float4(o[n][2 * g][e], o[n][2 * g][2 + e], o[n][2 * g + 1][e],
+                              o[n][2 * g + 1][2 + e]);
+            if (r8 == 0)
+              *reinterpret_cast<float2*>(mine + ROWS * D + 2 * row) =
+                  make_float2(m[n][e], l[n][e]);
           }
-          if (t4 == 0) {
-            ml[2 * (r8 + 8 * e)] = m[e];
-            ml[2 * (r8 + 8 * e) + 1] = l[e];
-          }
-        }
       }
-      named_barrier_sync(bar, 32 * wpt);
+      named_barrier_sync(1 + warp / wpt, 32 * wpt);
       if (sub == 0) {
         for (int w = 1; w < wpt; ++w) {
           const float* src = reinterpret_cast<const float*>(ring + (size_t)w * S * kBlock);
-          const float* src_ml = src + ROWS * D;
 #pragma unroll
-          for (int e = 0; e < (kTwo ? 2 : 1); ++e) {
-            const float mw = src_ml[2 * (r8 + 8 * e)], lw = src_ml[2 * (r8 + 8 * e) + 1];
-            const float mm = fmaxf(m[e], mw);
-            const float ca = m[e] == mm ? 1.0f : ex2_approx((m[e] - mm) * sl);
-            const float cb = mw == mm ? 1.0f : ex2_approx((mw - mm) * sl);
-            m[e] = mm;
-            l[e] = l[e] * ca + lw * cb;
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              const float4* s4 =
-                  reinterpret_cast<const float4*>(src + (r8 + 8 * e) * D + 32 * g + 8 * t4);
-              const float4 x = s4[0], y = s4[1];
-              o[4 * g][2 * e] = o[4 * g][2 * e] * ca + x.x * cb;
-              o[4 * g + 1][2 * e] = o[4 * g + 1][2 * e] * ca + x.y * cb;
-              o[4 * g + 2][2 * e] = o[4 * g + 2][2 * e] * ca + x.z * cb;
-              o[4 * g + 3][2 * e] = o[4 * g + 3][2 * e] * ca + x.w * cb;
-              o[4 * g][2 * e + 1] = o[4 * g][2 * e + 1] * ca + y.x * cb;
-              o[4 * g + 1][2 * e + 1] = o[4 * g + 1][2 * e + 1] * ca + y.y * cb;
-              o[4 * g + 2][2 * e + 1] = o[4 * g + 2][2 * e + 1] * ca + y.z * cb;
-              o[4 * g + 3][2 * e + 1] = o[4 * g + 3][2 * e + 1] * ca + y.w * cb;
+            for (int e = 0; e < 2; ++e) {
+              const int row = 8 * n + 2 * t4 + e;
+              const float2 ml = *reinterpret_cast<const float2*>(src + ROWS * D + 2 * row);
+              const float mm = fmaxf(m[n][e], ml.x);
+              const float ca = m[n][e] == mm ? 1.0f : ex2_approx((m[n][e] - mm) * sl);
+              const float cb = ml.x == mm ? 1.0f : ex2_approx((ml.x - mm) * sl);
+              m[n][e] = mm;
+              l[n][e] = l[n][e] * ca + ml.y * cb;
+#pragma unroll
+              for (int g = 0; g < G; ++g) {
+                const float4 x =
+                    *reinterpret_cast<const float4*>(src + row * D + 32 * g + 4 * r8);
+                o[n][2 * g][e] = o[n][2 * g][e] * ca + x.x * cb;
+                o[n][2 * g][2 + e] = o[n][2 * g][2 + e] * ca + x.y * cb;
+                o[n][2 * g + 1][e] = o[n][2 * g + 1][e] * ca + x.z * cb;
+                o[n][2 * g + 1][2 + e] = o[n][2 * g + 1][2 + e] * ca + x.w * cb;
+              }
             }
-          }
         }
       }
     }
     if (sub == 0) {
 #pragma unroll
-      for (int e = 0; e < (kTwo ? 2 : 1); ++e) {
-        if (row_at[e] < 0) continue;
-        if (gridDim.z == 1) {
-          const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
-          uint4* dst = reinterpret_cast<uint4*>(out + row_at[e] * D + 8 * t4);
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int g = 0; g < G; ++g)
-            dst[4 * g] = make_uint4(
-                Y::pack(o[4 * g][2 * e] * inv, o[4 * g + 1][2 * e] * inv),
-                Y::pack(o[4 * g + 2][2 * e] * inv, o[4 * g + 3][2 * e] * inv),
-                Y::pack(o[4 * g][2 * e + 1] * inv, o[4 * g + 1][2 * e + 1] * inv),
-                Y::pack(o[4 * g + 2][2 * e + 1] * inv, o[4 * g + 3][2 * e + 1] * inv));
-        } else {
-          const int64_t at = (int64_t)blockIdx.z * a.tokens * a.heads + row_at[e];
-          float4* dst = reinterpret_cast<float4*>(a.ws_o + at * D + 8 * t4);
+        for (int e = 0; e < 2; ++e) {
+          const int row = row0 + 8 * n + 2 * t4 + e;
+          if (row >= rows) continue;
+          const int i = (int)((unsigned)row / group);
+          const int64_t at = (int64_t)(begin + i) * a.heads + kvh * group + row - i * group;
+          if (gridDim.z == 1) {
+            const float inv = l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e];
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            dst[8 * g] = make_float4(o[4 * g][2 * e], o[4 * g + 1][2 * e], o[4 * g + 2][2 * e],
-                                     o[4 * g + 3][2 * e]);
-            dst[8 * g + 1] = make_float4(o[4 * g][2 * e + 1], o[4 * g + 1][2 * e + 1],
-                                         o[4 * g + 2][2 * e + 1], o[4 * g + 3][2 * e + 1]);
+            for (int g = 0; g < G; ++g)
+              *reinterpret_cast<uint2*>(out + at * D + 32 * g + 4 * r8) =
+                  make_uint2(Y::pack(o[n][2 * g][e] * inv, o[n][2 * g][2 + e] * inv),
+                             Y::pack(o[n][2 * g + 1][e] * inv, o[n][2 * g + 1][2 + e] * inv));
+          } else {
+            const int64_t ws = (int64_t)blockIdx.z * a.tokens * a.heads + at;
+            if (r8 == 0) a.ws_ml[ws] = make_float2(m[n][e], l[n][e]);
+            if (np > 0 || wpt > 1) {  // else the row is empty, and not read
+#pragma unroll
+              for (int g = 0; g < G; ++g)
+                *reinterpret_cast<float4*>(a.ws_o + ws * D + 32 * g + 4 * r8) =
+                    make_float4(o[n][2 * g][e], o[n][2 * g][2 + e], o[n][2 * g + 1][e],
+                                o[n][2 * g + 1][2 + e]);
+            }
           }
-          if (t4 == 0) a.ws_ml[at] = make_float2(m[e], l[e]);
         }
-      }
     }
     if (wpt > 1) {
       // The rings are free again (copies may overwrite them) once the first
@@ -503,6 +605,7 @@ __global__ void __launch_bounds__(128)
 #pragma unroll 4
   for (int z = 0; z < splits; ++z) {
     const float2 ml = a.ws_ml[z * rows + row];
+    if (ml.y == 0.0f) continue;  // no key of the split is seen
     const float w = ml.x == mm ? 1.0f : ex2_approx((ml.x - mm) * a.scale_log2);
     l = fmaf(ml.y, w, l);
 #pragma unroll
@@ -517,9 +620,9 @@ __global__ void __launch_bounds__(128)
 
 // How a call is laid out over the GPU; a function of the sizes alone.
 struct Plan {
-  int rows;            // rows of a tile
+  int row_tiles;       // of 8 rows, that a warp takes: 1, 2 or 4
   int warps_per_tile;  // that share a tile's pages in a block
-  int splits;          // blocks that share them
+  int splits, chunk;   // blocks that share them, and the pages of each
   int64_t tiles;       // row tiles of a sequence
 };
 
@@ -529,17 +632,31 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   const int64_t most = max_new < tokens ? max_new : tokens;
   const int64_t rows = (most > 0 ? most : 1) * (heads / kv_heads);
   Plan p;
-  p.rows = rows <= 8 ? 8 : 16;
-  p.tiles = (rows + p.rows - 1) / p.rows;
+  p.row_tiles = rows <= 8 ? 1 : rows <= 16 || G == 4 ? 2 : 4;
+  p.tiles = (rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
   const double units = (double)num_seqs * kv_heads * (double)p.tiles;
-  const int64_t pages = (max_kv_len + kPage - 1) / kPage;
-  // Warps that run at once; a tile is shared by as many as leave none idle.
-  const int64_t room = (int64_t)kSMs * blocks_per_sm(G) * kWarps;
-  int64_t share = (int64_t)(room / units);
-  share = share < 1 ? 1 : share > pages ? (pages > 0 ? pages : 1) : share;
-  p.warps_per_tile = share >= 4 ? 4 : share >= 2 ? 2 : 1;
-  p.splits = (int)(share / p.warps_per_tile);
-  if (p.splits > 256) p.splits = 256;
+  const int64_t pages = max_kv_len > 0 ? (max_kv_len + kPage - 1) / kPage : 1;
+  const double room = (double)kSMs * blocks_per_sm(G, p.row_tiles) * kWarps;  // warps at once
+  p.splits = 1;
+  p.chunk = 0;
+  if (units >= room && pages <= 8) {
+    // Short sequences, more tiles than warps: a warp each.
+    p.warps_per_tile = 1;
+    return p;
+  }
+  // A block's warps share a tile; with long sequences, blocks do too, so that
+  // all run at once, or, where that is more than 16 pages for a warp, in
+  // pieces of 12, small enough that sequences of any lengths balance out.
+  p.warps_per_tile = pages >= 4 ? 4 : pages >= 2 ? 2 : 1;
+  const double ideal = units * pages / room;
+  int64_t per_warp = ideal > 16 ? 12 : (int64_t)ideal + 1;
+  p.chunk = (int)(per_warp * p.warps_per_tile);
+  int64_t splits = (pages + p.chunk - 1) / p.chunk;
+  if (splits > 128) {
+    splits = 128;
+    p.chunk = (int)((pages + splits - 1) / splits);
+  }
+  p.splits = (int)splits;
   return p;
 }
 
@@ -549,25 +666,23 @@ size_t workspace_o_bytes(const Plan& p, int64_t tokens, int heads, int head_dim)
   return p.splits > 1 ? align256((size_t)p.splits * tokens * heads * head_dim * sizeof(float)) : 0;
 }
 
-template <typename T, int G, int ROWS>
+template <typename T, int G, int NT>
 int launch(const void* q, const void* pages, const Args& a, const Plan& p, void* out,
            cudaStream_t s) {
   static uint64_t configured = 0;
-  if (ensure_smem_limit(kv4_attention_kernel<T, G, ROWS>, (int)smem_bytes(G), configured) !=
+  if (ensure_smem_limit(kv4_attention_kernel<T, G, NT>, (int)smem_bytes(G), configured) !=
       cudaSuccess)
     return CTI_ERR_CUDA;
   const int64_t units = (int64_t)a.num_seqs * a.kv_heads;
   const int per = kWarps / p.warps_per_tile;
-  const int64_t x = (units + per - 1) / per;
-  if (x > INT32_MAX) return CTI_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)x, (unsigned)(p.tiles < 65535 ? p.tiles : 65535), (unsigned)p.splits);
-  if (launch_dependent(kv4_attention_kernel<T, G, ROWS>, grid, dim3(kThreads), smem_bytes(G), s,
+  const dim3 grid((unsigned)((units + per - 1) / per),
+                  (unsigned)(p.tiles < 65535 ? p.tiles : 65535), (unsigned)p.splits);
+  if (launch_dependent(kv4_attention_kernel<T, G, NT>, grid, dim3(kThreads), smem_bytes(G), s,
                        static_cast<const T*>(q), static_cast<const uint8_t*>(pages), a,
                        static_cast<T*>(out)) != cudaSuccess)
     return CTI_ERR_CUDA;
   if (p.splits > 1) {
     const int64_t blocks = ((int64_t)a.tokens * a.heads + 3) / 4;
-    if (blocks > INT32_MAX) return CTI_ERR_UNSUPPORTED;
     if (launch_dependent(kv4_join_kernel<T, G>, dim3((unsigned)blocks), dim3(128), 0, s, a,
                          p.splits, static_cast<T*>(out)) != cudaSuccess)
       return CTI_ERR_CUDA;
@@ -575,19 +690,19 @@ int launch(const void* q, const void* pages, const Args& a, const Plan& p, void*
   return CTI_OK;
 }
 
-template <typename T, int G>
-int launch_rows(const void* q, const void* pages, const Args& a, const Plan& p, void* out,
-                cudaStream_t s) {
-  return p.rows == 8 ? launch<T, G, 8>(q, pages, a, p, out, s)
-                     : launch<T, G, 16>(q, pages, a, p, out, s);
-}
-
 template <typename T>
 int launch_dim(const void* q, const void* pages, const Args& a, const Plan& p, int head_dim,
                void* out, cudaStream_t s) {
-  return head_dim == 32   ? launch_rows<T, 1>(q, pages, a, p, out, s)
-         : head_dim == 64 ? launch_rows<T, 2>(q, pages, a, p, out, s)
-                          : launch_rows<T, 4>(q, pages, a, p, out, s);
+  if (head_dim == 32)
+    return p.row_tiles == 1   ? launch<T, 1, 1>(q, pages, a, p, out, s)
+           : p.row_tiles == 2 ? launch<T, 1, 2>(q, pages, a, p, out, s)
+                              : launch<T, 1, 4>(q, pages, a, p, out, s);
+  if (head_dim == 64)
+    return p.row_tiles == 1   ? launch<T, 2, 1>(q, pages, a, p, out, s)
+           : p.row_tiles == 2 ? launch<T, 2, 2>(q, pages, a, p, out, s)
+                              : launch<T, 2, 4>(q, pages, a, p, out, s);
+  return p.row_tiles == 1 ? launch<T, 4, 1>(q, pages, a, p, out, s)
+                          : launch<T, 4, 2>(q, pages, a, p, out, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -621,7 +736,9 @@ extern "C" int cti_kv4_attention(const void* q, int64_t q_stride, int dtype,
     return CTI_ERR_INVALID_ARG;
   if (dtype != CTI_DTYPE_BF16 && dtype != CTI_DTYPE_F16) return CTI_ERR_UNSUPPORTED;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128) return CTI_ERR_UNSUPPORTED;
-  if (tokens > INT32_MAX - 256 || heads > 65535) return CTI_ERR_UNSUPPORTED;
+  if (tokens > INT32_MAX - 256 || heads > 65535 || tokens * heads > INT32_MAX - 64 ||
+      (int64_t)num_seqs * kv_heads > INT32_MAX || table_cols > INT32_MAX / kv4::kPage)
+    return CTI_ERR_UNSUPPORTED;
   if (num_seqs == 0 || tokens == 0) return CTI_OK;
   if (!q || !out || !pages || !cu_seqlens || !kv_lens || (!page_table && table_cols > 0))
     return CTI_ERR_INVALID_ARG;
@@ -650,6 +767,7 @@ extern "C" int cti_kv4_attention(const void* q, int64_t q_stride, int dtype,
                   num_pages,
                   q_stride,
                   p.warps_per_tile,
+                  p.chunk,
                   static_cast<float*>(workspace),
                   reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + ws_o),
                   status};
