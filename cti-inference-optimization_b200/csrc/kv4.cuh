@@ -22,7 +22,7 @@
 // operands want them.  Token tau = 8 nt + r of the page, group g:
 //   K codes  the 32-bit word of dims 32 g + 8 t .. + 7 (t = 0..3) belongs to
 //            lane 4 r + t; dims 2 j and 2 j + 1 are the nibbles at bits 4 j
-//            and 16 + 4 j, the word rotated left by 3.
+//            and 16 + 4 j.
 //   V codes  the 16-bit half of dims 32 g + 4 c .. + 3 (c = 0..7) belongs to
 //            lane 4 c + (tau >> 1) % 4, the low half for an even tau, the
 //            high one for an odd; dim j is the nibble at bit 4 j.
@@ -105,19 +105,11 @@ CTI_DEVICE uint32_t fma2<__half>(uint32_t a, uint32_t b, uint32_t c) {
   return *reinterpret_cast<uint32_t*>(&r);
 }
 
-// 16 + n twice from nibble j of both halves of a K word (rotated left by 3)
-// or a V word.
+// 16 + n twice from nibble j of both halves of a word.
 template <typename T>
-CTI_DEVICE uint32_t k_pair(uint32_t w, int j) {
+CTI_DEVICE uint32_t code_pair(uint32_t w, int j) {
   constexpr int s = Type16<T>::kShift;
-  const int r = 3 + 4 * j - s;  // right shift that brings the nibble to bits s..s+3
-  const uint32_t x = r < 0 ? w << -r : j == 3 ? __funnelshift_r(w, w, r) : w >> r;
-  return (x & (0x000f000fu << s)) | Type16<T>::kMagic;
-}
-template <typename T>
-CTI_DEVICE uint32_t v_pair(uint32_t w, int j) {
-  constexpr int s = Type16<T>::kShift;
-  const int r = 4 * j - s;
+  const int r = 4 * j - s;  // right shift that brings the nibble to bits s..s+3
   const uint32_t x = r < 0 ? w << -r : w >> r;
   return (x & (0x000f000fu << s)) | Type16<T>::kMagic;
 }

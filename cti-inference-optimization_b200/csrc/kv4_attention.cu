@@ -13,18 +13,21 @@
 // head dims as the 16 rows of m16n8k16 matrix instructions and 8 query rows as
 // their columns (a single token has few, and the cache's side is the one that
 // must be unpacked):
-//   S^T = K Q^T with fp32 sums.  A code n is turned into the 16-bit number
-//     16 + n by a shift and a logic operation, exactly; the group's scale
-//     multiplies the 32-dim partial sums in fp32, and the bases enter as one
-//     more matrix instruction, sum_g b_g sum(q_g), with the sums of q split
-//     into two 16-bit numbers.  So a score is exact but for fp32 sums and
-//     2^-16 of that term.
+//   S^T = K Q^T with fp32 sums.  Codes enter as fp16 numbers by one logic
+//     operation each: nibbles at bits 0..3 and 4..7 of a half are the fp16
+//     subnormals n 2^-24 and n 2^-20, so two of them need no shift.  Q is
+//     scaled row by row with a power of two into fp16 (and by 2^-4 more where
+//     it meets the second kind), which rounds nothing that is not 2^-35 of the
+//     row's largest.  The group's scale multiplies the 32-dim partial sums in
+//     fp32; the offsets enter as one more matrix instruction, sum_g (16 s_g +
+//     b_g) sum(q_g), with the sums of q split into two 16-bit numbers.  So a
+//     score is exact but for fp32 sums and 2^-16 of that term.
 //   P^T = 2^(S^T scale log2e - m), against the row's exponent offset m, which
 //     is raised (and O, l rescaled) only when a score exceeds it by 2^8.
 //   O^T += V^T P^T with V = (16 + n) s + b by one 16-bit fused multiply-add
 //     per two values; P and V are rounded to 16 bits once each, as 16-bit
 //     attention does.  P^T becomes an operand by a transposition of 8 x 8.
-// The warps of a row tile (1, 2 or 4 of a block) join their O, m and l in
+// Where a block's warps share a row tile, they join their O, m and l in
 // shared memory; where a sequence is also split over blocks, they go to the
 // workspace and a second kernel joins them.
 #include <cfloat>
@@ -36,19 +39,32 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kSMs = 148;
 constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Warps of a block, pages in flight for each, and blocks of an SM: what
+// shared memory and registers allow.
+__host__ __device__ constexpr int warps(int G, int NT) { return G == 4 && NT == 1 ? 5 : 4; }
 __host__ __device__ constexpr int stages(int G) { return G == 1 ? 3 : 2; }
 __host__ __device__ constexpr int blocks_per_sm(int G, int NT) {
   return G == 4 || NT == 4 ? 2 : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 5 : 4;
 }
-__host__ __device__ constexpr size_t smem_bytes(int G) {
-  return (size_t)kWarps * stages(G) * block_bytes(G) + kWarps * stages(G) * 8;
+__host__ __device__ constexpr size_t smem_bytes(int G, int NT) {
+  return (size_t)warps(G, NT) * stages(G) * (block_bytes(G) + 8);
 }
+
+// x / d for 0 <= x < 2^31 by a multiplication and a shift (the round-up
+// method of Granlund and Montgomery).
+struct Divisor {
+  uint32_t mul, shift;
+  explicit Divisor(uint32_t d) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  CTI_DEVICE uint32_t operator()(uint32_t x) const { return (__umulhi(mul, x) + x) >> shift; }
+};
 
 struct Args {
   const int32_t* cu;
@@ -58,13 +74,14 @@ struct Args {
   int table_cols;
   int num_seqs;
   int tokens;
-  int heads, kv_heads;
+  int heads, kv_heads, group;
   float scale_log2;  // |scale| log2(e), at least 1e-30 so that -inf stays -inf
   int negate;        // scale < 0: the queries' signs are flipped
   int causal;
   int64_t num_pages;
   int64_t q_stride;
-  int warps_per_tile;  // 1, 2 or 4
+  Divisor by_group, by_kv_heads;
+  int shared;          // a block's warps share a row tile; else each has its own
   int chunk;           // pages of a sequence for a block (gridDim.z > 1)
   float* ws_o;         // [splits][tokens * heads][D]; splits > 1 only
   float2* ws_ml;       // [splits][tokens * heads]
@@ -76,7 +93,7 @@ struct Mma;
 template <>
 struct Mma<__nv_bfloat16> {
   CTI_DEVICE static void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -87,7 +104,7 @@ struct Mma<__nv_bfloat16> {
 template <>
 struct Mma<__half> {
   CTI_DEVICE static void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -104,15 +121,28 @@ CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* 
       : "memory");
 }
 
+// Word i of a lane's vectors of codes (i is known when the code is compiled).
+template <int N>
+CTI_DEVICE uint32_t word_of(const uint4 (&v)[N], int i) {
+  return (i & 3) == 0 ? v[i >> 2].x : (i & 3) == 1 ? v[i >> 2].y
+         : (i & 3) == 2 ? v[i >> 2].z : v[i >> 2].w;
+}
+
 // Transposes an 8 x 8 matrix of 16-bit values, two to a register.
 CTI_DEVICE uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
+// Bits 4 j .. 4 j + 3 of both halves of a K word as fp16: n 2^-24 for an even
+// j, n 2^-20 for an odd one.
+CTI_DEVICE uint32_t k_codes(uint32_t w, int j) {
+  return (j < 2 ? w : w >> 8) & (j & 1 ? 0x00f000f0u : 0x000f000fu);
+}
+
 template <typename T, int G, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
+__global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
     kv4_attention_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pages, const Args a,
                          T* __restrict__ out) {
   using Y = Type16<T>;
@@ -120,12 +150,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
   constexpr int D = 32 * G;
   constexpr int ROWS = 8 * NT;
   constexpr int S = stages(G);
+  constexpr int W = warps(G, NT);
   constexpr int kBlock = block_bytes(G);
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = warp_id(), lane = lane_id();
   const int r8 = lane >> 2, t4 = lane & 3;
   uint8_t* ring = smem + (size_t)warp * S * kBlock;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)kWarps * S * kBlock) + warp * S;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)W * S * kBlock) + warp * S;
   if (lane == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
@@ -133,12 +164,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
   __syncwarp();
   grid_dependency_wait();
 
-  const int wpt = a.warps_per_tile;
-  const unsigned unit = blockIdx.x * (kWarps / wpt) + warp / wpt;
+  const bool shared = a.shared != 0;
+  const unsigned unit = shared ? blockIdx.x : blockIdx.x * W + warp;
   if (unit >= (unsigned)a.num_seqs * a.kv_heads) return;  // all warps of a tile alike
-  const int sub = warp & (wpt - 1);
-  const int s = (int)(unit / (unsigned)a.kv_heads), kvh = (int)(unit - s * (unsigned)a.kv_heads);
-  const int group = a.heads / a.kv_heads;
+  const int s = (int)a.by_kv_heads(unit), kvh = (int)unit - s * a.kv_heads;
+  const int group = a.group;
   const int begin = __ldg(a.cu + s), end = __ldg(a.cu + s + 1);
   const int len = __ldg(a.kv_lens + s);
   if (begin < 0 || end > a.tokens || end < begin) {
@@ -156,7 +186,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
   const int32_t* table = a.table + s * a.table_stride;
   const uint8_t* base = pages + (int64_t)kvh * kBlock;
   const int64_t page_stride = (int64_t)a.kv_heads * kBlock;
-  const float sl = a.scale_log2;
   uint32_t count = 0;  // pages copied so far: stage and parity
   bool dead = false;   // a copy did not arrive in time
 
@@ -164,8 +193,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     // Keys that some row and that every row of the tile sees.
     const int row0 = tile * ROWS, row_last = min(rows, row0 + ROWS) - 1;
     const int most =
-        max(a.causal ? min(first + (int)((unsigned)row_last / group) + 1, limit) : limit, 0);
-    const int all = a.causal ? min(first + (int)((unsigned)row0 / group) + 1, limit) : limit;
+        max(a.causal ? min(first + (int)a.by_group(row_last) + 1, limit) : limit, 0);
+    const int all = a.causal ? min(first + (int)a.by_group(row0) + 1, limit) : limit;
 
     // ---- this warp's pages ----
     int p0 = 0, np = (most + kPage - 1) / kPage;
@@ -173,8 +202,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
       p0 = min(np, (int)blockIdx.z * a.chunk);
       np = (blockIdx.z == gridDim.z - 1 ? np : min(np, p0 + a.chunk)) - p0;
     }
-    if (wpt > 1) {
-      const int per = (np + wpt - 1) / wpt, skip = min(np, sub * per);
+    if (shared) {
+      const int per = (np + W - 1) / W, skip = min(np, warp * per);
       p0 += skip;
       np = min(np - skip, per);
     }
@@ -203,39 +232,58 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     // ---- queries: lane 4 r + t has dims 8 t .. + 7 of every group of row r ----
     uint32_t qb[NT][G][4];
     uint32_t off_b[NT][2];
+    float sl[NT][2];  // of rows 2 t and 2 t + 1, for scores in units of the row's scale
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + 8 * n + r8;
-      const int i = (int)((unsigned)row / group), h = kvh * group + row - i * group;
+      const int i = (int)a.by_group(row), h = kvh * group + row - i * group;
+      uint4 v[G];
+      float most_q = 0.0f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        v[g] = make_uint4(0, 0, 0, 0);
+        if (row < rows)
+          v[g] = __ldg(reinterpret_cast<const uint4*>(q + (begin + i) * a.q_stride +
+                                                      (int64_t)h * D + 32 * g + 8 * t4));
+        const uint32_t w[4] = {v[g].x, v[g].y, v[g].z, v[g].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          most_q = fmaxf(most_q, fmaxf(fabsf(Y::low(w[j])), fabsf(Y::high(w[j]))));
+      }
+      most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 1));
+      most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 2));
+      // 2^k with most_q 2^k in [2^14, 2^15)
+      int k = 14 + 127 - (int)(__float_as_uint(most_q) >> 23);
+      k = most_q > 0.0f ? max(-100, min(k, 100)) : 0;
+      const float up = __uint_as_float((uint32_t)(127 + k) << 23) * (a.negate ? -1.0f : 1.0f);
       float sum_mine = 0.0f;  // of group t4's 32 dims (G = 2: t4 & 1; G = 1: the only one)
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < rows)
-          v = __ldg(reinterpret_cast<const uint4*>(q + (begin + i) * a.q_stride + (int64_t)h * D +
-                                                   32 * g + 8 * t4));
-        if (a.negate) {
-          v.x ^= 0x80008000u;
-          v.y ^= 0x80008000u;
-          v.z ^= 0x80008000u;
-          v.w ^= 0x80008000u;
+        const uint32_t w[4] = {v[g].x, v[g].y, v[g].z, v[g].w};
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = Y::low(w[j]) * up, y = Y::high(w[j]) * up;
+          sum += x + y;
+          const float f = j & 1 ? 0.0625f : 1.0f;
+          qb[n][g][j] = Type16<__half>::pack(x * f, y * f);
         }
-        qb[n][g][0] = v.x;
-        qb[n][g][1] = v.y;
-        qb[n][g][2] = v.z;
-        qb[n][g][3] = v.w;
-        float sum = Y::low(v.x) + Y::high(v.x) + Y::low(v.y) + Y::high(v.y) + Y::low(v.z) +
-                    Y::high(v.z) + Y::low(v.w) + Y::high(v.w);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         if (g == (t4 & (G - 1))) sum_mine = sum;
       }
-      // The bases' operand: the row that meets b of a group is the sum of q in
-      // it, in two parts; the one that meets its scale is 0.
-      const uint32_t hi = Y::bits(sum_mine);
-      const uint32_t lo = Y::bits(sum_mine - Y::to_float(hi));
-      off_b[n][0] = G == 4 || t4 < G ? hi << 16 : t4 < 2 * G ? lo << 16 : 0u;
-      off_b[n][1] = G == 4 ? lo << 16 : 0u;
+      // The offsets' operand: the rows that meet s and b of a group are 16 and
+      // 1 times the sum of q in it, in two parts, in units of 2^10.
+      sum_mine *= 0x1p-10f;
+      const float hi = Y::to_float(Y::bits(sum_mine));
+      const float lo = sum_mine - hi;
+      const uint32_t hi2 = Y::pack(16.0f * hi, hi), lo2 = Y::pack(16.0f * lo, lo);
+      off_b[n][0] = G == 4 || t4 < G ? hi2 : t4 < 2 * G ? lo2 : 0u;
+      off_b[n][1] = G == 4 ? lo2 : 0u;
+      const float mine =
+          fmaxf(a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - k) << 23), 1e-37f);
+      sl[n][0] = __shfl_sync(0xffffffffu, mine, 8 * t4);
+      sl[n][1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
     }
     int sees[NT][2];  // keys that rows 2 t and 2 t + 1 see
 #pragma unroll
@@ -243,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = min(row0 + 8 * n + 2 * t4 + e, row_last);
-        sees[n][e] = a.causal ? min(first + (int)((unsigned)row / group) + 1, limit) : limit;
+        sees[n][e] = a.causal ? min(first + (int)a.by_group(row) + 1, limit) : limit;
       }
 
     float o[NT][2 * G][4];
@@ -268,59 +316,48 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
 
       // ---- S^T = K Q^T, 16 keys at a time ----
       float sc[NT][4][4];
+      uint4 kw[2 * G];
+#pragma unroll
+      for (int v = 0; v < 2 * G; ++v)
+        kw[v] = *reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        uint32_t w[2][G];  // of tokens 16 mt + r and + 8
-        uint32_t meta[2][G];
+        uint32_t meta[2][G];  // of tokens 16 mt + r and + 8
+        uint32_t am[2];       // its word for the offsets: group t's
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int nt = 2 * mt + e;
-          const uint32_t* cw = reinterpret_cast<const uint32_t*>(
-              blk + ((nt * G >> 2) * 32 + lane) * 16 + (nt * G & 3) * 4);
           const uint32_t* mw =
-              reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) + (8 * nt + r8) * G;
-          if (G == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(cw);
-            w[e][0] = x.x, w[e][G > 1 ? 1 : 0] = x.y, w[e][G > 2 ? 2 : 0] = x.z, w[e][G - 1] = x.w;
+              reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) + (16 * mt + 8 * e + r8) * G;
+          if constexpr (G == 4) {
             const uint4 y = *reinterpret_cast<const uint4*>(mw);
-            meta[e][0] = y.x, meta[e][G > 1 ? 1 : 0] = y.y, meta[e][G > 2 ? 2 : 0] = y.z,
-            meta[e][G - 1] = y.w;
-          } else if (G == 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(cw);
-            w[e][0] = x.x, w[e][G - 1] = x.y;
+            meta[e][0] = y.x, meta[e][1] = y.y, meta[e][2] = y.z, meta[e][3] = y.w;
+          } else if constexpr (G == 2) {
             const uint2 y = *reinterpret_cast<const uint2*>(mw);
-            meta[e][0] = y.x, meta[e][G - 1] = y.y;
+            meta[e][0] = y.x, meta[e][1] = y.y;
           } else {
-            w[e][0] = *cw;
             meta[e][0] = *mw;
           }
+          am[e] = G == 1 ? meta[e][0] : mw[t4 & (G - 1)];
         }
-        // Each lane's own group of the meta for the bases.
-        uint32_t am[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          am[e] = G == 1 ? meta[e][0]
-                         : *(reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) +
-                             (16 * mt + 8 * e + r8) * G + (t4 & (G - 1)));
         const uint32_t off_a[4] = {am[0], am[1], G == 4 ? am[0] : 0u, G == 4 ? am[1] : 0u};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          Mma<T>::run(c, off_a, off_b[n][0], off_b[n][1]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[n][mt][e] = 0.0f;
-          M::run(sc[n][mt], off_a, off_b[n][0], off_b[n][1]);
+          for (int e = 0; e < 4; ++e) sc[n][mt][e] = c[e] * 0x1p-14f;
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const uint32_t a0[4] = {k_pair<T>(w[0][g], 0), k_pair<T>(w[1][g], 0),
-                                  k_pair<T>(w[0][g], 1), k_pair<T>(w[1][g], 1)};
-          const uint32_t a1[4] = {k_pair<T>(w[0][g], 2), k_pair<T>(w[1][g], 2),
-                                  k_pair<T>(w[0][g], 3), k_pair<T>(w[1][g], 3)};
+          const uint32_t w0 = word_of(kw, 2 * mt * G + g), w1 = word_of(kw, (2 * mt + 1) * G + g);
+          const uint32_t a0[4] = {k_codes(w0, 0), k_codes(w1, 0), k_codes(w0, 1), k_codes(w1, 1)};
+          const uint32_t a1[4] = {k_codes(w0, 2), k_codes(w1, 2), k_codes(w0, 3), k_codes(w1, 3)};
           const float s0 = Y::low(meta[0][g]), s1 = Y::low(meta[1][g]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            M::run(c, a0, qb[n][g][0], qb[n][g][1]);
-            M::run(c, a1, qb[n][g][2], qb[n][g][3]);
+            Mma<__half>::run(c, a0, qb[n][g][0], qb[n][g][1]);
+            Mma<__half>::run(c, a1, qb[n][g][2], qb[n][g][3]);
             sc[n][mt][0] = fmaf(c[0], s0, sc[n][mt][0]);
             sc[n][mt][1] = fmaf(c[1], s0, sc[n][mt][1]);
             sc[n][mt][2] = fmaf(c[2], s1, sc[n][mt][2]);
@@ -391,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
 #pragma unroll
           for (int mt = 1; mt < 4; ++mt) x = fmaxf(x, fmaxf(sc[n][mt][e], sc[n][mt][2 + e]));
           mx[n][e] = x;
-          raise = raise || (x - m[n][e]) * sl > kSlack;
+          raise = raise || (x - m[n][e]) * sl[n][e] > kSlack;
         }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -403,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             if (x > m[n][e]) {
-              const float corr = ex2_approx((m[n][e] - x) * sl);
+              const float corr = ex2_approx((m[n][e] - x) * sl[n][e]);
               m[n][e] = x;
               l[n][e] *= corr;
 #pragma unroll
@@ -420,7 +457,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) noff[n][e] = m[n][e] == -INFINITY ? 0.0f : -m[n][e] * sl;
+        for (int e = 0; e < 2; ++e) noff[n][e] = m[n][e] == -INFINITY ? 0.0f : -m[n][e] * sl[n][e];
+      uint4 vw[2 * G];
+#pragma unroll
+      for (int v = 0; v < 2 * G; ++v)
+        vw[v] = *reinterpret_cast<const uint4*>(blk + v_codes_at(G) + (v * 32 + lane) * 16);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         uint32_t pb[NT][2];
@@ -428,53 +469,42 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
         for (int n = 0; n < NT; ++n) {
           float(&x)[4] = sc[n][kk];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = ex2_approx(fmaf(x[e], sl, noff[n][e & 1]));
+          for (int e = 0; e < 4; ++e) x[e] = ex2_approx(fmaf(x[e], sl[n][e & 1], noff[n][e & 1]));
           l[n][0] += x[0] + x[2];
           l[n][1] += x[1] + x[3];
           pb[n][0] = transpose8(Y::pack(x[0], x[1]));
           pb[n][1] = transpose8(Y::pack(x[2], x[3]));
         }
-        uint32_t w[2][G];
         uint2 meta[2][G];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int nt = 2 * kk + e;
-          const uint32_t* cw = reinterpret_cast<const uint32_t*>(
-              blk + v_codes_at(G) + ((nt * G >> 2) * 32 + lane) * 16 + (nt * G & 3) * 4);
           const uint2* mw =
-              reinterpret_cast<const uint2*>(blk + v_meta_at(G)) + (4 * nt + t4) * G;
-          if (G == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(cw);
-            w[e][0] = x.x, w[e][G > 1 ? 1 : 0] = x.y, w[e][G > 2 ? 2 : 0] = x.z, w[e][G - 1] = x.w;
-          } else if (G == 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(cw);
-            w[e][0] = x.x, w[e][G - 1] = x.y;
-          } else {
-            w[e][0] = *cw;
-          }
-          if (G == 1) {
+              reinterpret_cast<const uint2*>(blk + v_meta_at(G)) + (8 * kk + 4 * e + t4) * G;
+          if constexpr (G == 1) {
             meta[e][0] = *mw;
           } else {
 #pragma unroll
             for (int g = 0; g < G; g += 2) {
               const uint4 y = *reinterpret_cast<const uint4*>(mw + g);
               meta[e][g] = make_uint2(y.x, y.y);
-              meta[e][g + (G > 1 ? 1 : 0)] = make_uint2(y.z, y.w);
+              meta[e][g + 1] = make_uint2(y.z, y.w);
             }
           }
         }
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          const uint32_t w0 = word_of(vw, 2 * kk * G + g), w1 = word_of(vw, (2 * kk + 1) * G + g);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t av[4] = {
-                fma2<T>(v_pair<T>(w[0][g], 2 * j), meta[0][g].x, meta[0][g].y),
-                fma2<T>(v_pair<T>(w[0][g], 2 * j + 1), meta[0][g].x, meta[0][g].y),
-                fma2<T>(v_pair<T>(w[1][g], 2 * j), meta[1][g].x, meta[1][g].y),
-                fma2<T>(v_pair<T>(w[1][g], 2 * j + 1), meta[1][g].x, meta[1][g].y)};
+                fma2<T>(code_pair<T>(w0, 2 * j), meta[0][g].x, meta[0][g].y),
+                fma2<T>(code_pair<T>(w0, 2 * j + 1), meta[0][g].x, meta[0][g].y),
+                fma2<T>(code_pair<T>(w1, 2 * j), meta[1][g].x, meta[1][g].y),
+                fma2<T>(code_pair<T>(w1, 2 * j + 1), meta[1][g].x, meta[1][g].y)};
 #pragma unroll
             for (int n = 0; n < NT; ++n) M::run(o[n][2 * g + j], av, pb[n][0], pb[n][1]);
           }
+        }
       }
       __syncwarp();
       if (done + S < np) issue(done + S);
@@ -495,12 +525,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
         l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
         l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
       }
-    if (wpt > 1) {
+    if (shared) {
       // Every warp's rows in its own ring, then the first warp adds them up.
       float* mine = reinterpret_cast<float*>(ring);
       static_assert((ROWS * D + 2 * ROWS) * 4 <= S * kBlock, "room for the rows");
       __syncwarp();
-      if (sub != 0) {
+      if (warp != 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -516,9 +546,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
                   make_float2(m[n][e], l[n][e]);
           }
       }
-      named_barrier_sync(1 + warp / wpt, 32 * wpt);
-      if (sub == 0) {
-        for (int w = 1; w < wpt; ++w) {
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < W; ++w) {
           const float* src = reinterpret_cast<const float*>(ring + (size_t)w * S * kBlock);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -527,8 +557,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
               const int row = 8 * n + 2 * t4 + e;
               const float2 ml = *reinterpret_cast<const float2*>(src + ROWS * D + 2 * row);
               const float mm = fmaxf(m[n][e], ml.x);
-              const float ca = m[n][e] == mm ? 1.0f : ex2_approx((m[n][e] - mm) * sl);
-              const float cb = ml.x == mm ? 1.0f : ex2_approx((ml.x - mm) * sl);
+              const float ca = m[n][e] == mm ? 1.0f : ex2_approx((m[n][e] - mm) * sl[n][e]);
+              const float cb = ml.x == mm ? 1.0f : ex2_approx((ml.x - mm) * sl[n][e]);
               m[n][e] = mm;
               l[n][e] = l[n][e] * ca + ml.y * cb;
 #pragma unroll
@@ -544,14 +574,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
         }
       }
     }
-    if (sub == 0) {
+    if (!shared || warp == 0) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int row = row0 + 8 * n + 2 * t4 + e;
           if (row >= rows) continue;
-          const int i = (int)((unsigned)row / group);
+          const int i = (int)a.by_group(row);
           const int64_t at = (int64_t)(begin + i) * a.heads + kvh * group + row - i * group;
           if (gridDim.z == 1) {
             const float inv = l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e];
@@ -562,8 +592,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
                              Y::pack(o[n][2 * g + 1][e] * inv, o[n][2 * g + 1][2 + e] * inv));
           } else {
             const int64_t ws = (int64_t)blockIdx.z * a.tokens * a.heads + at;
-            if (r8 == 0) a.ws_ml[ws] = make_float2(m[n][e], l[n][e]);
-            if (np > 0 || wpt > 1) {  // else the row is empty, and not read
+            // m times its row's scale: a power of 2 that weights can be told by
+            if (r8 == 0)
+              a.ws_ml[ws] = make_float2(m[n][e] == -INFINITY ? -INFINITY : m[n][e] * sl[n][e],
+                                        l[n][e]);
+            if (np > 0 || shared) {  // else the row is empty, and not read
 #pragma unroll
               for (int g = 0; g < G; ++g)
                 *reinterpret_cast<float4*>(a.ws_o + ws * D + 32 * g + 4 * r8) =
@@ -573,11 +606,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
           }
         }
     }
-    if (wpt > 1) {
+    if (shared) {
       // The rings are free again (copies may overwrite them) once the first
       // warp has read them.
       fence_proxy_async_smem();
-      named_barrier_sync(1 + warp / wpt, 32 * wpt);
+      __syncthreads();
     }
   }
 }
@@ -606,7 +639,7 @@ __global__ void __launch_bounds__(128)
   for (int z = 0; z < splits; ++z) {
     const float2 ml = a.ws_ml[z * rows + row];
     if (ml.y == 0.0f) continue;  // no key of the split is seen
-    const float w = ml.x == mm ? 1.0f : ex2_approx((ml.x - mm) * a.scale_log2);
+    const float w = ml.x == mm ? 1.0f : ex2_approx(ml.x - mm);
     l = fmaf(ml.y, w, l);
 #pragma unroll
     for (int g = 0; g < G; ++g)
@@ -621,7 +654,7 @@ __global__ void __launch_bounds__(128)
 // How a call is laid out over the GPU; a function of the sizes alone.
 struct Plan {
   int row_tiles;       // of 8 rows, that a warp takes: 1, 2 or 4
-  int warps_per_tile;  // that share a tile's pages in a block
+  bool shared;         // a block's warps share a tile's pages
   int splits, chunk;   // blocks that share them, and the pages of each
   int64_t tiles;       // row tiles of a sequence
 };
@@ -636,21 +669,21 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   p.tiles = (rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
   const double units = (double)num_seqs * kv_heads * (double)p.tiles;
   const int64_t pages = max_kv_len > 0 ? (max_kv_len + kPage - 1) / kPage : 1;
-  const double room = (double)kSMs * blocks_per_sm(G, p.row_tiles) * kWarps;  // warps at once
+  const double room = (double)kSMs * blocks_per_sm(G, p.row_tiles) * warps(G, p.row_tiles);  // warps at once
   p.splits = 1;
   p.chunk = 0;
   if (units >= room && pages <= 8) {
     // Short sequences, more tiles than warps: a warp each.
-    p.warps_per_tile = 1;
+    p.shared = false;
     return p;
   }
   // A block's warps share a tile; with long sequences, blocks do too, so that
   // all run at once, or, where that is more than 16 pages for a warp, in
   // pieces of 12, small enough that sequences of any lengths balance out.
-  p.warps_per_tile = pages >= 4 ? 4 : pages >= 2 ? 2 : 1;
+  p.shared = true;
   const double ideal = units * pages / room;
   int64_t per_warp = ideal > 16 ? 12 : (int64_t)ideal + 1;
-  p.chunk = (int)(per_warp * p.warps_per_tile);
+  p.chunk = (int)(per_warp * warps(G, p.row_tiles));
   int64_t splits = (pages + p.chunk - 1) / p.chunk;
   if (splits > 128) {
     splits = 128;
@@ -670,14 +703,14 @@ template <typename T, int G, int NT>
 int launch(const void* q, const void* pages, const Args& a, const Plan& p, void* out,
            cudaStream_t s) {
   static uint64_t configured = 0;
-  if (ensure_smem_limit(kv4_attention_kernel<T, G, NT>, (int)smem_bytes(G), configured) !=
+  if (ensure_smem_limit(kv4_attention_kernel<T, G, NT>, (int)smem_bytes(G, NT), configured) !=
       cudaSuccess)
     return CTI_ERR_CUDA;
   const int64_t units = (int64_t)a.num_seqs * a.kv_heads;
-  const int per = kWarps / p.warps_per_tile;
+  const int per = p.shared ? 1 : warps(G, NT);
   const dim3 grid((unsigned)((units + per - 1) / per),
                   (unsigned)(p.tiles < 65535 ? p.tiles : 65535), (unsigned)p.splits);
-  if (launch_dependent(kv4_attention_kernel<T, G, NT>, grid, dim3(kThreads), smem_bytes(G), s,
+  if (launch_dependent(kv4_attention_kernel<T, G, NT>, grid, dim3(warps(G, NT) * 32), smem_bytes(G, NT), s,
                        static_cast<const T*>(q), static_cast<const uint8_t*>(pages), a,
                        static_cast<T*>(out)) != cudaSuccess)
     return CTI_ERR_CUDA;
@@ -761,12 +794,15 @@ extern "C" int cti_kv4_attention(const void* q, int64_t q_stride, int dtype,
                   (int)tokens,
                   heads,
                   kv_heads,
+                  heads / kv_heads,
                   fmaxf(fabsf(scale) * kLog2e, 1e-30f),
                   scale < 0.0f,
                   causal,
                   num_pages,
                   q_stride,
-                  p.warps_per_tile,
+                  Divisor((uint32_t)(heads / kv_heads)),
+                  Divisor((uint32_t)kv_heads),
+                  p.shared,
                   p.chunk,
                   static_cast<float*>(workspace),
                   reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + ws_o),

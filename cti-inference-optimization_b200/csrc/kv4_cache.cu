@@ -197,15 +197,15 @@ CTI_DEVICE uint32_t twice(uint32_t h) { return __byte_perm(h, h, 0x1010); }
 template <typename T>
 CTI_DEVICE uint4 k_values(uint32_t w, uint32_t meta) {
   const uint32_t s = __byte_perm(meta, 0, 0x1010), b = __byte_perm(meta, 0, 0x3232);
-  return make_uint4(fma2<T>(k_pair<T>(w, 0), s, b), fma2<T>(k_pair<T>(w, 1), s, b),
-                    fma2<T>(k_pair<T>(w, 2), s, b), fma2<T>(k_pair<T>(w, 3), s, b));
+  return make_uint4(fma2<T>(code_pair<T>(w, 0), s, b), fma2<T>(code_pair<T>(w, 1), s, b),
+                    fma2<T>(code_pair<T>(w, 2), s, b), fma2<T>(code_pair<T>(w, 3), s, b));
 }
 // What a V word stands for: its even token's 4 values, and its odd one's.
 template <typename T>
 CTI_DEVICE void v_values(uint32_t w, uint32_t s, uint32_t b, uint2& even, uint2& odd) {
   uint32_t x[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = fma2<T>(v_pair<T>(w, j), s, b);
+  for (int j = 0; j < 4; ++j) x[j] = fma2<T>(code_pair<T>(w, j), s, b);
   even = make_uint2(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410));
   odd = make_uint2(__byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
 }
@@ -243,8 +243,7 @@ __global__ void __launch_bounds__(kThreads)
       rv = __ldg(reinterpret_cast<const uint4*>(v + (t0 + tok) * a.v_stride + piece * 8));
     }
     uint32_t ks, kb, vs, vb;
-    uint32_t wk = quantise<T, kKeys>(rk, ks, kb);
-    wk = __funnelshift_l(wk, wk, 3);
+    const uint32_t wk = quantise<T, kKeys>(rk, ks, kb);
     const uint32_t wv = quantise<T, kValues>(rv, vs, vb);
     if (!live) continue;  // the loop's bound is the same for a whole warp
     uint8_t* block = pages + (at.page * a.kv_heads + head) * (int64_t)block_bytes(G);
@@ -413,7 +412,7 @@ CTI_DEVICE void append_run(const T* __restrict__ rows, int stride, const Run& ru
       uint32_t s, b;
       const uint32_t word = quantise<T, ORDER>(raw[j], s, b);
       if (ORDER == kKeys) {
-        w[j] = __funnelshift_l(word, word, 3);
+        w[j] = word;
         if (live[j] && t == 0)
           *reinterpret_cast<uint32_t*>(block + k_meta_at(G) + k_meta_word_at(tau, g, G)) =
               s | b << 16;
