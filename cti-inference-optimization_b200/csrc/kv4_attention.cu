@@ -6,6 +6,9 @@
 // kv_heads).  One pass with the running maximum and sum of the softmax in
 // fp32; a row that sees no key is zero.
 //
+// Calls with many rows per sequence go to the tensor-core tiles of
+// kv4_tiles.cu; the rest of this file is for single tokens and a few.
+//
 // A warp takes a tile of 8, 16 or 32 rows (the query heads of one KV head,
 // token by token) and a range of the sequence's pages.  One bulk copy brings a
 // page's block of the KV head (2560 G bytes) into the warp's own ring in
@@ -32,15 +35,13 @@
 // workspace and a second kernel joins them.
 #include <cfloat>
 
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 
 namespace cti {
 namespace {
 
 using namespace kv4;
 
-constexpr int kSMs = 148;
-constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Warps of a block, pages in flight for each, and blocks of an SM: what
@@ -54,40 +55,6 @@ __host__ __device__ constexpr size_t smem_bytes(int G, int NT) {
   return (size_t)warps(G, NT) * stages(G) * (block_bytes(G) + 8);
 }
 
-// x / d for 0 <= x < 2^31 by a multiplication and a shift (the round-up
-// method of Granlund and Montgomery).
-struct Divisor {
-  uint32_t mul, shift;
-  explicit Divisor(uint32_t d) {
-    shift = 0;
-    while ((1ull << shift) < d) ++shift;
-    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  CTI_DEVICE uint32_t operator()(uint32_t x) const { return (__umulhi(mul, x) + x) >> shift; }
-};
-
-struct Args {
-  const int32_t* cu;
-  const int32_t* kv_lens;
-  const int32_t* table;
-  int64_t table_stride;
-  int table_cols;
-  int num_seqs;
-  int tokens;
-  int heads, kv_heads, group;
-  float scale_log2;  // |scale| log2(e), at least 1e-30 so that -inf stays -inf
-  int negate;        // scale < 0: the queries' signs are flipped
-  int causal;
-  int64_t num_pages;
-  int64_t q_stride;
-  Divisor by_group, by_kv_heads;
-  int shared;          // a block's warps share a row tile; else each has its own
-  int chunk;           // pages of a sequence for a block (gridDim.z > 1)
-  float* ws_o;         // [splits][tokens * heads][D]; splits > 1 only
-  float2* ws_ml;       // [splits][tokens * heads]
-  int32_t* status;
-};
-
 template <typename T>
 struct Mma;
 template <>
@@ -99,7 +66,6 @@ struct Mma<__nv_bfloat16> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  static constexpr uint32_t kInf = 0x7f80u;
 };
 template <>
 struct Mma<__half> {
@@ -110,7 +76,6 @@ struct Mma<__half> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  static constexpr uint32_t kInf = 0x7c00u;
 };
 
 CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -379,8 +344,8 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
         if (all < most) {
 #pragma unroll
           for (int i = 0; i < 2 * G; ++i) {
-            nan0 |= (vm[i] & M::kInf) == M::kInf;
-            nan1 |= ((vm[i] >> 16) & M::kInf) == M::kInf;
+            nan0 |= (vm[i] & Inf16<T>::kBits) == Inf16<T>::kBits;
+            nan1 |= ((vm[i] >> 16) & Inf16<T>::kBits) == Inf16<T>::kBits;
           }
         }
         const uint32_t keep = (nan0 || 2 * lane >= lim_most ? 0u : 0xffffu) |
@@ -651,8 +616,13 @@ __global__ void __launch_bounds__(128)
     reinterpret_cast<uint16_t*>(out)[row * D + 32 * g + lane] = (uint16_t)Y::bits(o[g] * inv);
 }
 
+// Query rows of a KV head, by the caller's bound, from which a sequence's rows
+// are taken in tiles of 128 on the tensor cores.
+constexpr int kTilesFrom = 33;
+
 // How a call is laid out over the GPU; a function of the sizes alone.
 struct Plan {
+  int big;             // 128-row tiles of a block (kv4_tiles.cu), 1 or 2; 0: warps as here
   int row_tiles;       // of 8 rows, that a warp takes: 1, 2 or 4
   bool shared;         // a block's warps share a tile's pages
   int splits, chunk;   // blocks that share them, and the pages of each
@@ -664,11 +634,23 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   const int G = head_dim / kGroup;
   const int64_t most = max_new < tokens ? max_new : tokens;
   const int64_t rows = (most > 0 ? most : 1) * (heads / kv_heads);
-  Plan p;
+  const int64_t pages = max_kv_len > 0 ? (max_kv_len + kPage - 1) / kPage : 1;
+  Plan p = {};
+  if (rows >= kTilesFrom) {
+    // Two tiles share the unpacking of a page.  Fewer blocks than the GPU holds
+    // share the pages, eight at least.
+    p.big = rows > 128 ? 2 : 1;
+    p.tiles = (rows + 128 * p.big - 1) / (128 * p.big);
+    const double blocks = (double)num_seqs * kv_heads * (double)p.tiles;
+    int64_t splits = (int64_t)(kSMs * (3 - p.big) / blocks);
+    splits = splits > pages / 8 ? pages / 8 : splits;
+    p.splits = (int)(splits < 1 ? 1 : splits > 128 ? 128 : splits);
+    p.chunk = (int)((pages + p.splits - 1) / p.splits);
+    return p;
+  }
   p.row_tiles = rows <= 8 ? 1 : rows <= 16 || G == 4 ? 2 : 4;
   p.tiles = (rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
   const double units = (double)num_seqs * kv_heads * (double)p.tiles;
-  const int64_t pages = max_kv_len > 0 ? (max_kv_len + kPage - 1) / kPage : 1;
   const double room = (double)kSMs * blocks_per_sm(G, p.row_tiles) * warps(G, p.row_tiles);  // warps at once
   p.splits = 1;
   p.chunk = 0;
@@ -714,28 +696,42 @@ int launch(const void* q, const void* pages, const Args& a, const Plan& p, void*
                        static_cast<const T*>(q), static_cast<const uint8_t*>(pages), a,
                        static_cast<T*>(out)) != cudaSuccess)
     return CTI_ERR_CUDA;
-  if (p.splits > 1) {
-    const int64_t blocks = ((int64_t)a.tokens * a.heads + 3) / 4;
-    if (launch_dependent(kv4_join_kernel<T, G>, dim3((unsigned)blocks), dim3(128), 0, s, a,
-                         p.splits, static_cast<T*>(out)) != cudaSuccess)
-      return CTI_ERR_CUDA;
-  }
   return CTI_OK;
 }
 
+template <typename T, int G>
+int launch_join(const Args& a, int splits, void* out, cudaStream_t s) {
+  const int64_t blocks = ((int64_t)a.tokens * a.heads + 3) / 4;
+  return launch_dependent(kv4_join_kernel<T, G>, dim3((unsigned)blocks), dim3(128), 0, s, a,
+                          splits, static_cast<T*>(out)) == cudaSuccess
+             ? CTI_OK
+             : CTI_ERR_CUDA;
+}
+
+template <typename T, int G>
+int launch_shape(const void* q, const void* pages, const Args& a, const Plan& p, int dtype,
+                 void* out, cudaStream_t s) {
+  int rc;
+  if (p.big) {
+    rc = launch_tiles(q, pages, a, dtype, 32 * G, p.big, p.tiles, p.splits, out, s);
+  } else if constexpr (G == 4) {
+    rc = p.row_tiles == 1 ? launch<T, G, 1>(q, pages, a, p, out, s)
+                          : launch<T, G, 2>(q, pages, a, p, out, s);
+  } else {
+    rc = p.row_tiles == 1   ? launch<T, G, 1>(q, pages, a, p, out, s)
+         : p.row_tiles == 2 ? launch<T, G, 2>(q, pages, a, p, out, s)
+                            : launch<T, G, 4>(q, pages, a, p, out, s);
+  }
+  if (rc != CTI_OK || p.splits == 1) return rc;
+  return launch_join<T, G>(a, p.splits, out, s);
+}
+
 template <typename T>
-int launch_dim(const void* q, const void* pages, const Args& a, const Plan& p, int head_dim,
-               void* out, cudaStream_t s) {
-  if (head_dim == 32)
-    return p.row_tiles == 1   ? launch<T, 1, 1>(q, pages, a, p, out, s)
-           : p.row_tiles == 2 ? launch<T, 1, 2>(q, pages, a, p, out, s)
-                              : launch<T, 1, 4>(q, pages, a, p, out, s);
-  if (head_dim == 64)
-    return p.row_tiles == 1   ? launch<T, 2, 1>(q, pages, a, p, out, s)
-           : p.row_tiles == 2 ? launch<T, 2, 2>(q, pages, a, p, out, s)
-                              : launch<T, 2, 4>(q, pages, a, p, out, s);
-  return p.row_tiles == 1 ? launch<T, 4, 1>(q, pages, a, p, out, s)
-                          : launch<T, 4, 2>(q, pages, a, p, out, s);
+int launch_dim(const void* q, const void* pages, const Args& a, const Plan& p, int dtype,
+               int head_dim, void* out, cudaStream_t s) {
+  return head_dim == 32   ? launch_shape<T, 1>(q, pages, a, p, dtype, out, s)
+         : head_dim == 64 ? launch_shape<T, 2>(q, pages, a, p, dtype, out, s)
+                          : launch_shape<T, 4>(q, pages, a, p, dtype, out, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -808,6 +804,7 @@ extern "C" int cti_kv4_attention(const void* q, int64_t q_stride, int dtype,
                   reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + ws_o),
                   status};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == CTI_DTYPE_BF16 ? launch_dim<__nv_bfloat16>(q, pages, a, p, head_dim, out, s)
-                                 : launch_dim<__half>(q, pages, a, p, head_dim, out, s);
+  return dtype == CTI_DTYPE_BF16
+             ? launch_dim<__nv_bfloat16>(q, pages, a, p, dtype, head_dim, out, s)
+             : launch_dim<__half>(q, pages, a, p, dtype, head_dim, out, s);
 }

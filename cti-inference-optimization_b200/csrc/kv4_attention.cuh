@@ -1,0 +1,68 @@
+// What the kernels of the attention over the 4-bit cache share: their
+// arguments, and how far a row's exponent offset may lag.
+#pragma once
+
+#include "kv4.cuh"
+
+namespace cti {
+namespace kv4 {
+
+constexpr int kSMs = 148;
+// A row's exponent offset m is only raised (and O, l rescaled) when a score
+// exceeds it by this power of 2: p <= 2^kSlack.
+constexpr float kSlack = 8.0f;
+
+// x / d for 0 <= x < 2^31 by a multiplication and a shift (the round-up
+// method of Granlund and Montgomery).
+struct Divisor {
+  uint32_t mul, shift;
+  explicit Divisor(uint32_t d) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  CTI_DEVICE uint32_t operator()(uint32_t x) const { return (__umulhi(mul, x) + x) >> shift; }
+};
+
+struct Args {
+  const int32_t* cu;
+  const int32_t* kv_lens;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_cols;
+  int num_seqs;
+  int tokens;
+  int heads, kv_heads, group;
+  float scale_log2;  // |scale| log2(e), at least 1e-30 so that -inf stays -inf
+  int negate;        // scale < 0: the queries' signs are flipped
+  int causal;
+  int64_t num_pages;
+  int64_t q_stride;
+  Divisor by_group, by_kv_heads;
+  int shared;          // a block's warps share a row tile; else each has its own
+  int chunk;           // pages of a sequence for a block (gridDim.z > 1)
+  float* ws_o;         // [splits][tokens * heads][D]; splits > 1 only
+  float2* ws_ml;       // [splits][tokens * heads]
+  int32_t* status;
+};
+
+// Exponent bits of T: set in infinities and NaN.
+template <typename T>
+struct Inf16;
+template <>
+struct Inf16<__nv_bfloat16> {
+  static constexpr uint32_t kBits = 0x7f80u;
+};
+template <>
+struct Inf16<__half> {
+  static constexpr uint32_t kBits = 0x7c00u;
+};
+
+// Rows tiles of 128 on the tensor cores (kv4_tiles.cu).  tiles: 128-row tiles
+// that a block takes side by side, 1 or 2; y: of a sequence; splits: as for
+// the row kernel.  CTI_OK or a CTI_ERR code.
+int launch_tiles(const void* q, const void* pages, const Args& a, int dtype, int head_dim,
+                 int tiles, int64_t y, int splits, void* out, cudaStream_t s);
+
+}  // namespace kv4
+}  // namespace cti

@@ -1,0 +1,692 @@
+// Attention of many new tokens over the 4-bit key/value cache: row tiles of
+// 128 on the tensor cores (the definition is in kv4_attention.cu, the format in
+// kv4.cuh).
+//
+// A block takes one or two 128-row tiles (the query heads of one KV head, token
+// by token) of a sequence and walks over its pages:
+//   warps 0..3 (and 4..7)  softmax of a tile, thread = row.  They lay the
+//          tile's queries out in shared memory first: fp16, each row scaled by
+//          a power of two.  Per page: the row's 64 scores from TMEM, masked;
+//          p = 2^(x - m), m raised (O and l rescaled) only when a score exceeds
+//          it by 2^8; P in 16 bits back over the scores.
+//   4 warps  unpacking: two take a page's keys, two its values, 16 bytes a lane
+//          at a time straight from global memory (requested before they wait
+//          for a free stage), to 16 bits in the swizzled layout of the matrix
+//          operands.  Two tiles share the work.
+//   1 warp issues S = Q K^T (M 128, N 64), 1 warp O += P V with P from TMEM and
+//          V as an MN-major operand.
+// Keys are rounded to fp16 (11 bits, as the queries hold 8 or 11) after a
+// scaling by a power of two, common to a page, that is 1 unless the page's
+// largest magnitude is outside [2^-6, 2^15); the scores are scaled back.  P and
+// V are rounded to the tensors' type, as 16-bit attention does.  Every wait is
+// a bounded mbarrier wait; one that runs out records its site in the status
+// word and the roles unwind.
+#include <cfloat>
+
+#include "kv4_attention.cuh"
+
+namespace cti {
+namespace {
+
+using namespace kv4;
+
+constexpr int kTile = 128;
+constexpr int kUnpackWarps = 4;
+
+template <int G, int TILES>
+struct Shape {
+  static constexpr int D = 32 * G;
+  static constexpr int kRow = D >= 64 ? 128 : 64;  // bytes of an operand row: one swizzle span
+  static constexpr int kPanels = D > 64 ? 2 : 1;   // that a row of D takes
+  static constexpr int kQPanel = kTile * kRow;
+  static constexpr int kQBytes = kPanels * kQPanel;
+  static constexpr int kKVPanel = kPage * kRow;
+  static constexpr int kKBytes = kPanels * kKVPanel;
+  static constexpr int kStages = G == 4 ? (TILES == 2 ? 4 : 2) : 4;
+  static constexpr int kSoftmaxWarps = 4 * TILES;
+  static constexpr int kThreads = (kSoftmaxWarps + kUnpackWarps + 2) * 32;
+  static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
+  // Of a tile: two S / P buffers of 64 columns, then O.
+  static constexpr uint32_t kTileCols = 128 + D;
+  static_assert(TILES * kTileCols <= kTmemCols, "TMEM budget");
+  static constexpr int kInfoBytes = kStages * 16;
+  static constexpr int kBarBytes = 256;
+  static constexpr size_t kSmem =
+      1024 + (size_t)TILES * kQBytes + (size_t)kStages * 2 * kKBytes + kInfoBytes + kBarBytes;
+  static_assert(kSmem <= (TILES == 2 ? 232448 : 115000), "shared memory");
+};
+
+// What the unpacking warps tell the softmax about a page.
+struct PageInfo {
+  float scale;        // of its scores
+  int keys;           // 64, or 0: not a page
+  uint32_t nan_v[2];  // bit per key: a value that is not finite (pages that some rows see in part)
+};
+
+// What the swizzle of operand rows of ROW bytes flips in a byte's place in row r.
+template <int ROW>
+CTI_DEVICE int swizzle_of(int r) {
+  return ROW == 128 ? (r & 7) << 4 : (r >> 1 & 3) << 4;
+}
+
+// Matrix descriptor of an operand tile, 8-row atoms stacked along its rows: K-major
+// for Q and K, MN-major (each row a key) for V.  The tile is one atom wide, so
+// both offset fields hold an atom's bytes.
+template <int ROW>
+CTI_DEVICE uint64_t tile_desc(uint32_t saddr) {
+  constexpr uint64_t atom = 8 * ROW;
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | (atom >> 4) << 16 | (atom >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)(ROW == 128 ? 2 : 4) << 61;
+}
+
+CTI_DEVICE float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 16 TMEM columns and their wait in one statement, as the 32-column form.
+CTI_DEVICE void tmem_ld_x16_sync(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <typename T, int G, int TILES>
+__global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
+    kv4_tiles_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pages, const Args a,
+                     T* __restrict__ out) {
+  using Y = Type16<T>;
+  using Z = Shape<G, TILES>;
+  constexpr int D = Z::D;
+  constexpr int S = Z::kStages;
+  constexpr int kRow = Z::kRow;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + TILES * Z::kQBytes;  // [S] x {K, V}
+  PageInfo* info = reinterpret_cast<PageInfo*>(sKV + (size_t)S * 2 * Z::kKBytes);
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(info + S);  // [S] (4 unpacking warps)
+  uint64_t* kv_empty = kv_full + S;                           // [S] PV of every tile done
+  uint64_t* q_full = kv_empty + S;                            // [TILES] (4 softmax warps)
+  uint64_t* q_empty = q_full + TILES;                         // [TILES] last S done
+  uint64_t* o_empty = q_empty + TILES;                        // [TILES] O read (4 warps)
+  uint64_t* s_full = o_empty + TILES;                         // [TILES][2]
+  uint64_t* p_full = s_full + 2 * TILES;                      // [TILES][2] (4 warps)
+  uint64_t* pv_done = p_full + 2 * TILES;                     // [TILES][2]
+  uint64_t* drain = pv_done + 2 * TILES;                      // [2] each issuer's last
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 * S + 9 * TILES + 2) * 8 + 8 <= Z::kBarBytes, "barrier area");
+
+  const int warp = warp_id(), lane = lane_id();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&kv_full[i], kUnpackWarps);
+      mbar_init(&kv_empty[i], TILES);
+    }
+    for (int i = 0; i < TILES; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&o_empty[i], 4);
+    }
+    for (int i = 0; i < 2 * TILES; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == Z::kSoftmaxWarps + kUnpackWarps) {
+    tmem_alloc(tmem_slot, Z::kTmemCols);
+    tmem_relinquish();
+  }
+  grid_dependency_wait();  // everything read below may come from the kernel before
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // ---- the sequence ----
+  const int s = (int)a.by_kv_heads(blockIdx.x), kvh = (int)blockIdx.x - s * a.kv_heads;
+  const int group = a.group;
+  const int begin = __ldg(a.cu + s), end = __ldg(a.cu + s + 1);
+  const int len = max(__ldg(a.kv_lens + s), 0);
+  const bool sound = begin >= 0 && end <= a.tokens && end >= begin;
+  if (!sound && threadIdx.x == 0) raise_status(a.status, CTI_ERR_INVALID_ARG, s);
+  const int n_new = sound ? end - begin : 0;
+  const int first = len - n_new;
+  const int rows = n_new * group;
+  int limit = len;
+  if (limit > a.table_cols * kPage || (limit > 0 && a.num_pages <= 0)) {
+    if (threadIdx.x == 0 && rows > 0) raise_status(a.status, CTI_ERR_BOUNDS, s);
+    limit = a.num_pages <= 0 ? 0 : a.table_cols * kPage;
+  }
+  constexpr int kRows = TILES * kTile;
+  const int ntiles = (rows + kRows - 1) / kRows;
+
+  // The pages [p0, p0 + np) of this block for the rows from row0 on, and the
+  // keys that some row and that every row sees.
+  struct Range {
+    int p0, np, most, all;
+  };
+  auto range_of = [&](int tile) {
+    const int row0 = tile * kRows, row_last = min(rows, row0 + kRows) - 1;
+    Range r;
+    r.most = max(a.causal ? min(first + (int)a.by_group(row_last) + 1, limit) : limit, 0);
+    r.all = a.causal ? min(first + (int)a.by_group(row0) + 1, limit) : limit;
+    r.p0 = 0;
+    r.np = (r.most + kPage - 1) / kPage;
+    if (gridDim.z > 1) {  // the last block takes what the caller's bound left out
+      r.p0 = min(r.np, (int)blockIdx.z * a.chunk);
+      r.np = (blockIdx.z == gridDim.z - 1 ? r.np : min(r.np, r.p0 + a.chunk)) - r.p0;
+    }
+    return r;
+  };
+
+  if (warp < Z::kSoftmaxWarps) {
+    // ---------------- softmax ----------------
+    const int i = warp >> 2, wq = warp & 3;
+    const int r = wq * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16) + i * Z::kTileCols;
+    uint8_t* myq = sQ + i * Z::kQBytes;
+    const int swizzle = swizzle_of<kRow>(r);
+    int it = 0, g = 0;
+    bool ok = true;
+    for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y, ++it) {
+      const Range rg = range_of(tile);
+      const int row = tile * kRows + i * kTile + r;
+      const bool live = row < rows;
+      const int tok = live ? (int)a.by_group(row) : 0;
+      const int head = kvh * group + (live ? row - tok * group : 0);
+      const int64_t at = (int64_t)(begin + tok) * a.heads + head;
+      const int sees = !live ? 0 : a.causal ? min(first + tok + 1, limit) : limit;
+      // Queries: the row's largest magnitude, then fp16 in [2^14, 2^15) at most.
+      const uint4* src =
+          reinterpret_cast<const uint4*>(q + (begin + tok) * a.q_stride + (int64_t)head * D);
+      float most_q = 0.0f;
+      if (live) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 v = __ldg(src + c);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            most_q = max3f(most_q, fabsf(Y::low(w[j])), fabsf(Y::high(w[j])));
+        }
+      }
+      int k = 14 + 127 - (int)(__float_as_uint(most_q) >> 23);
+      k = most_q > 0.0f ? max(-100, min(k, 100)) : 0;
+      const float up = __uint_as_float((uint32_t)(127 + k) << 23) * (a.negate ? -1.0f : 1.0f);
+      const float down = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait(&q_empty[i], (uint32_t)(it & 1) ^ 1u, a.status, 0x710, abort_flag)))
+        break;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live) v = __ldg(src + c);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          h[j] = Type16<__half>::pack(Y::low(w[j]) * up, Y::high(w[j]) * up);
+        const int panel = c * 16 / kRow, off = c * 16 % kRow;
+        *reinterpret_cast<uint4*>(myq + panel * Z::kQPanel + r * kRow + (off ^ swizzle)) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[i]);
+
+      float m = -INFINITY, l = 0.0f;  // m in powers of 2
+      for (int j = 0; j < rg.np; ++j, ++g) {
+        const int b = g & 1, st = g % S;
+        // kv_full has completed once s_full has; waited for here to see the info.
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait(&kv_full[st], (uint32_t)((g / S) & 1), a.status, 0x711,
+                                  abort_flag) &&
+                            mbar_wait(&s_full[2 * i + b], (uint32_t)((g >> 1) & 1), a.status,
+                                      0x712, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t sb = lanes + 64u * b;
+        uint32_t v[2][32];
+        tmem_ld_32x32b_2x32_sync(sb, sb + 32, v[0], v[1]);
+        const PageInfo pi = info[st];
+        const int key0 = (rg.p0 + j) * kPage;
+        if (pi.nan_v[0] | pi.nan_v[1]) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (pi.nan_v[c] >> e & 1) v[c][e] = 0x7fffffffu;
+        }
+        const int lim = min(sees - key0, pi.keys);
+        if (!__all_sync(0xffffffffu, lim >= kPage)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * c + e >= lim) v[c][e] = __float_as_uint(-INFINITY);
+        }
+        float mx = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            mx = max3f(mx, __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+            mx1 = max3f(mx1, __uint_as_float(v[c][e + 2]), __uint_as_float(v[c][e + 3]));
+          }
+        const float factor = fmaxf(down * pi.scale, 1e-37f);  // not 0: -inf stays -inf
+        mx = fmaxf(mx, mx1) * factor;
+        float corr = 1.0f;
+        if (mx - m > kSlack) {
+          corr = ex2_approx(m - mx);
+          m = mx;
+        }
+        if (__any_sync(0xffffffffu, corr != 1.0f)) {
+          l *= corr;
+          if (j > 0) {
+            // O holds the tile's pages up to g - 1: wait for their PV.
+            if (!__all_sync(0xffffffffu,
+                            mbar_wait(&pv_done[2 * i + (b ^ 1)], (uint32_t)(((g - 1) >> 1) & 1),
+                                      a.status, 0x713, abort_flag))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 2 * G; ++c) {
+              uint32_t o[16];
+              tmem_ld_x16_sync(lanes + 128 + 16 * c, o);
+#pragma unroll
+              for (int d = 0; d < 16; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * corr);
+              tmem_st_32x32b_x16(lanes + 128 + 16 * c, o);
+            }
+          }
+        }
+        const float noff = m == -INFINITY ? 0.0f : -m;
+        const uint64_t factor2 = f2_pack(factor, factor), noff2 = f2_pack(noff, noff);
+        uint64_t sum_a = f2_pack(0.0f, 0.0f), sum_b = sum_a;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c][2 * e]),
+                                     __uint_as_float(v[c][2 * e + 1])),
+                             factor2, noff2),
+                      x0, x1);
+            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            if (e & 1) sum_b = f2_add(sum_b, f2_pack(p0, p1));
+            else sum_a = f2_add(sum_a, f2_pack(p0, p1));
+            pk[e] = Y::pack(p0, p1);
+          }
+          tmem_st_32x32b_x16(sb + 16 * c, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * i + b]);
+        float s0, s1;
+        f2_unpack(f2_add(sum_a, sum_b), s0, s1);
+        l += s0 + s1;
+      }
+      if (!ok) break;
+      // ---- the rows ----
+      if (rg.np > 0) {
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait(&pv_done[2 * i + ((g - 1) & 1)], (uint32_t)(((g - 1) >> 1) & 1),
+                                  a.status, 0x714, abort_flag)))
+          break;
+        tc_fence_after();
+      }
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int64_t ws = (int64_t)blockIdx.z * a.tokens * a.heads + at;
+#pragma unroll 1
+      for (int c = 0; c < 2 * G; ++c) {
+        uint32_t o[16];
+        if (rg.np > 0) {
+          tmem_ld_x16_sync(lanes + 128 + 16 * c, o);
+        } else {
+#pragma unroll
+          for (int d = 0; d < 16; ++d) o[d] = 0;
+        }
+        if (!live) continue;
+        if (gridDim.z == 1) {
+          uint4* dst = reinterpret_cast<uint4*>(out + at * D + 16 * c);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              w[x] = Y::pack(__uint_as_float(o[8 * d + 2 * x]) * inv,
+                             __uint_as_float(o[8 * d + 2 * x + 1]) * inv);
+            dst[d] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else if (rg.np > 0) {
+          uint4* dst = reinterpret_cast<uint4*>(a.ws_o + ws * D + 16 * c);
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            dst[d] = make_uint4(o[4 * d], o[4 * d + 1], o[4 * d + 2], o[4 * d + 3]);
+        }
+      }
+      if (live && gridDim.z > 1) a.ws_ml[ws] = make_float2(m, l);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[i]);
+    }
+  } else if (warp < Z::kSoftmaxWarps + kUnpackWarps) {
+    // ---------------- unpacking ----------------
+    const int dw = warp - Z::kSoftmaxWarps;
+    const bool keys = dw < 2;
+    const int half = dw & 1;  // of the page's tokens: vectors half G .. half G + G - 1
+    const int hi = lane >> 2, lo = lane & 3;
+    const int32_t* table = a.table + s * a.table_stride;
+    const uint8_t* base = pages + (int64_t)kvh * block_bytes(G);
+    const int64_t page_stride = (int64_t)a.kv_heads * block_bytes(G);
+    // Bytes of this lane's pieces in an octet of rows, for an even group; an odd
+    // one differs in bit 6.  Keys: row hi, dims 8 lo .. + 7.  Values: rows
+    // 2 lo and 2 lo + 1, dims 4 hi .. + 3.
+    const int at_k = hi * kRow + (16 * lo ^ swizzle_of<kRow>(hi));
+    const int at_v0 = 2 * lo * kRow + (8 * hi ^ swizzle_of<kRow>(2 * lo));
+    const int at_v1 = (2 * lo + 1) * kRow + (8 * hi ^ swizzle_of<kRow>(2 * lo + 1));
+    int g = 0;
+    bool ok = true;
+    for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y) {
+      const Range rg = range_of(tile);
+      int ids = 0;
+      for (int j = 0; j < rg.np; ++j, ++g) {
+        if ((j & 31) == 0) {
+          ids = j + lane < rg.np ? __ldg(table + rg.p0 + j + lane) : 0;
+          if (ids < 0 || ids >= a.num_pages) {
+            raise_status(a.status, CTI_ERR_BOUNDS, s);
+            ids = -1;
+          }
+        }
+        int id = __shfl_sync(0xffffffffu, ids, j & 31);
+        const bool is_page = id >= 0;
+        if (!is_page) id = 0;
+        const uint8_t* blk = base + id * page_stride;
+        const int key0 = (rg.p0 + j) * kPage;
+        const int most = is_page ? rg.most - key0 : 0;  // keys of the page that some row sees
+        const bool whole = is_page && key0 + kPage <= rg.all;
+        const int st = g % S;
+        uint8_t* dst = sKV + (size_t)st * 2 * Z::kKBytes;
+        uint4 w4[G];
+        if (keys) {
+          uint32_t meta[G][4];
+          uint32_t scan[2 * G];
+#pragma unroll
+          for (int x = 0; x < G; ++x) {
+            const int v = half * G + x;
+            w4[x] = __ldg(reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16));
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int nt = (4 * v + y) / G, gr = (4 * v + y) % G;
+              meta[x][y] = __ldg(reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) +
+                                 (8 * nt + hi) * G + gr);
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 2 * G; ++x)
+            scan[x] = __ldg(reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) + 32 * x + lane);
+          // The page's scaling: every key warp finds the same.
+          float most_k = 0.0f;
+#pragma unroll
+          for (int x = 0; x < 2 * G; ++x) {
+            const float sx = Y::low(scan[x]), bx = Y::high(scan[x]);
+            const float z = fmaxf(fabsf(fmaf(16.0f, sx, bx)), fabsf(fmaf(31.0f, sx, bx)));
+            if (z <= FLT_MAX && (32 * x + lane) / G < most) most_k = fmaxf(most_k, z);
+          }
+          const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most_k));
+          int e = 0;
+          if (top != 0 && (top < 0x3c800000u || top >= 0x47000000u))  // [2^-6, 2^15)
+            e = max(-100, min((int)(top >> 23) - 127, 100));
+          const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[st], (uint32_t)((g / S) & 1) ^ 1u,
+                                                 a.status, 0x720, abort_flag));
+          if (!ok) break;
+          if (half == 0 && lane == 0) {
+            info[st].scale = __uint_as_float((uint32_t)(127 + e) << 23);
+            info[st].keys = is_page ? kPage : 0;
+          }
+#pragma unroll
+          for (int x = 0; x < G; ++x) {
+            const uint32_t w[4] = {w4[x].x, w4[x].y, w4[x].z, w4[x].w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int nt = (4 * (half * G + x) + y) / G, gr = (4 * (half * G + x) + y) % G;
+              const int tau = 8 * nt + hi;
+              const float sx = Y::low(meta[x][y]) * down, bx = Y::high(meta[x][y]) * down;
+              uint32_t s2 = Type16<__half>::pack(sx, sx), b2 = Type16<__half>::pack(bx, bx);
+              if (tau >= most) s2 = b2 = 0;
+              uint32_t o[4];
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+                o[p] = fma2<__half>(code_pair<__half>(w[y], p), s2, b2);
+              *reinterpret_cast<uint4*>(dst + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow +
+                                        (at_k ^ 64 * (gr & 1))) =
+                  make_uint4(o[0], o[1], o[2], o[3]);
+            }
+          }
+        } else {
+          uint2 meta[G][4];
+#pragma unroll
+          for (int x = 0; x < G; ++x) {
+            const int v = half * G + x;
+            w4[x] = __ldg(
+                reinterpret_cast<const uint4*>(blk + v_codes_at(G) + (v * 32 + lane) * 16));
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int nt = (4 * v + y) / G, gr = (4 * v + y) % G;
+              meta[x][y] = __ldg(reinterpret_cast<const uint2*>(blk + v_meta_at(G)) +
+                                 (4 * nt + lo) * G + gr);
+            }
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[st], (uint32_t)((g / S) & 1) ^ 1u,
+                                                 a.status, 0x721, abort_flag));
+          if (!ok) break;
+          uint32_t nan_bits = 0;
+          if (!whole) {
+            // Behind the last key: zero.  Not finite: zero, and the softmax is told.
+#pragma unroll
+            for (int x = 0; x < G; ++x)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const int nt = (4 * (half * G + x) + y) / G;
+                const int tau = 8 * nt + 2 * lo;
+                uint2& mv = meta[x][y];
+                constexpr uint32_t inf = Inf16<T>::kBits;
+                const bool n0 = tau < most && ((mv.x & inf) == inf || (mv.y & inf) == inf);
+                const bool n1 = tau + 1 < most &&
+                                ((mv.x >> 16 & inf) == inf || (mv.y >> 16 & inf) == inf);
+                const uint32_t keep = (n0 || tau >= most ? 0u : 0xffffu) |
+                                      (n1 || tau + 1 >= most ? 0u : 0xffff0000u);
+                mv.x &= keep;
+                mv.y &= keep;
+                if (n0) nan_bits |= 1u << (tau & 31);
+                if (n1) nan_bits |= 1u << ((tau + 1) & 31);
+              }
+            // The groups of a key must all go, wherever one is not finite.
+            nan_bits = __reduce_or_sync(0xffffffffu, nan_bits);
+          }
+          if (lane == 0) info[st].nan_v[half] = nan_bits;
+          uint8_t* vt = dst + Z::kKBytes;
+#pragma unroll
+          for (int x = 0; x < G; ++x) {
+            const uint32_t w[4] = {w4[x].x, w4[x].y, w4[x].z, w4[x].w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int nt = (4 * (half * G + x) + y) / G, gr = (4 * (half * G + x) + y) % G;
+              uint32_t o[4];
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+                o[p] = fma2<T>(code_pair<T>(w[y], p), meta[x][y].x, meta[x][y].y);
+              uint8_t* to = vt + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow;
+              *reinterpret_cast<uint2*>(to + (at_v0 ^ 64 * (gr & 1))) =
+                  make_uint2(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410));
+              *reinterpret_cast<uint2*>(to + (at_v1 ^ 64 * (gr & 1))) =
+                  make_uint2(__byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[st]);
+      }
+    }
+  } else if (warp == Z::kSoftmaxWarps + kUnpackWarps) {
+    // ---------------- S issuer ----------------
+    if (lane == 0) {
+      // fp16 operands, fp32 sums; M 128, N 64
+      constexpr uint32_t id_s = (1u << 4) | ((kPage >> 3) << 17) | ((kTile >> 4) << 24);
+      const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
+      int it = 0, g = 0;
+      bool ok = true, any = false;
+      for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y, ++it) {
+        const Range rg = range_of(tile);
+        for (int i = 0; ok && i < TILES; ++i)
+          ok = mbar_wait(&q_full[i], (uint32_t)(it & 1), a.status, 0x730, abort_flag);
+        for (int j = 0; ok && j < rg.np; ++j, ++g) {
+          const int st = g % S, b = g & 1;
+          ok = mbar_wait(&kv_full[st], (uint32_t)((g / S) & 1), a.status, 0x731, abort_flag);
+          for (int i = 0; ok && i < TILES; ++i) {
+            // The buffer's last reader is the PV of page g - 2.
+            ok = mbar_wait(&pv_done[2 * i + b], (uint32_t)((g >> 1) & 1) ^ 1u, a.status, 0x732,
+                           abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t qa = q_addr + i * Z::kQBytes, ka = kv_addr + st * 2 * Z::kKBytes;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const int panel = kk * 32 / kRow, off = kk * 32 % kRow;
+              umma_bf16(tmem + i * Z::kTileCols + 64u * b,
+                        tile_desc<kRow>(qa + panel * Z::kQPanel + off),
+                        tile_desc<kRow>(ka + panel * Z::kKVPanel + off), id_s, kk != 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[2 * i + b]);
+            any = true;
+          }
+        }
+        if (!ok) break;
+        for (int i = 0; i < TILES; ++i) {
+          if (any) umma_commit(&q_empty[i]);
+          else mbar_arrive(&q_empty[i]);
+        }
+      }
+      if (any) {
+        umma_commit(&drain[0]);
+        mbar_wait(&drain[0], 0, a.status, 0x733, nullptr);
+      }
+    }
+  } else {
+    // ---------------- PV issuer ----------------
+    if (lane == 0) {
+      constexpr uint32_t type = sizeof(T) == 2 && Type16<T>::kShift == 3 ? 1u : 0u;  // bf16, fp16
+      constexpr int kN = D < 64 ? D : 64;  // head dims of one instruction: a panel's
+      constexpr uint32_t id_pv = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) |
+                                 ((kN >> 3) << 17) | ((kTile >> 4) << 24);  // V MN-major
+      const uint32_t kv_addr = smem_u32(sKV);
+      int it = 0, g = 0;
+      bool ok = true, any = false;
+      for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y, ++it) {
+        const Range rg = range_of(tile);
+        for (int j = 0; ok && j < rg.np; ++j, ++g) {
+          const int st = g % S, b = g & 1;
+          for (int i = 0; ok && i < TILES; ++i) {
+            if (j == 0)  // the last tile's O has been read
+              ok = mbar_wait(&o_empty[i], (uint32_t)(it & 1) ^ 1u, a.status, 0x740, abort_flag);
+            ok = ok && mbar_wait(&p_full[2 * i + b], (uint32_t)((g >> 1) & 1), a.status, 0x741,
+                                 abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t pbuf = tmem + i * Z::kTileCols + 64u * b;
+            const uint32_t ocol = tmem + i * Z::kTileCols + 128u;
+            const uint32_t va = kv_addr + st * 2 * Z::kKBytes + Z::kKBytes;
+#pragma unroll
+            for (int kk = 0; kk < kPage / 16; ++kk)
+#pragma unroll
+              for (int panel = 0; panel < Z::kPanels; ++panel)
+                umma_bf16_ts(ocol + 64u * panel, pbuf + kk * 8,
+                             tile_desc<kRow>(va + panel * Z::kKVPanel + kk * 16 * kRow), id_pv,
+                             j == 0 && kk == 0 ? 0u : 1u);
+            umma_commit(&pv_done[2 * i + b]);
+            umma_commit(&kv_empty[st]);
+            any = true;
+          }
+        }
+        // A tile without pages leaves O alone, but its turn counts.
+        for (int i = 0; ok && rg.np == 0 && i < TILES; ++i)
+          ok = mbar_wait(&o_empty[i], (uint32_t)(it & 1) ^ 1u, a.status, 0x742, abort_flag);
+      }
+      if (any) {
+        umma_commit(&drain[1]);
+        mbar_wait(&drain[1], 0, a.status, 0x743, nullptr);
+      }
+    }
+  }
+
+  __syncthreads();
+  if (warp == Z::kSoftmaxWarps + kUnpackWarps) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, Z::kTmemCols);
+  }
+}
+
+template <typename T, int G, int TILES>
+int launch(const void* q, const void* pages, const Args& a, int64_t y, int splits, void* out,
+           cudaStream_t s) {
+  using Z = Shape<G, TILES>;
+  static uint64_t configured = 0;
+  if (ensure_smem_limit(kv4_tiles_kernel<T, G, TILES>, (int)Z::kSmem, configured) != cudaSuccess)
+    return CTI_ERR_CUDA;
+  const dim3 grid((unsigned)((int64_t)a.num_seqs * a.kv_heads), (unsigned)(y < 65535 ? y : 65535),
+                  (unsigned)splits);
+  return launch_dependent(kv4_tiles_kernel<T, G, TILES>, grid, dim3(Z::kThreads), Z::kSmem, s,
+                          static_cast<const T*>(q), static_cast<const uint8_t*>(pages), a,
+                          static_cast<T*>(out)) == cudaSuccess
+             ? CTI_OK
+             : CTI_ERR_CUDA;
+}
+
+template <typename T, int G>
+int launch_shape(const void* q, const void* pages, const Args& a, int tiles, int64_t y, int splits,
+                 void* out, cudaStream_t s) {
+  return tiles == 2 ? launch<T, G, 2>(q, pages, a, y, splits, out, s)
+                    : launch<T, G, 1>(q, pages, a, y, splits, out, s);
+}
+
+template <typename T>
+int launch_dim(const void* q, const void* pages, const Args& a, int head_dim, int tiles, int64_t y,
+               int splits, void* out, cudaStream_t s) {
+  return head_dim == 32   ? launch_shape<T, 1>(q, pages, a, tiles, y, splits, out, s)
+         : head_dim == 64 ? launch_shape<T, 2>(q, pages, a, tiles, y, splits, out, s)
+                          : launch_shape<T, 4>(q, pages, a, tiles, y, splits, out, s);
+}
+
+}  // namespace
+
+int kv4::launch_tiles(const void* q, const void* pages, const Args& a, int dtype, int head_dim,
+                      int tiles, int64_t y, int splits, void* out, cudaStream_t s) {
+  return dtype == CTI_DTYPE_BF16
+             ? launch_dim<__nv_bfloat16>(q, pages, a, head_dim, tiles, y, splits, out, s)
+             : launch_dim<__half>(q, pages, a, head_dim, tiles, y, splits, out, s);
+}
+
+}  // namespace cti

@@ -34,16 +34,22 @@ def attention(q, k, v, new, total, causal, scale):
     """float64 attention of the last new[i] tokens of every sequence over its total[i]; q packs the
     new tokens, k and v (what the cache holds) all of them.  Returns (out, tol): tol bounds the
     error of an implementation that keeps scores, maxima, sums and outputs in fp32, rounds the
-    weights p and the values once each to the tensors' type, and rounds the output.
+    weights p and the values once each to the tensors' type, may round the keys to 11 bits, and
+    rounds the output.
 
     With e = eps / 2 of the type, u = 2^-24 of fp32, A = sum p |v|:
       p's and v's rounding: 2 e A; the output's: e |out|;
       p below the type's normals: half its smallest step for each key, over a sum l >= 1;
       a score is off by at most d: 2 d A in the weights and their sum (first order; d << 1).
-    d: the products q (16 + n) s and q b are summed apart in fp32, up to head_dim + 4 terms with
-    magnitudes up to |q| (|k| + 2 |b|) with |b| <= 48 s + |k|; taking |k| + 2 |b| <= 16 max |k|
-    over the group bounds that by 16 sum |q| kmax (head_dim + 8) u, and the sum of q over a group, split
-    into two numbers of the type, is short by e^2 of itself: 2 e^2 16 sum |q| kmax."""
+    d, for a score q . k with k = (16 + n) s + b:
+      - q (16 + n) s and q b may be summed apart, in fp32, over up to head_dim + 8 terms.  In a
+        group with largest magnitude kmax, s <= 2 kmax / 15 and |b| <= kmax + 16 s, so 31 s + |b| <
+        8 kmax: below 16 sum |q| kmax (head_dim + 8) u;
+      - the sum of q over a group may be split into two numbers of the type, short by e^2 of
+        itself, twice (for s and b): below 2 e^2 16 sum |q| kmax;
+      - keys rounded to 11 bits: 2^-12 sum |q| |k|; their scales may lie below fp16's normals,
+        31 2^-25 < 2^-20 for each, times a common factor where the largest key is above 1:
+        2^-20 max(1, max |k|) sum |q|."""
     dtype = q.dtype
     e, u = rounding(dtype), 2.0 ** -24
     tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
@@ -61,6 +67,9 @@ def attention(q, k, v, new, total, causal, scale):
             -1, -1, -1, GROUP).flatten(-2)
         d = torch.einsum("nhd,lhd->hnl", qs.abs(), kmax) * abs(scale) * 16 * (
             (D + 8) * u + 2 * e * e)
+        d = d + abs(scale) * (2.0 ** -12 * torch.einsum("nhd,lhd->hnl", qs.abs(), ks.abs()) +
+                              2.0 ** -20 * max(1.0, float(torch.nan_to_num(ks).abs().max()) if L
+                                               else 0.0) * qs.abs().sum(-1).T[:, :, None])
         if causal:
             pos = L - n + torch.arange(n)
             s = s.masked_fill(torch.arange(L)[None, :] > pos[:, None], float("-inf"))
