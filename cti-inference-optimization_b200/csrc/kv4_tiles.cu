@@ -9,10 +9,9 @@
 //          a power of two.  Per page: the row's 64 scores from TMEM, masked;
 //          p = 2^(x - m), m raised (O and l rescaled) only when a score exceeds
 //          it by 2^8; P in 16 bits back over the scores.
-//   4 warps  unpacking: two take a page's keys, two its values, 16 bytes a lane
-//          at a time straight from global memory (requested before they wait
-//          for a free stage), to 16 bits in the swizzled layout of the matrix
-//          operands.  Two tiles share the work.
+//   4 or 8 warps  unpacking: half of them take a page's keys, half its values,
+//          from a ring of page blocks that bulk copies fill, to 16 bits in the
+//          swizzled layout of the matrix operands.  Two tiles share the work.
 //   1 warp issues S = Q K^T (M 128, N 64), 1 warp O += P V with P from TMEM and
 //          V as an MN-major operand.
 // Keys are rounded to fp16 (11 bits, as the queries hold 8 or 11) after a
@@ -31,7 +30,6 @@ namespace {
 using namespace kv4;
 
 constexpr int kTile = 128;
-constexpr int kUnpackWarps = 4;
 
 template <int G, int TILES>
 struct Shape {
@@ -42,25 +40,29 @@ struct Shape {
   static constexpr int kQBytes = kPanels * kQPanel;
   static constexpr int kKVPanel = kPage * kRow;
   static constexpr int kKBytes = kPanels * kKVPanel;
-  static constexpr int kStages = G == 4 ? (TILES == 2 ? 4 : 2) : 4;
+  static constexpr int kStages = G == 4 ? (TILES == 2 ? 3 : 2) : G == 2 ? 3 : 4;
+  static constexpr int kRaw = G == 4 && TILES == 1 ? 1 : 3;  // page blocks in flight
   static constexpr int kSoftmaxWarps = 4 * TILES;
+  static constexpr int kUnpackWarps = TILES == 2 && G > 1 ? 8 : 4;
   static constexpr int kThreads = (kSoftmaxWarps + kUnpackWarps + 2) * 32;
   static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
   // Of a tile: two S / P buffers of 64 columns, then O.
   static constexpr uint32_t kTileCols = 128 + D;
   static_assert(TILES * kTileCols <= kTmemCols, "TMEM budget");
-  static constexpr int kInfoBytes = kStages * 16;
-  static constexpr int kBarBytes = 256;
+  static constexpr int kInfoBytes = kStages * 48;
+  static constexpr int kBarBytes = 320;
   static constexpr size_t kSmem =
-      1024 + (size_t)TILES * kQBytes + (size_t)kStages * 2 * kKBytes + kInfoBytes + kBarBytes;
+      1024 + (size_t)TILES * kQBytes + (size_t)kStages * 2 * kKBytes +
+                                  (size_t)kRaw * block_bytes(G) + kInfoBytes + kBarBytes;
   static_assert(kSmem <= (TILES == 2 ? 232448 : 115000), "shared memory");
 };
 
 // What the unpacking warps tell the softmax about a page.
-struct PageInfo {
+struct alignas(16) PageInfo {
   float scale;        // of its scores
   int keys;           // 64, or 0: not a page
-  uint32_t nan_v[2];  // bit per key: a value that is not finite (pages that some rows see in part)
+  int pad[2];
+  uint64_t nan_v[4];  // bit per key: a value that is not finite (pages that some rows see in part)
 };
 
 // What the swizzle of operand rows of ROW bytes flips in a byte's place in row r.
@@ -77,6 +79,14 @@ CTI_DEVICE uint64_t tile_desc(uint32_t saddr) {
   constexpr uint64_t atom = 8 * ROW;
   return (uint64_t)((saddr >> 4) & 0x3fffu) | (atom >> 4) << 16 | (atom >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)(ROW == 128 ? 2 : 4) << 61;
+}
+
+CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
 }
 
 CTI_DEVICE float max3f(float a, float b, float c) {
@@ -105,15 +115,16 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
   using Y = Type16<T>;
   using Z = Shape<G, TILES>;
   constexpr int D = Z::D;
-  constexpr int S = Z::kStages;
+  constexpr int S = Z::kStages, R = Z::kRaw;
   constexpr int kRow = Z::kRow;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + TILES * Z::kQBytes;  // [S] x {K, V}
-  PageInfo* info = reinterpret_cast<PageInfo*>(sKV + (size_t)S * 2 * Z::kKBytes);
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(info + S);  // [S] (4 unpacking warps)
+  uint8_t* sRaw = sKV + (size_t)S * 2 * Z::kKBytes;  // [R] page blocks
+  PageInfo* info = reinterpret_cast<PageInfo*>(sRaw + (size_t)R * block_bytes(G));
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(info + S);  // [S] (unpacking warps)
   uint64_t* kv_empty = kv_full + S;                           // [S] PV of every tile done
   uint64_t* q_full = kv_empty + S;                            // [TILES] (4 softmax warps)
   uint64_t* q_empty = q_full + TILES;                         // [TILES] last S done
@@ -121,15 +132,17 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
   uint64_t* s_full = o_empty + TILES;                         // [TILES][2]
   uint64_t* p_full = s_full + 2 * TILES;                      // [TILES][2] (4 warps)
   uint64_t* pv_done = p_full + 2 * TILES;                     // [TILES][2]
-  uint64_t* drain = pv_done + 2 * TILES;                      // [2] each issuer's last
+  uint64_t* raw_full = pv_done + 2 * TILES;                   // [R]
+  uint64_t* raw_empty = raw_full + R;                         // [R] (unpacking warps)
+  uint64_t* drain = raw_empty + R;                            // [2] each issuer's last
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * S + 9 * TILES + 2) * 8 + 8 <= Z::kBarBytes, "barrier area");
+  static_assert((2 * S + 9 * TILES + 2 * R + 2) * 8 + 8 <= Z::kBarBytes, "barrier area");
 
   const int warp = warp_id(), lane = lane_id();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(&kv_full[i], kUnpackWarps);
+      mbar_init(&kv_full[i], Z::kUnpackWarps);
       mbar_init(&kv_empty[i], TILES);
     }
     for (int i = 0; i < TILES; ++i) {
@@ -142,12 +155,16 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
       mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
     }
+    for (int i = 0; i < R; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], Z::kUnpackWarps);
+    }
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == Z::kSoftmaxWarps + kUnpackWarps) {
+  if (warp == Z::kSoftmaxWarps + Z::kUnpackWarps) {
     tmem_alloc(tmem_slot, Z::kTmemCols);
     tmem_relinquish();
   }
@@ -267,12 +284,13 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         tmem_ld_32x32b_2x32_sync(sb, sb + 32, v[0], v[1]);
         const PageInfo pi = info[st];
         const int key0 = (rg.p0 + j) * kPage;
-        if (pi.nan_v[0] | pi.nan_v[1]) {
+        const uint64_t nan_v = pi.nan_v[0] | pi.nan_v[1] | pi.nan_v[2] | pi.nan_v[3];
+        if (nan_v) {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (pi.nan_v[c] >> e & 1) v[c][e] = 0x7fffffffu;
+              if (nan_v >> (32 * c + e) & 1) v[c][e] = 0x7fffffffu;
         }
         const int lim = min(sees - key0, pi.keys);
         if (!__all_sync(0xffffffffu, lim >= kPage)) {
@@ -390,11 +408,13 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_empty[i]);
     }
-  } else if (warp < Z::kSoftmaxWarps + kUnpackWarps) {
+  } else if (warp < Z::kSoftmaxWarps + Z::kUnpackWarps) {
     // ---------------- unpacking ----------------
+    constexpr int kEach = Z::kUnpackWarps / 2;  // warps for keys, and for values
+    constexpr int kVecs = 2 * G / kEach;        // vectors of codes that each takes
     const int dw = warp - Z::kSoftmaxWarps;
-    const bool keys = dw < 2;
-    const int half = dw & 1;  // of the page's tokens: vectors half G .. half G + G - 1
+    const bool keys = dw < kEach;
+    const int part = keys ? dw : dw - kEach;
     const int hi = lane >> 2, lo = lane & 3;
     const int32_t* table = a.table + s * a.table_stride;
     const uint8_t* base = pages + (int64_t)kvh * block_bytes(G);
@@ -405,7 +425,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
     const int at_k = hi * kRow + (16 * lo ^ swizzle_of<kRow>(hi));
     const int at_v0 = 2 * lo * kRow + (8 * hi ^ swizzle_of<kRow>(2 * lo));
     const int at_v1 = (2 * lo + 1) * kRow + (8 * hi ^ swizzle_of<kRow>(2 * lo + 1));
-    int g = 0;
+    int g = 0, asked = 0;  // pages unpacked, and (the first of these warps) copies asked for
     bool ok = true;
     for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y) {
       const Range rg = range_of(tile);
@@ -418,38 +438,44 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             ids = -1;
           }
         }
-        int id = __shfl_sync(0xffffffffu, ids, j & 31);
-        const bool is_page = id >= 0;
-        if (!is_page) id = 0;
-        const uint8_t* blk = base + id * page_stride;
+        // The first warp keeps R pages of these 32 in flight.
+        if (dw == 0) {
+          const int ahead = min(g + R, g - j + min(rg.np, (j & ~31) + 32));
+          for (; asked < ahead; ++asked) {
+            const int slot = asked % R, id = __shfl_sync(0xffffffffu, ids, (asked - g + j) & 31);
+            ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[slot],
+                                                   (uint32_t)((asked / R) & 1) ^ 1u, a.status,
+                                                   0x722, abort_flag));
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&raw_full[slot], block_bytes(G));
+              bulk_load(sRaw + slot * block_bytes(G), base + max(id, 0) * page_stride,
+                        block_bytes(G), &raw_full[slot]);
+            }
+          }
+          if (!ok) break;
+        }
+        const bool is_page = __shfl_sync(0xffffffffu, ids, j & 31) >= 0;
         const int key0 = (rg.p0 + j) * kPage;
         const int most = is_page ? rg.most - key0 : 0;  // keys of the page that some row sees
         const bool whole = is_page && key0 + kPage <= rg.all;
         const int st = g % S;
         uint8_t* dst = sKV + (size_t)st * 2 * Z::kKBytes;
-        uint4 w4[G];
+        const uint8_t* blk = sRaw + (g % R) * block_bytes(G);
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&raw_full[g % R], (uint32_t)((g / R) & 1), a.status, 0x720,
+                                  abort_flag) &&
+                            mbar_wait(&kv_empty[st], (uint32_t)((g / S) & 1) ^ 1u, a.status,
+                                      0x721, abort_flag));
+        if (!ok) break;
         if (keys) {
-          uint32_t meta[G][4];
-          uint32_t scan[2 * G];
-#pragma unroll
-          for (int x = 0; x < G; ++x) {
-            const int v = half * G + x;
-            w4[x] = __ldg(reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16));
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const int nt = (4 * v + y) / G, gr = (4 * v + y) % G;
-              meta[x][y] = __ldg(reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) +
-                                 (8 * nt + hi) * G + gr);
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < 2 * G; ++x)
-            scan[x] = __ldg(reinterpret_cast<const uint32_t*>(blk + k_meta_at(G)) + 32 * x + lane);
           // The page's scaling: every key warp finds the same.
+          const uint32_t* km = reinterpret_cast<const uint32_t*>(blk + k_meta_at(G));
           float most_k = 0.0f;
 #pragma unroll
           for (int x = 0; x < 2 * G; ++x) {
-            const float sx = Y::low(scan[x]), bx = Y::high(scan[x]);
+            const uint32_t w = km[32 * x + lane];
+            const float sx = Y::low(w), bx = Y::high(w);
             const float z = fmaxf(fabsf(fmaf(16.0f, sx, bx)), fabsf(fmaf(31.0f, sx, bx)));
             if (z <= FLT_MAX && (32 * x + lane) / G < most) most_k = fmaxf(most_k, z);
           }
@@ -458,99 +484,96 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
           if (top != 0 && (top < 0x3c800000u || top >= 0x47000000u))  // [2^-6, 2^15)
             e = max(-100, min((int)(top >> 23) - 127, 100));
           const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-          ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[st], (uint32_t)((g / S) & 1) ^ 1u,
-                                                 a.status, 0x720, abort_flag));
-          if (!ok) break;
-          if (half == 0 && lane == 0) {
+          if (part == 0 && lane == 0) {
             info[st].scale = __uint_as_float((uint32_t)(127 + e) << 23);
             info[st].keys = is_page ? kPage : 0;
           }
-#pragma unroll
-          for (int x = 0; x < G; ++x) {
-            const uint32_t w[4] = {w4[x].x, w4[x].y, w4[x].z, w4[x].w};
+#pragma unroll 1
+          for (int v = part * kVecs; v < (part + 1) * kVecs; ++v) {
+            const uint4 w4 = *reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            const int nt0 = 4 * v / G;
+            const uint32_t* mv = km + (8 * nt0 + hi) * G;
+            uint8_t* to = dst + nt0 * 8 * kRow;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const int nt = (4 * (half * G + x) + y) / G, gr = (4 * (half * G + x) + y) % G;
-              const int tau = 8 * nt + hi;
-              const float sx = Y::low(meta[x][y]) * down, bx = Y::high(meta[x][y]) * down;
+              const int nt = y / G, gr = y % G;  // nt: octets past nt0
+              const uint32_t meta = mv[8 * nt * G + gr];
+              const float sx = Y::low(meta) * down, bx = Y::high(meta) * down;
               uint32_t s2 = Type16<__half>::pack(sx, sx), b2 = Type16<__half>::pack(bx, bx);
-              if (tau >= most) s2 = b2 = 0;
+              if (8 * (nt0 + nt) + hi >= most) s2 = b2 = 0;
               uint32_t o[4];
 #pragma unroll
               for (int p = 0; p < 4; ++p)
                 o[p] = fma2<__half>(code_pair<__half>(w[y], p), s2, b2);
-              *reinterpret_cast<uint4*>(dst + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow +
+              *reinterpret_cast<uint4*>(to + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow +
                                         (at_k ^ 64 * (gr & 1))) =
                   make_uint4(o[0], o[1], o[2], o[3]);
             }
           }
         } else {
-          uint2 meta[G][4];
-#pragma unroll
-          for (int x = 0; x < G; ++x) {
-            const int v = half * G + x;
-            w4[x] = __ldg(
-                reinterpret_cast<const uint4*>(blk + v_codes_at(G) + (v * 32 + lane) * 16));
+          uint64_t nan_bits = 0;
+          uint8_t* vt = dst + Z::kKBytes;
+#pragma unroll 1
+          for (int v = part * kVecs; v < (part + 1) * kVecs; ++v) {
+            const uint4 w4 =
+                *reinterpret_cast<const uint4*>(blk + v_codes_at(G) + (v * 32 + lane) * 16);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            const int nt0 = 4 * v / G;
+            const uint2* mv =
+                reinterpret_cast<const uint2*>(blk + v_meta_at(G)) + (4 * nt0 + lo) * G;
+            uint8_t* to = vt + nt0 * 8 * kRow;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const int nt = (4 * v + y) / G, gr = (4 * v + y) % G;
-              meta[x][y] = __ldg(reinterpret_cast<const uint2*>(blk + v_meta_at(G)) +
-                                 (4 * nt + lo) * G + gr);
-            }
-          }
-          ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[st], (uint32_t)((g / S) & 1) ^ 1u,
-                                                 a.status, 0x721, abort_flag));
-          if (!ok) break;
-          uint32_t nan_bits = 0;
-          if (!whole) {
-            // Behind the last key: zero.  Not finite: zero, and the softmax is told.
-#pragma unroll
-            for (int x = 0; x < G; ++x)
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const int nt = (4 * (half * G + x) + y) / G;
-                const int tau = 8 * nt + 2 * lo;
-                uint2& mv = meta[x][y];
+              const int nt = y / G, gr = y % G;
+              uint2 meta = mv[4 * nt * G + gr];
+              if (!whole) {
+                // Behind the last key: zero.  Not finite: zero, and the softmax is told.
+                const int tau = 8 * (nt0 + nt) + 2 * lo;
                 constexpr uint32_t inf = Inf16<T>::kBits;
-                const bool n0 = tau < most && ((mv.x & inf) == inf || (mv.y & inf) == inf);
+                const bool n0 =
+                    tau < most && ((meta.x & inf) == inf || (meta.y & inf) == inf);
                 const bool n1 = tau + 1 < most &&
-                                ((mv.x >> 16 & inf) == inf || (mv.y >> 16 & inf) == inf);
+                                ((meta.x >> 16 & inf) == inf || (meta.y >> 16 & inf) == inf);
                 const uint32_t keep = (n0 || tau >= most ? 0u : 0xffffu) |
                                       (n1 || tau + 1 >= most ? 0u : 0xffff0000u);
-                mv.x &= keep;
-                mv.y &= keep;
-                if (n0) nan_bits |= 1u << (tau & 31);
-                if (n1) nan_bits |= 1u << ((tau + 1) & 31);
+                meta.x &= keep;
+                meta.y &= keep;
+                nan_bits |= (uint64_t)(n0 ? 1 : 0) << tau | (uint64_t)(n1 ? 2 : 0) << tau;
               }
-            // The groups of a key must all go, wherever one is not finite.
-            nan_bits = __reduce_or_sync(0xffffffffu, nan_bits);
-          }
-          if (lane == 0) info[st].nan_v[half] = nan_bits;
-          uint8_t* vt = dst + Z::kKBytes;
-#pragma unroll
-          for (int x = 0; x < G; ++x) {
-            const uint32_t w[4] = {w4[x].x, w4[x].y, w4[x].z, w4[x].w};
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const int nt = (4 * (half * G + x) + y) / G, gr = (4 * (half * G + x) + y) % G;
               uint32_t o[4];
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
-                o[p] = fma2<T>(code_pair<T>(w[y], p), meta[x][y].x, meta[x][y].y);
-              uint8_t* to = vt + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow;
-              *reinterpret_cast<uint2*>(to + (at_v0 ^ 64 * (gr & 1))) =
+              for (int p = 0; p < 4; ++p) o[p] = fma2<T>(code_pair<T>(w[y], p), meta.x, meta.y);
+              uint8_t* row = to + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow;
+              *reinterpret_cast<uint2*>(row + (at_v0 ^ 64 * (gr & 1))) =
                   make_uint2(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410));
-              *reinterpret_cast<uint2*>(to + (at_v1 ^ 64 * (gr & 1))) =
+              *reinterpret_cast<uint2*>(row + (at_v1 ^ 64 * (gr & 1))) =
                   make_uint2(__byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
             }
+          }
+          if (!whole) {
+            const uint32_t n0 = __reduce_or_sync(0xffffffffu, (uint32_t)nan_bits);
+            const uint32_t n1 = __reduce_or_sync(0xffffffffu, (uint32_t)(nan_bits >> 32));
+            nan_bits = (uint64_t)n1 << 32 | n0;
+          }
+          if (lane == 0) {
+            info[st].nan_v[part] = nan_bits;
+            if (kEach == 2) info[st].nan_v[part + 2] = 0;
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[st]);
+        if (lane == 0) {
+          mbar_arrive(&raw_empty[g % R]);
+          mbar_arrive(&kv_full[st]);
+        }
       }
     }
-  } else if (warp == Z::kSoftmaxWarps + kUnpackWarps) {
+    // Let the copies in flight land before the block can end.
+    if (dw == 0)
+      for (int i = max(0, asked - R); i < asked; ++i)
+        mbar_wait(&raw_full[i % R], (uint32_t)((i / R) & 1), a.status, 0x723, nullptr);
+  } else if (warp == Z::kSoftmaxWarps + Z::kUnpackWarps) {
     // ---------------- S issuer ----------------
     if (lane == 0) {
       // fp16 operands, fp32 sums; M 128, N 64
@@ -642,7 +665,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
   }
 
   __syncthreads();
-  if (warp == Z::kSoftmaxWarps + kUnpackWarps) {
+  if (warp == Z::kSoftmaxWarps + Z::kUnpackWarps) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, Z::kTmemCols);
