@@ -16,7 +16,7 @@
 //          V as an MN-major operand.
 // Keys are rounded to fp16 (11 bits, as the queries hold 8 or 11) after a
 // scaling by a power of two, common to a page, that is 1 unless the page's
-// largest magnitude is outside [2^-6, 2^15); the scores are scaled back.  P and
+// magnitudes are all below 2^-3 or come near 2^15; the scores are scaled back.  P and
 // V are rounded to the tensors' type, as 16-bit attention does.  Every wait is
 // a bounded mbarrier wait; one that runs out records its site in the status
 // word and the roles unwind.
@@ -72,12 +72,12 @@ CTI_DEVICE int swizzle_of(int r) {
 }
 
 // Matrix descriptor of an operand tile, 8-row atoms stacked along its rows: K-major
-// for Q and K, MN-major (each row a key) for V.  The tile is one atom wide, so
-// both offset fields hold an atom's bytes.
+// for Q and K, MN-major (each row a key) for V.  The stride field holds an
+// atom's bytes; the leading one the bytes between the panels of a wide V.
 template <int ROW>
-CTI_DEVICE uint64_t tile_desc(uint32_t saddr) {
+CTI_DEVICE uint64_t tile_desc(uint32_t saddr, uint32_t panel = 8 * ROW) {
   constexpr uint64_t atom = 8 * ROW;
-  return (uint64_t)((saddr >> 4) & 0x3fffu) | (atom >> 4) << 16 | (atom >> 4) << 32 |
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)(panel >> 4) << 16 | (atom >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)(ROW == 128 ? 2 : 4) << 61;
 }
 
@@ -87,6 +87,18 @@ CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* 
           "r"(smem_u32(dst)),
       "l"(src), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
+}
+
+// The larger of both halves of two numbers of T that are not negative; a NaN
+// counts nothing.
+template <typename T>
+CTI_DEVICE uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (Type16<T>::kShift == 3)
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else
+    asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
 CTI_DEVICE float max3f(float a, float b, float c) {
@@ -469,39 +481,47 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
                                       0x721, abort_flag));
         if (!ok) break;
         if (keys) {
-          // The page's scaling: every key warp finds the same.
+          // The page's scaling, from a bound of its magnitudes, 31 max s + max
+          // |b| (at most 8 times the largest): every key warp finds the same.
           const uint32_t* km = reinterpret_cast<const uint32_t*>(blk + k_meta_at(G));
-          float most_k = 0.0f;
+          uint32_t top_sb = 0;  // max s in the low half, max |b| in the high one
 #pragma unroll
           for (int x = 0; x < 2 * G; ++x) {
-            const uint32_t w = km[32 * x + lane];
-            const float sx = Y::low(w), bx = Y::high(w);
-            const float z = fmaxf(fabsf(fmaf(16.0f, sx, bx)), fabsf(fmaf(31.0f, sx, bx)));
-            if (z <= FLT_MAX && (32 * x + lane) / G < most) most_k = fmaxf(most_k, z);
+            uint32_t w = km[32 * x + lane] & 0x7fff7fffu;
+            if (!whole && (32 * x + lane) / G >= most) w = 0;
+            top_sb = max2<T>(top_sb, w);
           }
+          const float most_k = fminf(fmaf(31.0f, Y::low(top_sb), Y::high(top_sb)), FLT_MAX);
           const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most_k));
           int e = 0;
-          if (top != 0 && (top < 0x3c800000u || top >= 0x47000000u))  // [2^-6, 2^15)
+          if (top != 0 && (top < 0x3e000000u || top >= 0x47000000u))  // [2^-3, 2^15)
             e = max(-100, min((int)(top >> 23) - 127, 100));
           const float down = __uint_as_float((uint32_t)(127 - e) << 23);
           if (part == 0 && lane == 0) {
             info[st].scale = __uint_as_float((uint32_t)(127 + e) << 23);
             info[st].keys = is_page ? kPage : 0;
           }
-#pragma unroll 1
-          for (int v = part * kVecs; v < (part + 1) * kVecs; ++v) {
+#pragma unroll
+          for (int x = 0; x < kVecs; ++x) {
+            const int v = part * kVecs + x, nt0 = 4 * v / G;
             const uint4 w4 = *reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16);
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-            const int nt0 = 4 * v / G;
             const uint32_t* mv = km + (8 * nt0 + hi) * G;
+            uint32_t meta[4];
+            if constexpr (G == 4) {
+              const uint4 m4 = *reinterpret_cast<const uint4*>(mv);
+              meta[0] = m4.x, meta[1] = m4.y, meta[2] = m4.z, meta[3] = m4.w;
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; ++y) meta[y] = mv[8 * (y / G) * G + y % G];
+            }
             uint8_t* to = dst + nt0 * 8 * kRow;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const int nt = y / G, gr = y % G;  // nt: octets past nt0
-              const uint32_t meta = mv[8 * nt * G + gr];
-              const float sx = Y::low(meta) * down, bx = Y::high(meta) * down;
-              uint32_t s2 = Type16<__half>::pack(sx, sx), b2 = Type16<__half>::pack(bx, bx);
-              if (8 * (nt0 + nt) + hi >= most) s2 = b2 = 0;
+              const uint32_t sb =
+                  Type16<__half>::pack(Y::low(meta[y]) * down, Y::high(meta[y]) * down);
+              const uint32_t s2 = __byte_perm(sb, sb, 0x1010), b2 = __byte_perm(sb, sb, 0x3232);
               uint32_t o[4];
 #pragma unroll
               for (int p = 0; p < 4; ++p)
@@ -514,19 +534,32 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         } else {
           uint64_t nan_bits = 0;
           uint8_t* vt = dst + Z::kKBytes;
-#pragma unroll 1
-          for (int v = part * kVecs; v < (part + 1) * kVecs; ++v) {
+#pragma unroll
+          for (int x = 0; x < kVecs; ++x) {
+            const int v = part * kVecs + x, nt0 = 4 * v / G;
             const uint4 w4 =
                 *reinterpret_cast<const uint4*>(blk + v_codes_at(G) + (v * 32 + lane) * 16);
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-            const int nt0 = 4 * v / G;
             const uint2* mv =
                 reinterpret_cast<const uint2*>(blk + v_meta_at(G)) + (4 * nt0 + lo) * G;
+            uint2 metas[4];
+            if constexpr (G == 1) {
+#pragma unroll
+              for (int y = 0; y < 4; ++y) metas[y] = mv[4 * y];
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; y += 2) {
+                const uint4 m4 =
+                    *reinterpret_cast<const uint4*>(mv + 4 * (y / G) * G + y % G);
+                metas[y] = make_uint2(m4.x, m4.y);
+                metas[y + 1] = make_uint2(m4.z, m4.w);
+              }
+            }
             uint8_t* to = vt + nt0 * 8 * kRow;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const int nt = y / G, gr = y % G;
-              uint2 meta = mv[4 * nt * G + gr];
+              uint2 meta = metas[y];
               if (!whole) {
                 // Behind the last key: zero.  Not finite: zero, and the softmax is told.
                 const int tau = 8 * (nt0 + nt) + 2 * lo;
@@ -621,9 +654,8 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
     // ---------------- PV issuer ----------------
     if (lane == 0) {
       constexpr uint32_t type = sizeof(T) == 2 && Type16<T>::kShift == 3 ? 1u : 0u;  // bf16, fp16
-      constexpr int kN = D < 64 ? D : 64;  // head dims of one instruction: a panel's
       constexpr uint32_t id_pv = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) |
-                                 ((kN >> 3) << 17) | ((kTile >> 4) << 24);  // V MN-major
+                                 ((D >> 3) << 17) | ((kTile >> 4) << 24);  // V MN-major
       const uint32_t kv_addr = smem_u32(sKV);
       int it = 0, g = 0;
       bool ok = true, any = false;
@@ -643,11 +675,10 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             const uint32_t va = kv_addr + st * 2 * Z::kKBytes + Z::kKBytes;
 #pragma unroll
             for (int kk = 0; kk < kPage / 16; ++kk)
-#pragma unroll
-              for (int panel = 0; panel < Z::kPanels; ++panel)
-                umma_bf16_ts(ocol + 64u * panel, pbuf + kk * 8,
-                             tile_desc<kRow>(va + panel * Z::kKVPanel + kk * 16 * kRow), id_pv,
-                             j == 0 && kk == 0 ? 0u : 1u);
+              umma_bf16_ts(ocol, pbuf + kk * 8,
+                           tile_desc<kRow>(va + kk * 16 * kRow,
+                                           Z::kPanels == 2 ? Z::kKVPanel : 8 * kRow),
+                           id_pv, j == 0 && kk == 0 ? 0u : 1u);
             umma_commit(&pv_done[2 * i + b]);
             umma_commit(&kv_empty[st]);
             any = true;
