@@ -37,11 +37,8 @@ class KV4Cache:
         self.dtype = dtype
         self.pages = torch.zeros((int(num_pages), self.kv_heads, page_bytes // self.kv_heads),
                                  dtype=torch.uint8, device=device)
+        self.device = self.pages.device
 
     @property
     def num_pages(self) -> int:
         return self.pages.shape[0]
-
-    @property
-    def device(self) -> torch.device:
-        return self.pages.device

@@ -7,8 +7,8 @@ tensors.  They are the building blocks of :class:`SMoE` and
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -358,53 +358,64 @@ def ctr_head(h: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tens
     return logits, probs
 
 
-def _on(dev: torch.device):
-    """Makes ``dev`` the current device for a launch (no switch where it is)."""
-    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _kv4_run(cache: KV4Cache, fn, what: str, *args) -> None:
+    """Calls a kv4 entry point on the cache's device and its current stream."""
+    index = cache.device.index
+    args += (status_word(cache.device).data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc:
+        check(rc, what)
 
 
-def _kv4_rows(t: torch.Tensor, name: str, cache: KV4Cache, heads: int) -> None:
-    """A [tokens, heads, head_dim] view with contiguous heads in the cache's type."""
+def _kv4_rows(t: torch.Tensor, name: str, cache: KV4Cache, heads: int) -> tuple[int, int]:
+    """(tokens, token stride) of a [tokens, heads, head_dim] view with contiguous heads in the
+    cache's type."""
+    hd = cache.head_dim
     if not t.is_cuda or t.dtype != cache.dtype:
         raise TypeError(f"{name} must be a {cache.dtype} CUDA tensor")
-    if t.device != cache.device:
+    if t.get_device() != cache.device.index:
         raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    hd = cache.head_dim
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd:
+    if t.dim() != 3 or t.size(1) != heads or t.size(2) != hd:
         raise ValueError(f"{name} must be [tokens, {heads}, {hd}], got {tuple(t.shape)}")
-    if t.shape[0] and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd)):
+    n = t.size(0)
+    if n and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd)):
         raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous heads")
-
-
-def _kv4_stride(t: torch.Tensor, row: int) -> int:
-    """Token stride as the C entry points take it (a single token has any)."""
-    return t.stride(0) if t.shape[0] > 1 else row
+    return n, t.stride(0) if n > 1 else heads * hd  # a single token has any stride
 
 
 def _kv4_index(cache: KV4Cache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
-               page_table: torch.Tensor) -> int:
-    """Checks the index tensors; returns the number of sequences."""
-    dev = cache.device
-    for name, t in (("cu_seqlens", cu_seqlens), ("kv_lens", kv_lens)):
-        require_cuda(t, name, torch.int32)
-        if t.dim() != 1:
-            raise ValueError(f"{name} must have one dimension")
-    if not page_table.is_cuda or page_table.dtype != torch.int32:
-        raise TypeError("page_table must be an int32 CUDA tensor")
-    n = kv_lens.shape[0]
-    if cu_seqlens.shape[0] != n + 1:
-        raise ValueError(f"cu_seqlens must have {n + 1} entries for {n} sequences")
-    if page_table.dim() != 2 or page_table.shape[0] != n:
+               page_table: torch.Tensor) -> tuple:
+    """Checks the index tensors; the arguments that every kv4 entry point takes of them, up to the
+    number of sequences."""
+    index = cache.device.index
+    for name, t in (("cu_seqlens", cu_seqlens), ("kv_lens", kv_lens), ("page_table", page_table)):
+        if t.dtype is not torch.int32 or not t.is_cuda:
+            require_cuda(t, name)
+            raise TypeError(f"{name} must be torch.int32, got {t.dtype}")
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    n = kv_lens.size(0) if kv_lens.dim() == 1 else -1
+    if n < 0 or cu_seqlens.dim() != 1 or cu_seqlens.size(0) != n + 1:
+        raise ValueError("kv_lens must be [N] and cu_seqlens [N + 1], got "
+                         f"{tuple(kv_lens.shape)} and {tuple(cu_seqlens.shape)}")
+    if not kv_lens.is_contiguous() or not cu_seqlens.is_contiguous():
+        raise ValueError("kv_lens and cu_seqlens must be contiguous")
+    if page_table.dim() != 2 or page_table.size(0) != n:
         raise ValueError(f"page_table must be [{n}, pages], got {tuple(page_table.shape)}")
-    if page_table.numel() and page_table.shape[1] > 1 and page_table.stride(1) != 1:
+    cols = page_table.size(1)
+    if n and cols > 1 and page_table.stride(1) != 1:
         raise ValueError("page_table rows must be contiguous")
-    if cu_seqlens.device != dev or kv_lens.device != dev or page_table.device != dev:
-        raise ValueError(f"cu_seqlens, kv_lens and page_table must be on {dev}")
-    return n
+    return (cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
+            page_table.stride(0) if n > 1 else cols, cols, n)
 
 
-def _table_stride(page_table: torch.Tensor) -> int:
-    return page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+@lru_cache(maxsize=256)
+def _kv4_workspace_bytes(*sizes: int) -> int:
+    return lib.cti_kv4_attention_workspace_bytes(*sizes)
 
 
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -415,20 +426,16 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, cu_seqlens: to
     are the sequences' lengths with these tokens, which are their last;
     page_table int32 [N, pages].  A position past the table or a page outside
     the cache is skipped and reported in the device status word."""
-    n = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
-    H, hd, dev = cache.kv_heads, cache.head_dim, cache.device
-    _kv4_rows(k, "k", cache, H)
-    _kv4_rows(v, "v", cache, H)
-    if v.shape[0] != k.shape[0]:
+    seqs = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
+    H = cache.kv_heads
+    tokens, k_stride = _kv4_rows(k, "k", cache, H)
+    v_tokens, v_stride = _kv4_rows(v, "v", cache, H)
+    if v_tokens != tokens:
         raise ValueError("k and v must have the same number of tokens")
-    with _on(dev):
-        rc = lib.cti_kv4_append(
-            k.data_ptr(), v.data_ptr(), _kv4_stride(k, H * hd), _kv4_stride(v, H * hd),
-            _lib.DTYPE_CODES[cache.dtype], cu_seqlens.data_ptr(), kv_lens.data_ptr(),
-            page_table.data_ptr(), _table_stride(page_table), page_table.shape[1], n, k.shape[0],
-            H, hd, cache.pages.data_ptr(), cache.num_pages, status_word(dev).data_ptr(),
-            stream_handle(dev))
-    check(rc, "cti_kv4_append")
+    pages = cache.pages
+    _kv4_run(cache, lib.cti_kv4_append, "cti_kv4_append", k.data_ptr(), v.data_ptr(), k_stride,
+             v_stride, _lib.DTYPE_CODES[cache.dtype], *seqs, tokens, H, cache.head_dim,
+             pages.data_ptr(), pages.size(0))
 
 
 def kv4_read(cache: KV4Cache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
@@ -439,28 +446,25 @@ def kv4_read(cache: KV4Cache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
     head_dim] in the cache's dtype.  ``tokens`` is cu_seqlens[-1]; with
     cu_seqlens the offsets of kv_lens, whole sequences are read.  ``out``: the
     two tensors to write (rows of no sequence keep their contents)."""
-    n = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
-    H, hd, dev = cache.kv_heads, cache.head_dim, cache.device
+    seqs = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
+    H, hd = cache.kv_heads, cache.head_dim
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
     if out is None:
-        k = torch.empty((tokens, H, hd), dtype=cache.dtype, device=dev)
+        k = torch.empty((tokens, H, hd), dtype=cache.dtype, device=cache.device)
         v = torch.empty_like(k)
+        k_stride = v_stride = H * hd
     else:
         k, v = out
-        for name, t in (("out[0]", k), ("out[1]", v)):
-            _kv4_rows(t, name, cache, H)
-            if t.shape[0] != tokens:
-                raise ValueError(f"{name} must hold {tokens} tokens")
-    with _on(dev):
-        rc = lib.cti_kv4_read(
-            cache.pages.data_ptr(), cache.num_pages, _lib.DTYPE_CODES[cache.dtype],
-            cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
-            _table_stride(page_table), page_table.shape[1], n, tokens, H, hd, k.data_ptr(),
-            v.data_ptr(), _kv4_stride(k, H * hd), _kv4_stride(v, H * hd),
-            status_word(dev).data_ptr(), stream_handle(dev))
-    check(rc, "cti_kv4_read")
+        k_tokens, k_stride = _kv4_rows(k, "out[0]", cache, H)
+        v_tokens, v_stride = _kv4_rows(v, "out[1]", cache, H)
+        if k_tokens != tokens or v_tokens != tokens:
+            raise ValueError(f"out must hold {tokens} tokens")
+    pages = cache.pages
+    _kv4_run(cache, lib.cti_kv4_read, "cti_kv4_read", pages.data_ptr(), pages.size(0),
+             _lib.DTYPE_CODES[cache.dtype], *seqs, tokens, H, hd, k.data_ptr(), v.data_ptr(),
+             k_stride, v_stride)
     return k, v
 
 
@@ -478,14 +482,14 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
     (defaults: from the token count and the table's width); the work is split
     by them, results hold for any.  Returns a contiguous [tokens, heads,
     head_dim]; a token that sees no key is zero."""
-    n = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
-    hd, dev = cache.head_dim, cache.device
-    if q.dim() != 3 or q.shape[1] <= 0 or q.shape[1] % cache.kv_heads:
-        raise ValueError(f"q must be [tokens, heads, head_dim] with heads a multiple of "
-                         f"{cache.kv_heads}, got {tuple(q.shape)}")
-    T, H, _ = q.shape
-    _kv4_rows(q, "q", cache, H)
-    cols = page_table.shape[1]
+    seqs = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
+    hd, Hkv = cache.head_dim, cache.kv_heads
+    H = q.size(1) if q.dim() == 3 else 0
+    if H <= 0 or H % Hkv:
+        raise ValueError(f"q must be [tokens, heads, head_dim] with heads a multiple of {Hkv}, "
+                         f"got {tuple(q.shape)}")
+    T, q_stride = _kv4_rows(q, "q", cache, H)
+    cols, n = seqs[4:]
     if max_new is None:
         max_new = 1 if T <= n else T
     if max_kv_len is None:
@@ -493,21 +497,17 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
     if scale is None:
         scale = hd ** -0.5
     if out is None:
-        out = torch.empty((T, H, hd), dtype=cache.dtype, device=dev)
+        out = torch.empty((T, H, hd), dtype=cache.dtype, device=cache.device)
     else:
         _kv4_rows(out, "out", cache, H)
-        if out.shape[0] != T or not out.is_contiguous():
+        if out.size(0) != T or not out.is_contiguous():
             raise ValueError("out must be contiguous, of q's shape")
-    with _on(dev):
-        need = lib.cti_kv4_attention_workspace_bytes(n, T, int(max_new), int(max_kv_len), H,
-                                                     cache.kv_heads, hd)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        rc = lib.cti_kv4_attention(
-            q.data_ptr(), _kv4_stride(q, H * hd), _lib.DTYPE_CODES[cache.dtype],
-            cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
-            _table_stride(page_table), cols, n, T, int(max_new), int(max_kv_len), H,
-            cache.kv_heads, hd, float(scale), int(bool(causal)), cache.pages.data_ptr(),
-            cache.num_pages, out.data_ptr(), ptr(ws), need, status_word(dev).data_ptr(),
-            stream_handle(dev))
-    check(rc, "cti_kv4_attention")
+    max_new, max_kv_len = int(max_new), int(max_kv_len)
+    need = _kv4_workspace_bytes(n, T, max_new, max_kv_len, H, Hkv, hd)
+    ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    pages = cache.pages
+    _kv4_run(cache, lib.cti_kv4_attention, "cti_kv4_attention", q.data_ptr(), q_stride,
+             _lib.DTYPE_CODES[cache.dtype], *seqs, T, max_new, max_kv_len, H, Hkv, hd,
+             float(scale), 1 if causal else 0, pages.data_ptr(), pages.size(0), out.data_ptr(),
+             ptr(ws), need)
     return out
