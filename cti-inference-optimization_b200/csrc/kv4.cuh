@@ -17,7 +17,7 @@
 //
 // A page holds 64 tokens of every KV head; one head's part of it is one
 // contiguous block of 2560 G bytes, G = head_dim / 32 groups:
-//   K codes 1024 G | V codes 1024 G | K meta 256 G | V meta 256 G
+//   K codes 1024 G | K meta 256 G | V codes 1024 G | V meta 256 G
 // with the codes in the order in which the attention kernels' matrix
 // operands want them.  Token tau = 8 nt + r of the page, group g:
 //   K codes  the 32-bit word of dims 32 g + 8 t .. + 7 (t = 0..3) belongs to
@@ -42,8 +42,9 @@ constexpr int kGroup = 32;  // values that share a scale and a base
 
 // Bytes of one head's part of a page, and where its sections start.
 __host__ __device__ constexpr int block_bytes(int G) { return 2560 * G; }
-__host__ __device__ constexpr int v_codes_at(int G) { return 1024 * G; }
-__host__ __device__ constexpr int k_meta_at(int G) { return 2048 * G; }
+__host__ __device__ constexpr int part_bytes(int G) { return 1280 * G; }  // of keys, or values
+__host__ __device__ constexpr int k_meta_at(int G) { return 1024 * G; }
+__host__ __device__ constexpr int v_codes_at(int G) { return 1280 * G; }
 __host__ __device__ constexpr int v_meta_at(int G) { return 2304 * G; }
 
 // Byte of lane `lane`'s code word i inside a codes section.

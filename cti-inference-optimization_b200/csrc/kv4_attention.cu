@@ -44,15 +44,16 @@ using namespace kv4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Warps of a block, pages in flight for each, and blocks of an SM: what
-// shared memory and registers allow.
-__host__ __device__ constexpr int warps(int G, int NT) { return G == 4 && NT == 1 ? 5 : 4; }
-__host__ __device__ constexpr int stages(int G) { return G == 1 ? 3 : 2; }
+// Warps of a block, and blocks of an SM: what registers allow.  Page parts (a
+// page's keys, or its values) in a warp's ring.
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+__host__ __device__ constexpr int slots(int G) { return G == 4 ? 2 : 4; }
 __host__ __device__ constexpr int blocks_per_sm(int G, int NT) {
-  return G == 4 || NT == 4 ? 2 : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 5 : 4;
+  return NT == 4 ? 2 : G == 4 ? (NT == 1 ? 4 : 2) : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 5 : 4;
 }
-__host__ __device__ constexpr size_t smem_bytes(int G, int NT) {
-  return (size_t)warps(G, NT) * stages(G) * (block_bytes(G) + 8);
+__host__ __device__ constexpr size_t smem_bytes(int G) {
+  return (size_t)kWarps * slots(G) * (part_bytes(G) + 8);
 }
 
 template <typename T>
@@ -107,21 +108,21 @@ CTI_DEVICE uint32_t k_codes(uint32_t w, int j) {
 }
 
 template <typename T, int G, int NT>
-__global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     kv4_attention_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pages, const Args a,
                          T* __restrict__ out) {
   using Y = Type16<T>;
   using M = Mma<T>;
   constexpr int D = 32 * G;
   constexpr int ROWS = 8 * NT;
-  constexpr int S = stages(G);
-  constexpr int W = warps(G, NT);
-  constexpr int kBlock = block_bytes(G);
+  constexpr int S = slots(G);
+  constexpr int W = kWarps;
+  constexpr int kPart = part_bytes(G);
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = warp_id(), lane = lane_id();
   const int r8 = lane >> 2, t4 = lane & 3;
-  uint8_t* ring = smem + (size_t)warp * S * kBlock;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)W * S * kBlock) + warp * S;
+  uint8_t* ring = smem + (size_t)warp * S * kPart;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)W * S * kPart) + warp * S;
   if (lane == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
@@ -149,9 +150,9 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
     limit = a.num_pages <= 0 ? 0 : a.table_cols * kPage;
   }
   const int32_t* table = a.table + s * a.table_stride;
-  const uint8_t* base = pages + (int64_t)kvh * kBlock;
-  const int64_t page_stride = (int64_t)a.kv_heads * kBlock;
-  uint32_t count = 0;  // pages copied so far: stage and parity
+  const uint8_t* base = pages + (int64_t)kvh * block_bytes(G);
+  const int64_t page_stride = (int64_t)a.kv_heads * block_bytes(G);
+  uint32_t count = 0;  // page parts copied so far: slot and parity
   bool dead = false;   // a copy did not arrive in time
 
   for (int tile = blockIdx.y; tile < (rows + ROWS - 1) / ROWS; tile += gridDim.y) {
@@ -173,26 +174,31 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
       np = min(np - skip, per);
     }
     if (dead) np = 0;
-    int ids = -1;  // lane i: page p0 + (chunk of 32) + i
-    uint32_t bad = 0;  // bit per stage: not a page, nothing of it is seen
-    auto issue = [&](int i) {  // page i of the range into its stage
-      if ((i & 31) == 0) {
+    int ids = -1;      // lane i: page p0 + (chunk of 32) + i
+    uint32_t bad[2] = {0, 0};  // by chunk: bit per page that is none; nothing of it is seen
+    auto issue = [&](int h) {  // keys (h = 2 i) or values (2 i + 1) of page i of the range
+      const int i = h >> 1;
+      if ((h & 63) == 0) {
         ids = i + lane < np ? __ldg(table + p0 + i + lane) : 0;
         if (ids < 0 || ids >= a.num_pages) {
           raise_status(a.status, CTI_ERR_BOUNDS, s);
           ids = -1;
         }
+        bad[(h >> 6) & 1] = __ballot_sync(0xffffffffu, ids < 0);
       }
-      int id = __shfl_sync(0xffffffffu, ids, i & 31);
-      const uint32_t st = (count + i) % S;
-      bad = id < 0 ? bad | 1u << st : bad & ~(1u << st);
-      if (id < 0) id = 0;
+      const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+      const uint32_t slot = (count + h) % S;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&full[st], kBlock);
-        bulk_load(ring + st * kBlock, base + id * page_stride, kBlock, &full[st]);
+        mbar_arrive_expect_tx(&full[slot], kPart);
+        bulk_load(ring + slot * kPart, base + max(id, 0) * page_stride + (h & 1) * kPart, kPart,
+                  &full[slot]);
       }
     };
-    for (int i = 0; i < S && i < np; ++i) issue(i);
+    auto arrived = [&](int h) {
+      return __all_sync(0xffffffffu, mbar_wait(&full[(count + h) % S], ((count + h) / S) & 1,
+                                               a.status, 0x700 + (h & 1), nullptr));
+    };
+    for (int h = 0; h < S && h < 2 * np; ++h) issue(h);
 
     // ---- queries: lane 4 r + t has dims 8 t .. + 7 of every group of row r ----
     uint32_t qb[NT][G][4];
@@ -273,20 +279,22 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
 
     int done = 0;
     for (; done < np; ++done) {
-      const uint32_t st = (count + done) % S;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[st], ((count + done) / S) & 1, a.status, 0x700,
-                                             nullptr)))
-        break;
-      uint8_t* blk = ring + st * kBlock;
+      if (!arrived(2 * done)) break;
+      const uint8_t* blk = ring + (count + 2 * done) % S * kPart;
+      uint8_t* vblk = ring + (count + 2 * done + 1) % S * kPart;
 
       // ---- S^T = K Q^T, 16 keys at a time ----
       float sc[NT][4][4];
-      uint4 kw[2 * G];
-#pragma unroll
-      for (int v = 0; v < 2 * G; ++v)
-        kw[v] = *reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16);
+      uint4 kw[2];  // of 16 tokens (G = 4), 32 (2) or 64 (1)
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
+        constexpr int kTiles = 4 / G;  // of 16 tokens, that the two vectors hold
+        if (mt % kTiles == 0) {
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+            kw[v] = *reinterpret_cast<const uint4*>(
+                blk + ((2 * (mt / kTiles) + v) * 32 + lane) * 16);
+        }
         uint32_t meta[2][G];  // of tokens 16 mt + r and + 8
         uint32_t am[2];       // its word for the offsets: group t's
 #pragma unroll
@@ -314,7 +322,8 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const uint32_t w0 = word_of(kw, 2 * mt * G + g), w1 = word_of(kw, (2 * mt + 1) * G + g);
+          const uint32_t w0 = word_of(kw, 2 * (mt % kTiles) * G + g);
+          const uint32_t w1 = word_of(kw, (2 * (mt % kTiles) + 1) * G + g);
           const uint32_t a0[4] = {k_codes(w0, 0), k_codes(w1, 0), k_codes(w0, 1), k_codes(w1, 1)};
           const uint32_t a1[4] = {k_codes(w0, 2), k_codes(w1, 2), k_codes(w0, 3), k_codes(w1, 3)};
           const float s0 = Y::low(meta[0][g]), s1 = Y::low(meta[1][g]);
@@ -331,15 +340,20 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
         }
       }
 
+      __syncwarp();
+      if (2 * done + S < 2 * np) issue(2 * done + S);
+      if (!arrived(2 * done + 1)) break;
+
       const int key0 = (p0 + done) * kPage;
-      const bool is_bad = (bad >> st) & 1;
+      const bool is_bad = bad[(done >> 5) & 1] >> (done & 31) & 1;
       if (is_bad || key0 + kPage > all) {
         // Keys that a row does not see count nothing, whatever they hold: a
         // value behind the last key gets a meta of zero.  One that is not
         // finite and that only some rows see gets the same, and a score of NaN
         // for those that do.
         const int lim_most = is_bad ? 0 : most - key0;
-        uint32_t* vm = reinterpret_cast<uint32_t*>(blk + v_meta_at(G)) + lane * 2 * G;
+        uint32_t* vm =
+            reinterpret_cast<uint32_t*>(vblk + v_meta_at(G) - v_codes_at(G)) + lane * 2 * G;
         bool nan0 = false, nan1 = false;  // of tokens 2 lane and 2 lane + 1
         if (all < most) {
 #pragma unroll
@@ -423,12 +437,16 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) noff[n][e] = m[n][e] == -INFINITY ? 0.0f : -m[n][e] * sl[n][e];
-      uint4 vw[2 * G];
-#pragma unroll
-      for (int v = 0; v < 2 * G; ++v)
-        vw[v] = *reinterpret_cast<const uint4*>(blk + v_codes_at(G) + (v * 32 + lane) * 16);
+      uint4 vw[2];
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
+        constexpr int kTiles = 4 / G;
+        if (kk % kTiles == 0) {
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+            vw[v] = *reinterpret_cast<const uint4*>(
+                vblk + ((2 * (kk / kTiles) + v) * 32 + lane) * 16);
+        }
         uint32_t pb[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -444,7 +462,8 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint2* mw =
-              reinterpret_cast<const uint2*>(blk + v_meta_at(G)) + (8 * kk + 4 * e + t4) * G;
+              reinterpret_cast<const uint2*>(vblk + v_meta_at(G) - v_codes_at(G)) +
+              (8 * kk + 4 * e + t4) * G;
           if constexpr (G == 1) {
             meta[e][0] = *mw;
           } else {
@@ -458,7 +477,8 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const uint32_t w0 = word_of(vw, 2 * kk * G + g), w1 = word_of(vw, (2 * kk + 1) * G + g);
+          const uint32_t w0 = word_of(vw, 2 * (kk % kTiles) * G + g);
+          const uint32_t w1 = word_of(vw, (2 * (kk % kTiles) + 1) * G + g);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t av[4] = {
@@ -472,14 +492,13 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
         }
       }
       __syncwarp();
-      if (done + S < np) issue(done + S);
+      if (2 * done + 1 + S < 2 * np) issue(2 * done + 1 + S);
     }
     if (done < np) {  // let the copies in flight land, then give up
       dead = true;
-      for (int i = done; i < np && i < done + S; ++i)
-        mbar_wait(&full[(count + i) % S], ((count + i) / S) & 1, a.status, 0x701, nullptr);
+      for (int h = 2 * done; h < 2 * np && h <= 2 * done + S; ++h) arrived(h);
     }
-    count += np;
+    count += 2 * np;
 
     // ---- join and store: lane 4 r + t has dims 4 r .. + 3 of every group ----
 #pragma unroll
@@ -493,7 +512,7 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
     if (shared) {
       // Every warp's rows in its own ring, then the first warp adds them up.
       float* mine = reinterpret_cast<float*>(ring);
-      static_assert((ROWS * D + 2 * ROWS) * 4 <= S * kBlock, "room for the rows");
+      static_assert((ROWS * D + 2 * ROWS) * 4 <= S * kPart, "room for the rows");
       __syncwarp();
       if (warp != 0) {
 #pragma unroll
@@ -514,7 +533,7 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
       __syncthreads();
       if (warp == 0) {
         for (int w = 1; w < W; ++w) {
-          const float* src = reinterpret_cast<const float*>(ring + (size_t)w * S * kBlock);
+          const float* src = reinterpret_cast<const float*>(ring + (size_t)w * S * kPart);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -580,40 +599,62 @@ __global__ void __launch_bounds__(warps(G, NT) * 32, blocks_per_sm(G, NT))
   }
 }
 
-// Joins the splits of every row: one warp per row.
+// Joins the splits of every row: a block per row, whose warps share the splits.
+// Bound by latency (the rows of a call with splits are few): every warp finds
+// all weights, 32 splits at a time, then sums its own splits with independent
+// loads.
+constexpr int kJoinWarps = 4;
 template <typename T, int G>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kJoinWarps * 32)
     kv4_join_kernel(const Args a, int splits, T* __restrict__ out) {
   using Y = Type16<T>;
   constexpr int D = 32 * G;
+  __shared__ float part[kJoinWarps][D];
   grid_dependency_wait();
-  const int64_t rows = (int64_t)a.tokens * a.heads;
-  const int64_t row = (int64_t)blockIdx.x * 4 + warp_id();
-  const int lane = lane_id();
-  if (row >= rows) return;
-  const int64_t t = row / a.heads;
+  const int64_t rows = (int64_t)a.tokens * a.heads, row = blockIdx.x;
+  const int lane = lane_id(), warp = warp_id();
+  const int t = blockIdx.x / (unsigned)a.heads;
   if (t < __ldg(a.cu) || t >= __ldg(a.cu + a.num_seqs)) return;
+  float2 ml[4];  // of splits 32 i + lane
   float mm = -INFINITY;
-  for (int z = lane; z < splits; z += 32) mm = fmaxf(mm, a.ws_ml[z * rows + row].x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ml[i] = make_float2(-INFINITY, 0.0f);
+    if (32 * i + lane < splits) ml[i] = a.ws_ml[(32 * i + lane) * rows + row];
+    mm = fmaxf(mm, ml[i].x);
+  }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
   float l = 0.0f, o[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) o[g] = 0.0f;
-#pragma unroll 4
-  for (int z = 0; z < splits; ++z) {
-    const float2 ml = a.ws_ml[z * rows + row];
-    if (ml.y == 0.0f) continue;  // no key of the split is seen
-    const float w = ml.x == mm ? 1.0f : ex2_approx(ml.x - mm);
-    l = fmaf(ml.y, w, l);
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-      o[g] = fmaf(a.ws_o[(z * rows + row) * D + 32 * g + lane], w, o[g]);
+  for (int i = 0; i < 4; ++i) {
+    if (32 * i >= splits) break;
+    // No key of the split is seen where l is 0: its rows were not written.
+    const float w = ml[i].y == 0.0f ? 0.0f : ml[i].x == mm ? 1.0f : ex2_approx(ml[i].x - mm);
+    l += ml[i].y * w;
+#pragma unroll 8
+    for (int z = warp; z < min(32, splits - 32 * i); z += kJoinWarps) {
+      const float wz = __shfl_sync(0xffffffffu, w, z);
+      if (wz == 0.0f) continue;
+      const float* src = a.ws_o + ((32 * i + z) * rows + row) * D + lane;
+#pragma unroll
+      for (int g = 0; g < G; ++g) o[g] = fmaf(src[32 * g], wz, o[g]);
+    }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-    reinterpret_cast<uint16_t*>(out)[row * D + 32 * g + lane] = (uint16_t)Y::bits(o[g] * inv);
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+  for (int g = 0; g < G; ++g) part[warp][32 * g + lane] = o[g];
+  __syncthreads();
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+    float sum = part[0][d];
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) sum += part[w][d];
+    reinterpret_cast<uint16_t*>(out)[row * D + d] = (uint16_t)Y::bits(sum * inv);
+  }
 }
 
 // Query rows of a KV head, by the caller's bound, from which a sequence's rows
@@ -651,7 +692,7 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   p.row_tiles = rows <= 8 ? 1 : rows <= 16 || G == 4 ? 2 : 4;
   p.tiles = (rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
   const double units = (double)num_seqs * kv_heads * (double)p.tiles;
-  const double room = (double)kSMs * blocks_per_sm(G, p.row_tiles) * warps(G, p.row_tiles);  // warps at once
+  const double room = (double)kSMs * blocks_per_sm(G, p.row_tiles) * kWarps;  // warps at once
   p.splits = 1;
   p.chunk = 0;
   if (units >= room && pages <= 8) {
@@ -665,7 +706,7 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   p.shared = true;
   const double ideal = units * pages / room;
   int64_t per_warp = ideal > 16 ? 12 : (int64_t)ideal + 1;
-  p.chunk = (int)(per_warp * warps(G, p.row_tiles));
+  p.chunk = (int)(per_warp * kWarps);
   int64_t splits = (pages + p.chunk - 1) / p.chunk;
   if (splits > 128) {
     splits = 128;
@@ -685,14 +726,14 @@ template <typename T, int G, int NT>
 int launch(const void* q, const void* pages, const Args& a, const Plan& p, void* out,
            cudaStream_t s) {
   static uint64_t configured = 0;
-  if (ensure_smem_limit(kv4_attention_kernel<T, G, NT>, (int)smem_bytes(G, NT), configured) !=
+  if (ensure_smem_limit(kv4_attention_kernel<T, G, NT>, (int)smem_bytes(G), configured) !=
       cudaSuccess)
     return CTI_ERR_CUDA;
   const int64_t units = (int64_t)a.num_seqs * a.kv_heads;
-  const int per = p.shared ? 1 : warps(G, NT);
+  const int per = p.shared ? 1 : kWarps;
   const dim3 grid((unsigned)((units + per - 1) / per),
                   (unsigned)(p.tiles < 65535 ? p.tiles : 65535), (unsigned)p.splits);
-  if (launch_dependent(kv4_attention_kernel<T, G, NT>, grid, dim3(warps(G, NT) * 32), smem_bytes(G, NT), s,
+  if (launch_dependent(kv4_attention_kernel<T, G, NT>, grid, dim3(kThreads), smem_bytes(G), s,
                        static_cast<const T*>(q), static_cast<const uint8_t*>(pages), a,
                        static_cast<T*>(out)) != cudaSuccess)
     return CTI_ERR_CUDA;
@@ -701,9 +742,9 @@ int launch(const void* q, const void* pages, const Args& a, const Plan& p, void*
 
 template <typename T, int G>
 int launch_join(const Args& a, int splits, void* out, cudaStream_t s) {
-  const int64_t blocks = ((int64_t)a.tokens * a.heads + 3) / 4;
-  return launch_dependent(kv4_join_kernel<T, G>, dim3((unsigned)blocks), dim3(128), 0, s, a,
-                          splits, static_cast<T*>(out)) == cudaSuccess
+  const dim3 grid((unsigned)((int64_t)a.tokens * a.heads));
+  return launch_dependent(kv4_join_kernel<T, G>, grid, dim3(kJoinWarps * 32), 0, s, a, splits,
+                          static_cast<T*>(out)) == cudaSuccess
              ? CTI_OK
              : CTI_ERR_CUDA;
 }
