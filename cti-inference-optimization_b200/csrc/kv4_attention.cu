@@ -44,16 +44,21 @@ using namespace kv4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Warps of a block, and blocks of an SM: what registers allow.  Page parts (a
-// page's keys, or its values) in a warp's ring.
+// Warps of a block, and blocks of an SM: what registers allow.  The slots of a
+// warp's ring hold pages, or, where those are large, a page's keys or its
+// values.
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-__host__ __device__ constexpr int slots(int G) { return G == 4 ? 2 : 4; }
+__host__ __device__ constexpr bool halves(int G) { return G == 4; }
+__host__ __device__ constexpr int slot_bytes(int G) {
+  return halves(G) ? part_bytes(G) : block_bytes(G);
+}
+__host__ __device__ constexpr int slots(int G) { return G == 1 ? 3 : 2; }
 __host__ __device__ constexpr int blocks_per_sm(int G, int NT) {
   return NT == 4 ? 2 : G == 4 ? (NT == 1 ? 4 : 2) : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 5 : 4;
 }
 __host__ __device__ constexpr size_t smem_bytes(int G) {
-  return (size_t)kWarps * slots(G) * (part_bytes(G) + 8);
+  return (size_t)kWarps * slots(G) * (slot_bytes(G) + 8);
 }
 
 template <typename T>
@@ -87,6 +92,12 @@ CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* 
       : "memory");
 }
 
+CTI_DEVICE float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Word i of a lane's vectors of codes (i is known when the code is compiled).
 template <int N>
 CTI_DEVICE uint32_t word_of(const uint4 (&v)[N], int i) {
@@ -117,12 +128,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
   constexpr int ROWS = 8 * NT;
   constexpr int S = slots(G);
   constexpr int W = kWarps;
-  constexpr int kPart = part_bytes(G);
+  constexpr int kSlot = slot_bytes(G);
+  constexpr float kOffUnit = Y::kShift == 3 ? 1.0f : 0x1p14f;
+  constexpr int H = halves(G) ? 2 : 1;  // slots that a page takes
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = warp_id(), lane = lane_id();
   const int r8 = lane >> 2, t4 = lane & 3;
-  uint8_t* ring = smem + (size_t)warp * S * kPart;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)W * S * kPart) + warp * S;
+  uint8_t* ring = smem + (size_t)warp * S * kSlot;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)W * S * kSlot) + warp * S;
   if (lane == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
@@ -152,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
   const int32_t* table = a.table + s * a.table_stride;
   const uint8_t* base = pages + (int64_t)kvh * block_bytes(G);
   const int64_t page_stride = (int64_t)a.kv_heads * block_bytes(G);
-  uint32_t count = 0;  // page parts copied so far: slot and parity
+  uint32_t count = 0;  // slots filled so far: place and parity
   bool dead = false;   // a copy did not arrive in time
 
   for (int tile = blockIdx.y; tile < (rows + ROWS - 1) / ROWS; tile += gridDim.y) {
@@ -176,29 +189,30 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     if (dead) np = 0;
     int ids = -1;      // lane i: page p0 + (chunk of 32) + i
     uint32_t bad[2] = {0, 0};  // by chunk: bit per page that is none; nothing of it is seen
-    auto issue = [&](int h) {  // keys (h = 2 i) or values (2 i + 1) of page i of the range
-      const int i = h >> 1;
-      if ((h & 63) == 0) {
+    auto issue = [&](int h) {  // page i of the range; with halves its keys (h = 2 i) or values
+      const int i = h / H;
+      if ((h & (32 * H - 1)) == 0) {
         ids = i + lane < np ? __ldg(table + p0 + i + lane) : 0;
         if (ids < 0 || ids >= a.num_pages) {
           raise_status(a.status, CTI_ERR_BOUNDS, s);
           ids = -1;
         }
-        bad[(h >> 6) & 1] = __ballot_sync(0xffffffffu, ids < 0);
+        bad[(i >> 5) & 1] = __ballot_sync(0xffffffffu, ids < 0);
       }
       const int id = __shfl_sync(0xffffffffu, ids, i & 31);
       const uint32_t slot = (count + h) % S;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&full[slot], kPart);
-        bulk_load(ring + slot * kPart, base + max(id, 0) * page_stride + (h & 1) * kPart, kPart,
+        mbar_arrive_expect_tx(&full[slot], kSlot);
+        bulk_load(ring + slot * kSlot, base + max(id, 0) * page_stride + (h & (H - 1)) * kSlot, kSlot,
                   &full[slot]);
       }
     };
     auto arrived = [&](int h) {
       return __all_sync(0xffffffffu, mbar_wait(&full[(count + h) % S], ((count + h) / S) & 1,
-                                               a.status, 0x700 + (h & 1), nullptr));
+                                               a.status, 0x700, nullptr));
     };
-    for (int h = 0; h < S && h < 2 * np; ++h) issue(h);
+#pragma unroll 1
+    for (int h = 0; h < S && h < H * np; ++h) issue(h);
 
     // ---- queries: lane 4 r + t has dims 8 t .. + 7 of every group of row r ----
     uint32_t qb[NT][G][4];
@@ -244,8 +258,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
         if (g == (t4 & (G - 1))) sum_mine = sum;
       }
       // The offsets' operand: the rows that meet s and b of a group are 16 and
-      // 1 times the sum of q in it, in two parts, in units of 2^10.
-      sum_mine *= 0x1p-10f;
+      // 1 times the sum of q in it, in two parts, in the scores' units (fp16
+      // cannot hold those: 2^14 above them).
+      sum_mine *= kOffUnit * 0x1p-24f;
       const float hi = Y::to_float(Y::bits(sum_mine));
       const float lo = sum_mine - hi;
       const uint32_t hi2 = Y::pack(16.0f * hi, hi), lo2 = Y::pack(16.0f * lo, lo);
@@ -279,9 +294,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
 
     int done = 0;
     for (; done < np; ++done) {
-      if (!arrived(2 * done)) break;
-      const uint8_t* blk = ring + (count + 2 * done) % S * kPart;
-      uint8_t* vblk = ring + (count + 2 * done + 1) % S * kPart;
+      if (!arrived(H * done)) break;
+      uint8_t* blk = ring + (count + H * done) % S * kSlot;
+      uint8_t* vblk = H == 1 ? blk + part_bytes(G) : ring + (count + 2 * done + 1) % S * kSlot;
 
       // ---- S^T = K Q^T, 16 keys at a time ----
       float sc[NT][4][4];
@@ -315,10 +330,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
         const uint32_t off_a[4] = {am[0], am[1], G == 4 ? am[0] : 0u, G == 4 ? am[1] : 0u};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          Mma<T>::run(c, off_a, off_b[n][0], off_b[n][1]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[n][mt][e] = c[e] * 0x1p-14f;
+          for (int e = 0; e < 4; ++e) sc[n][mt][e] = 0.0f;
+          Mma<T>::run(sc[n][mt], off_a, off_b[n][0], off_b[n][1]);
+          if (kOffUnit != 1.0f) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][mt][e] *= 1.0f / kOffUnit;
+          }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -332,17 +350,20 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             Mma<__half>::run(c, a0, qb[n][g][0], qb[n][g][1]);
             Mma<__half>::run(c, a1, qb[n][g][2], qb[n][g][3]);
-            sc[n][mt][0] = fmaf(c[0], s0, sc[n][mt][0]);
-            sc[n][mt][1] = fmaf(c[1], s0, sc[n][mt][1]);
-            sc[n][mt][2] = fmaf(c[2], s1, sc[n][mt][2]);
-            sc[n][mt][3] = fmaf(c[3], s1, sc[n][mt][3]);
+            float(&x)[4] = sc[n][mt];
+            f2_unpack(f2_fma(f2_pack(c[0], c[1]), f2_pack(s0, s0), f2_pack(x[0], x[1])), x[0],
+                      x[1]);
+            f2_unpack(f2_fma(f2_pack(c[2], c[3]), f2_pack(s1, s1), f2_pack(x[2], x[3])), x[2],
+                      x[3]);
           }
         }
       }
 
-      __syncwarp();
-      if (2 * done + S < 2 * np) issue(2 * done + S);
-      if (!arrived(2 * done + 1)) break;
+      if (H == 2) {
+        __syncwarp();
+        if (2 * done + S < 2 * np) issue(2 * done + S);
+        if (!arrived(2 * done + 1)) break;
+      }
 
       const int key0 = (p0 + done) * kPage;
       const bool is_bad = bad[(done >> 5) & 1] >> (done & 31) & 1;
@@ -405,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
         for (int e = 0; e < 2; ++e) {
           float x = fmaxf(sc[n][0][e], sc[n][0][2 + e]);
 #pragma unroll
-          for (int mt = 1; mt < 4; ++mt) x = fmaxf(x, fmaxf(sc[n][mt][e], sc[n][mt][2 + e]));
+          for (int mt = 1; mt < 4; ++mt) x = max3f(x, sc[n][mt][e], sc[n][mt][2 + e]);
           mx[n][e] = x;
           raise = raise || (x - m[n][e]) * sl[n][e] > kSlack;
         }
@@ -451,10 +472,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float(&x)[4] = sc[n][kk];
+          const uint64_t sl2 = f2_pack(sl[n][0], sl[n][1]), no2 = f2_pack(noff[n][0], noff[n][1]);
+          f2_unpack(f2_fma(f2_pack(x[0], x[1]), sl2, no2), x[0], x[1]);
+          f2_unpack(f2_fma(f2_pack(x[2], x[3]), sl2, no2), x[2], x[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = ex2_approx(fmaf(x[e], sl[n][e & 1], noff[n][e & 1]));
-          l[n][0] += x[0] + x[2];
-          l[n][1] += x[1] + x[3];
+          for (int e = 0; e < 4; ++e) x[e] = ex2_approx(x[e]);
+          f2_unpack(f2_add(f2_pack(l[n][0], l[n][1]),
+                           f2_add(f2_pack(x[0], x[1]), f2_pack(x[2], x[3]))),
+                    l[n][0], l[n][1]);
           pb[n][0] = transpose8(Y::pack(x[0], x[1]));
           pb[n][1] = transpose8(Y::pack(x[2], x[3]));
         }
@@ -492,13 +517,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
         }
       }
       __syncwarp();
-      if (2 * done + 1 + S < 2 * np) issue(2 * done + 1 + S);
+      if (H * (done + 1) - 1 + S < H * np) issue(H * (done + 1) - 1 + S);
     }
     if (done < np) {  // let the copies in flight land, then give up
       dead = true;
-      for (int h = 2 * done; h < 2 * np && h <= 2 * done + S; ++h) arrived(h);
+      for (int h = H * done; h < H * np && h <= H * done + S; ++h) arrived(h);
     }
-    count += 2 * np;
+    count += H * np;
 
     // ---- join and store: lane 4 r + t has dims 4 r .. + 3 of every group ----
 #pragma unroll
@@ -512,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     if (shared) {
       // Every warp's rows in its own ring, then the first warp adds them up.
       float* mine = reinterpret_cast<float*>(ring);
-      static_assert((ROWS * D + 2 * ROWS) * 4 <= S * kPart, "room for the rows");
+      static_assert((ROWS * D + 2 * ROWS) * 4 <= S * kSlot, "room for the rows");
       __syncwarp();
       if (warp != 0) {
 #pragma unroll
@@ -533,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
       __syncthreads();
       if (warp == 0) {
         for (int w = 1; w < W; ++w) {
-          const float* src = reinterpret_cast<const float*>(ring + (size_t)w * S * kPart);
+          const float* src = reinterpret_cast<const float*>(ring + (size_t)w * S * kSlot);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
