@@ -55,7 +55,7 @@ __host__ __device__ constexpr int slot_bytes(int G) {
 }
 __host__ __device__ constexpr int slots(int G) { return G == 1 ? 3 : 2; }
 __host__ __device__ constexpr int blocks_per_sm(int G, int NT) {
-  return NT == 4 ? 2 : G == 4 ? (NT == 1 ? 4 : 2) : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 5 : 4;
+  return NT == 4 ? 2 : G == 4 ? (NT == 1 ? 4 : 2) : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 6 : 4;
 }
 __host__ __device__ constexpr size_t smem_bytes(int G) {
   return (size_t)kWarps * slots(G) * (slot_bytes(G) + 8);

@@ -35,9 +35,11 @@ class KV4Cache:
         self.kv_heads = int(kv_heads)
         self.head_dim = int(head_dim)
         self.dtype = dtype
+        self.dtype_code = _lib.DTYPE_CODES[dtype]
         self.pages = torch.zeros((int(num_pages), self.kv_heads, page_bytes // self.kv_heads),
                                  dtype=torch.uint8, device=device)
         self.device = self.pages.device
+        self.index = self.pages.get_device()  # -1 on the CPU
 
     @property
     def num_pages(self) -> int:

@@ -358,15 +358,18 @@ def ctr_head(h: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tens
     return logits, probs
 
 
-def _kv4_run(cache: KV4Cache, fn, what: str, *args) -> None:
+_INT32 = torch.int32
+
+
+def _kv4_run(cache: KV4Cache, fn, what: str, args: tuple) -> None:
     """Calls a kv4 entry point on the cache's device and its current stream."""
-    index = cache.device.index
-    args += (status_word(cache.device).data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+    index = cache.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
     if torch._C._cuda_getDevice() == index:
-        rc = fn(*args)
+        rc = fn(*args, status_word(cache.device).data_ptr(), stream)
     else:
         with torch.cuda.device(index):
-            rc = fn(*args)
+            rc = fn(*args, status_word(cache.device).data_ptr(), stream)
     if rc:
         check(rc, what)
 
@@ -375,42 +378,54 @@ def _kv4_rows(t: torch.Tensor, name: str, cache: KV4Cache, heads: int) -> tuple[
     """(tokens, token stride) of a [tokens, heads, head_dim] view with contiguous heads in the
     cache's type."""
     hd = cache.head_dim
-    if not t.is_cuda or t.dtype != cache.dtype:
+    if t.dtype is not cache.dtype or not t.is_cuda:
         raise TypeError(f"{name} must be a {cache.dtype} CUDA tensor")
-    if t.get_device() != cache.device.index:
+    if t.get_device() != cache.index:
         raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    if t.dim() != 3 or t.size(1) != heads or t.size(2) != hd:
-        raise ValueError(f"{name} must be [tokens, {heads}, {hd}], got {tuple(t.shape)}")
-    n = t.size(0)
-    if n and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd)):
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != hd:
+        raise ValueError(f"{name} must be [tokens, {heads}, {hd}], got {tuple(shape)}")
+    n, stride = shape[0], t.stride()
+    if n and (stride[2] != 1 or (heads > 1 and stride[1] != hd)):
         raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous heads")
-    return n, t.stride(0) if n > 1 else heads * hd  # a single token has any stride
+    return n, stride[0] if n > 1 else heads * hd  # a single token has any stride
 
 
 def _kv4_index(cache: KV4Cache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
                page_table: torch.Tensor) -> tuple:
     """Checks the index tensors; the arguments that every kv4 entry point takes of them, up to the
     number of sequences."""
-    index = cache.device.index
-    for name, t in (("cu_seqlens", cu_seqlens), ("kv_lens", kv_lens), ("page_table", page_table)):
-        if t.dtype is not torch.int32 or not t.is_cuda:
-            require_cuda(t, name)
-            raise TypeError(f"{name} must be torch.int32, got {t.dtype}")
-        if t.get_device() != index:
-            raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    n = kv_lens.size(0) if kv_lens.dim() == 1 else -1
-    if n < 0 or cu_seqlens.dim() != 1 or cu_seqlens.size(0) != n + 1:
-        raise ValueError("kv_lens must be [N] and cu_seqlens [N + 1], got "
-                         f"{tuple(kv_lens.shape)} and {tuple(cu_seqlens.shape)}")
-    if not kv_lens.is_contiguous() or not cu_seqlens.is_contiguous():
-        raise ValueError("kv_lens and cu_seqlens must be contiguous")
-    if page_table.dim() != 2 or page_table.size(0) != n:
-        raise ValueError(f"page_table must be [{n}, pages], got {tuple(page_table.shape)}")
-    cols = page_table.size(1)
-    if n and cols > 1 and page_table.stride(1) != 1:
-        raise ValueError("page_table rows must be contiguous")
-    return (cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
-            page_table.stride(0) if n > 1 else cols, cols, n)
+    index, shape = cache.index, page_table.shape
+    n = kv_lens.numel()
+    if (index >= 0 and cu_seqlens.dtype is _INT32 and kv_lens.dtype is _INT32
+            and page_table.dtype is _INT32 and cu_seqlens.get_device() == index
+            and kv_lens.get_device() == index and page_table.get_device() == index
+            and kv_lens.dim() == 1 and cu_seqlens.dim() == 1 and cu_seqlens.numel() == n + 1
+            and len(shape) == 2 and shape[0] == n and kv_lens.is_contiguous()
+            and cu_seqlens.is_contiguous()):
+        cols, stride = shape[1], page_table.stride()
+        if not n or cols <= 1 or stride[1] == 1:
+            return (cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
+                    stride[0] if n > 1 else cols, cols, n)
+    raise _kv4_index_error(cache, cu_seqlens, kv_lens, page_table)
+
+
+def _kv4_index_error(cache, cu_seqlens, kv_lens, page_table) -> Exception:
+    """What is wrong with the index tensors."""
+    if cache.index < 0:
+        return RuntimeError("the cache must be on a CUDA device (this library has no CPU path)")
+    for name, t, dims in (("cu_seqlens", cu_seqlens, 1), ("kv_lens", kv_lens, 1),
+                          ("page_table", page_table, 2)):
+        if t.dtype is not _INT32 or not t.is_cuda:
+            return TypeError(f"{name} must be an int32 CUDA tensor, got {t.dtype} on {t.device}")
+        if t.get_device() != cache.index:
+            return ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+        if t.dim() != dims or (dims == 1 and not t.is_contiguous()):
+            return ValueError(f"{name} must have {dims} contiguous dimension(s), got "
+                              f"{tuple(t.shape)}")
+    return ValueError("kv_lens must be [N], cu_seqlens [N + 1] and page_table [N, pages] with "
+                      f"contiguous rows, got {tuple(kv_lens.shape)}, {tuple(cu_seqlens.shape)} "
+                      f"and {tuple(page_table.shape)}")
 
 
 @lru_cache(maxsize=256)
@@ -433,9 +448,9 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, cu_seqlens: to
     if v_tokens != tokens:
         raise ValueError("k and v must have the same number of tokens")
     pages = cache.pages
-    _kv4_run(cache, lib.cti_kv4_append, "cti_kv4_append", k.data_ptr(), v.data_ptr(), k_stride,
-             v_stride, _lib.DTYPE_CODES[cache.dtype], *seqs, tokens, H, cache.head_dim,
-             pages.data_ptr(), pages.size(0))
+    _kv4_run(cache, lib.cti_kv4_append, "cti_kv4_append",
+             (k.data_ptr(), v.data_ptr(), k_stride, v_stride, cache.dtype_code, *seqs, tokens, H,
+              cache.head_dim, pages.data_ptr(), pages.size(0)))
 
 
 def kv4_read(cache: KV4Cache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
@@ -462,9 +477,9 @@ def kv4_read(cache: KV4Cache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
         if k_tokens != tokens or v_tokens != tokens:
             raise ValueError(f"out must hold {tokens} tokens")
     pages = cache.pages
-    _kv4_run(cache, lib.cti_kv4_read, "cti_kv4_read", pages.data_ptr(), pages.size(0),
-             _lib.DTYPE_CODES[cache.dtype], *seqs, tokens, H, hd, k.data_ptr(), v.data_ptr(),
-             k_stride, v_stride)
+    _kv4_run(cache, lib.cti_kv4_read, "cti_kv4_read",
+             (pages.data_ptr(), pages.size(0), cache.dtype_code, *seqs, tokens, H, hd,
+              k.data_ptr(), v.data_ptr(), k_stride, v_stride))
     return k, v
 
 
@@ -484,12 +499,12 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
     head_dim]; a token that sees no key is zero."""
     seqs = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
     hd, Hkv = cache.head_dim, cache.kv_heads
-    H = q.size(1) if q.dim() == 3 else 0
+    H = q.shape[1] if q.dim() == 3 else 0
     if H <= 0 or H % Hkv:
         raise ValueError(f"q must be [tokens, heads, head_dim] with heads a multiple of {Hkv}, "
                          f"got {tuple(q.shape)}")
     T, q_stride = _kv4_rows(q, "q", cache, H)
-    cols, n = seqs[4:]
+    cols, n = seqs[4], seqs[5]
     if max_new is None:
         max_new = 1 if T <= n else T
     if max_kv_len is None:
@@ -497,7 +512,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
     if scale is None:
         scale = hd ** -0.5
     if out is None:
-        out = torch.empty((T, H, hd), dtype=cache.dtype, device=cache.device)
+        out = q.new_empty((T, H, hd))
     else:
         _kv4_rows(out, "out", cache, H)
         if out.size(0) != T or not out.is_contiguous():
@@ -506,8 +521,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
     need = _kv4_workspace_bytes(n, T, max_new, max_kv_len, H, Hkv, hd)
     ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     pages = cache.pages
-    _kv4_run(cache, lib.cti_kv4_attention, "cti_kv4_attention", q.data_ptr(), q_stride,
-             _lib.DTYPE_CODES[cache.dtype], *seqs, T, max_new, max_kv_len, H, Hkv, hd,
-             float(scale), 1 if causal else 0, pages.data_ptr(), pages.size(0), out.data_ptr(),
-             ptr(ws), need)
+    _kv4_run(cache, lib.cti_kv4_attention, "cti_kv4_attention",
+             (q.data_ptr(), q_stride, cache.dtype_code, *seqs, T, max_new, max_kv_len, H, Hkv, hd,
+              float(scale), 1 if causal else 0, pages.data_ptr(), pages.size(0), out.data_ptr(),
+              ptr(ws), need))
     return out
