@@ -6,7 +6,7 @@
 //           side by side in one page; a warp takes a run's keys or values in
 //           one head.  Its lanes are those of the page's layout, so it moves
 //           whole 16-byte vectors of codes.
-//   tokens  a block takes 8 packed tokens, every thread 8 dims of a token's
+//   tokens  a block takes 8 packed tokens, every thread 16 dims of a token's
 //           key and value.  For calls with a few tokens per sequence, whose
 //           runs would leave most lanes of a warp idle.
 // HBM-bound: 4 + 1.25 bytes per element pair (a key's and a value's) either
@@ -43,16 +43,6 @@ struct Args {
   int tile;  // packed tokens of a block
 };
 
-CTI_DEVICE float min_nan(float a, float b) {
-  float d;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-CTI_DEVICE float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 CTI_DEVICE float min3_nan(float a, float b, float c) {
   float d;
   asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -61,6 +51,17 @@ CTI_DEVICE float min3_nan(float a, float b, float c) {
 CTI_DEVICE float max3_nan(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The smaller of both halves of two numbers of T; NaN if one is.
+template <typename T>
+CTI_DEVICE uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (Type16<T>::kShift == 3)
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 
@@ -84,7 +85,7 @@ __host__ __device__ constexpr int dim_at(Order order, int nibble) {
 }
 
 template <typename T>
-CTI_DEVICE void unpack(const uint4& raw, float (&x)[8]) {
+CTI_DEVICE void unpack(const uint4& raw, float* x) {
   using Y = Type16<T>;
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
@@ -97,7 +98,7 @@ CTI_DEVICE void unpack(const uint4& raw, float (&x)[8]) {
 // The nibbles of the 8 t (kRoundBits + 16 + n as bits): a chain of shift-adds
 // less what is not n.
 template <Order ORDER>
-CTI_DEVICE uint32_t pack_codes(const float (&t)[8]) {
+CTI_DEVICE uint32_t pack_codes(const float* t) {
   uint32_t word = 0, less = 0;
 #pragma unroll
   for (int i = 7; i >= 0; --i) {
@@ -128,67 +129,84 @@ __device__ __noinline__ uint32_t codes_again(uint4 raw, float s, float b, float 
   return pack_codes<ORDER>(t);
 }
 
-// Packs 8 values of a group of 32 (the lanes of the quad have the others)
-// into a word of codes.  Also the group's scale and base, 16 bits each.
-// Bound by instructions: about 80 with the group's part, the element's
-// arithmetic two at a time.
+// Packs 16 values of a group of 32 (the lane whose number differs in bit 0 has
+// the others) into two words of codes.  Also the group's scale and base, 16
+// bits each.  Bound by instructions: about 9 a value with the group's part, the
+// values' arithmetic two at a time.  (With 8 values a lane, where the group's
+// part is done by four lanes: 13.)
 template <typename T, Order ORDER>
-CTI_DEVICE uint32_t quantise(const uint4& raw, uint32_t& s_bits, uint32_t& b_bits) {
+CTI_DEVICE void quantise(const uint4 (&raw)[2], uint32_t (&word)[2], uint32_t& s_bits,
+                         uint32_t& b_bits) {
   using Y = Type16<T>;
-  float x[8];
-  unpack<T>(raw, x);
-  float lo = min3_nan(min3_nan(min3_nan(x[0], x[1], x[2]), x[3], x[4]), x[5], min_nan(x[6], x[7]));
-  float hi = max3_nan(max3_nan(max3_nan(x[0], x[1], x[2]), x[3], x[4]), x[5], max_nan(x[6], x[7]));
+  float x[16];
+  unpack<T>(raw[0], x);
+  unpack<T>(raw[1], x + 8);
+  float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  for (int i = 1; i < 15; i += 2) {
+    lo = min3_nan(lo, x[i], x[i + 1]);
+    hi = max3_nan(hi, x[i], x[i + 1]);
   }
-  // (hi - lo) / 15 in the same way; its rounding on to T is right too: the
-  // quotient is nearer to the true value than to any border of T that it does
-  // not lie on.
+  lo = min3_nan(lo, x[15], x[15]);
+  hi = max3_nan(hi, x[15], x[15]);
+  // Both ends in one exchange: they are numbers of T.
+  uint32_t both = Y::pack(lo, -hi);
+  both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, 1));
+  lo = Y::low(both);
+  hi = -Y::high(both);
+  // (hi - lo) / 15 in the same way as the codes' quotients; its rounding on to
+  // T is right too: it is nearer to the true value than to any border of T that
+  // it does not lie on.
   const float range = hi - lo;
   const float q = range * (1.0f / 15.0f);
   s_bits = Y::bits(fmaf(fmaf(-15.0f, q, range), 1.0f / 15.0f, q));
-  float s = Y::to_float(s_bits);
-  if (s < FLT_MIN) {  // below the smallest normal fp32 number: a constant group
-    s = 0.0f;
-    s_bits = 0;
-  }
+  const float s = Y::to_float(s_bits);
   b_bits = Y::bits(fmaf(-16.0f, s, lo));
   const float b = Y::to_float(b_bits);
-  if (!(fabsf(b) <= FLT_MAX) || !(s <= FLT_MAX)) s_bits = b_bits = 0x7fffu;  // NaN in both types
+  if (!(s >= FLT_MIN && s <= FLT_MAX && fabsf(b) <= FLT_MAX)) {
+    word[0] = word[1] = 0;
+    if (s < FLT_MIN) {  // below the smallest normal fp32 number: a constant group
+      s_bits = 0;
+      b_bits = Y::bits(lo);
+    } else {
+      s_bits = b_bits = 0x7fffu;  // NaN in both types
+    }
+    return;
+  }
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  float add = kRound;
-  if (s == 0.0f) {
-    inv = 0.0f;
-    add = kRound + 16.0f;
-  }
   // a / s for two values at once
   const uint64_t ns2 = f2_pack(-s, -s), nb2 = f2_pack(-b, -b), inv2 = f2_pack(inv, inv);
-  const uint64_t add2 = f2_pack(add, add);
-  auto k_of = [&](float x0, float x1, float& t0, float& t1) {
+  const uint64_t add2 = f2_pack(kRound, kRound);
+  auto quotient = [&](float x0, float x1) {
     const uint64_t a = f2_add(f2_pack(x0, x1), nb2);
     const uint64_t e = f2_mul(a, inv2);
-    f2_unpack(f2_add(f2_fma(f2_fma(ns2, e, a), inv2, e), add2), t0, t1);
+    return f2_fma(f2_fma(ns2, e, a), inv2, e);
   };
-  float t[8];
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) k_of(x[i], x[i + 1], t[i], t[i + 1]);
   float t_lo, t_hi;
-  k_of(lo, hi, t_lo, t_hi);
+  f2_unpack(f2_add(quotient(lo, hi), add2), t_lo, t_hi);
   bool again = t_lo < kRound + 16.0f || t_hi > kRound + 31.0f;
   // -b on a border: -b / s = a whole number and a half
   const float e0 = -b * inv, e1 = fmaf(fmaf(-s, e0, -b), inv, e0);
-  if (fabsf(e1 - rintf(e1)) == 0.5f) {
+  if (fabsf(e1 - ((e1 + kRound) - kRound)) == 0.5f) {
     float least = INFINITY;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) least = fminf(least, x[i] == 0.0f ? INFINITY : fabsf(x[i]));
+    for (int i = 0; i < 16; ++i) least = fminf(least, x[i] == 0.0f ? INFINITY : fabsf(x[i]));
     again = again || least < fabsf(b) * 0x1p-12f;
   }
-  if (again) return codes_again<T, ORDER>(raw, s, b, inv);
-  return pack_codes<ORDER>(t);
+  if (again) {
+    word[0] = codes_again<T, ORDER>(raw[0], s, b, inv);
+    word[1] = codes_again<T, ORDER>(raw[1], s, b, inv);
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+      f2_unpack(f2_add(quotient(x[8 * h + i], x[8 * h + i + 1]), add2), t[i], t[i + 1]);
+    word[h] = pack_codes<ORDER>(t);
+  }
 }
 
 CTI_DEVICE uint32_t twice(uint32_t h) { return __byte_perm(h, h, 0x1010); }
@@ -230,28 +248,39 @@ __global__ void __launch_bounds__(kThreads)
   const int t0 = blockIdx.x * kTokens;
   if (threadIdx.x < kTokens) places[threadIdx.x] = find_place(a, t0 + threadIdx.x);
   __syncthreads();
-  const int per = a.kv_heads * G * 4;  // 8-dim pieces of a token
-  const int total = kTokens * per;     // a multiple of 32
+  const int per = a.kv_heads * G * 2;  // 16-dim pieces of a token
+  const int total = (kTokens * per + 31) & ~31;
   for (int i = threadIdx.x; i < total; i += kThreads) {
     const int tok = i / per, piece = i - tok * per;
-    const Place at = places[tok];
-    const int head = piece / (4 * G), g = (piece >> 2) & (G - 1), t = piece & 3;
+    const Place at = tok < kTokens ? places[tok] : Place{-1, 0};
+    const int head = piece / (2 * G), g = (piece >> 1) & (G - 1), t = 2 * (piece & 1);
     const bool live = at.page >= 0;
-    uint4 rk = make_uint4(0, 0, 0, 0), rv = rk;
+    uint4 rk[2], rv[2];
+    rk[0] = rk[1] = rv[0] = rv[1] = make_uint4(0, 0, 0, 0);
     if (live) {
-      rk = __ldg(reinterpret_cast<const uint4*>(k + (t0 + tok) * a.k_stride + piece * 8));
-      rv = __ldg(reinterpret_cast<const uint4*>(v + (t0 + tok) * a.v_stride + piece * 8));
+      const uint4* pk =
+          reinterpret_cast<const uint4*>(k + (t0 + tok) * a.k_stride + piece * 16);
+      const uint4* pv =
+          reinterpret_cast<const uint4*>(v + (t0 + tok) * a.v_stride + piece * 16);
+      rk[0] = __ldg(pk);
+      rk[1] = __ldg(pk + 1);
+      rv[0] = __ldg(pv);
+      rv[1] = __ldg(pv + 1);
     }
-    uint32_t ks, kb, vs, vb;
-    const uint32_t wk = quantise<T, kKeys>(rk, ks, kb);
-    const uint32_t wv = quantise<T, kValues>(rv, vs, vb);
+    uint32_t ks, kb, vs, vb, wk[2], wv[2];
+    quantise<T, kKeys>(rk, wk, ks, kb);
+    quantise<T, kValues>(rv, wv, vs, vb);
     if (!live) continue;  // the loop's bound is the same for a whole warp
     uint8_t* block = pages + (at.page * a.kv_heads + head) * (int64_t)block_bytes(G);
-    *reinterpret_cast<uint32_t*>(block + k_word_at(at.slot, g, t, G)) = wk;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-      *reinterpret_cast<uint16_t*>(block + v_codes_at(G) + v_half_at(at.slot, g, 2 * t + c, G)) =
-          (uint16_t)(wv >> (16 * c));
+    for (int x = 0; x < 2; ++x) {
+      *reinterpret_cast<uint32_t*>(block + k_word_at(at.slot, g, t + x, G)) = wk[x];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<uint16_t*>(block + v_codes_at(G) +
+                                     v_half_at(at.slot, g, 2 * (t + x) + c, G)) =
+            (uint16_t)(wv[x] >> (16 * c));
+    }
     if (t == 0) {
       *reinterpret_cast<uint32_t*>(block + k_meta_at(G) + k_meta_word_at(at.slot, g, G)) =
           ks | kb << 16;
@@ -375,77 +404,89 @@ CTI_DEVICE int find_runs(const Args& a, int t0, Run (&runs)[kRunTokens]) {
   return count;
 }
 
-// A run's keys (or values) of one head.  Lane 4 r + t takes dims 8 t .. + 7 of
-// every group of token 8 nt + r.
+// A run's keys (or values) of one head.  Lane 16 z + 2 r + u takes dims 16 u ..
+// + 15 of token r of an octet: for every group (G = 2, 4), or of two octets
+// (G = 1).  A step takes 2 octets (4).
 template <typename T, int G, Order ORDER>
 CTI_DEVICE void append_run(const T* __restrict__ rows, int stride, const Run& run,
                            uint8_t* __restrict__ block, int lane) {
-  constexpr int kOctets = 4 / G;  // of tokens, in a vector of codes
-  const int r = lane >> 2, t = lane & 3, last = run.slot + run.count - 1;
-  // The lane whose word this one has in the end: keys, its own; values, the
-  // pair of tokens r / 2 and the 4 dims 2 t + r % 2.
-  const int owner = ORDER == kKeys ? lane : (2 * t + (r & 1)) * 4 + (r >> 1);
-  const int v0 = (run.slot >> 3) / kOctets;
-  int tau0 = v0 * kOctets * 8 + r;
-  int src = (tau0 - run.slot) * stride + 8 * t;
-  uint8_t* dst = block + (ORDER == kKeys ? 0 : v_codes_at(G)) + (v0 * 32 + owner) * 16;
-  for (; tau0 - r <= last; tau0 += 8 * kOctets, src += 8 * kOctets * stride, dst += 512) {
-    uint4 raw[4];
-    bool live[4];
+  constexpr int kOctets = G == 1 ? 4 : 2;
+  constexpr int N = G == 4 ? 4 : 2;  // words of a lane's two: side by side in a vector of codes
+  const int z = lane >> 4, r = (lane >> 1) & 7, u = lane & 1, last = run.slot + run.count - 1;
+  const bool odd = r & 1;
+  // The lanes of the layout whose words this one has in the end: keys, 4 r + 2 u
+  // and the next; values, those of the pair of tokens r / 2 and the dims 16 u + 8
+  // (r % 2) .. + 7.
+  const int owner0 = ORDER == kKeys ? 4 * r + 2 * u : (4 * u + 2 * (r & 1)) * 4 + (r >> 1);
+  constexpr int kNext = ORDER == kKeys ? 16 : 64;  // bytes to the second
+  uint8_t* codes = block + (ORDER == kKeys ? 0 : v_codes_at(G));
+  for (int nt0 = (run.slot >> 3) / kOctets * kOctets; 8 * nt0 <= last; nt0 += kOctets) {
+    const int nt = nt0 + (G == 1 ? 2 * z : z);  // this lane's (first) octet
+    const int src = (8 * nt + r - run.slot) * stride + 16 * u;
+    uint4 raw[N][2];
+    bool live[N];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int nt = j / G, g = j % G, tau = tau0 + 8 * nt;
+    for (int j = 0; j < N; ++j) {
+      const int tau = 8 * (G == 1 ? nt + j : nt) + r;
       live[j] = tau >= run.slot && tau <= last;
-      raw[j] = make_uint4(0, 0, 0, 0);
-      if (live[j])
-        raw[j] = __ldg(reinterpret_cast<const uint4*>(rows + (src + 8 * nt * stride) + 32 * g));
+      raw[j][0] = raw[j][1] = make_uint4(0, 0, 0, 0);
+      if (live[j]) {
+        const uint4* p = reinterpret_cast<const uint4*>(
+            rows + src + (G == 1 ? 8 * j * stride : 32 * j));
+        raw[j][0] = __ldg(p);
+        raw[j][1] = __ldg(p + 1);
+      }
     }
-    uint32_t w[4];
-    bool whole = true;
+    uint32_t w[N][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int nt = j / G, g = j % G, tau = tau0 + 8 * nt;
-      const bool pair = ORDER == kKeys ? live[j]
-                                       : live[j] && (tau ^ 1) >= run.slot && (tau ^ 1) <= last;
-      whole = whole && pair;
-      if (!__any_sync(0xffffffffu, live[j])) continue;
+    for (int j = 0; j < N; ++j) {
+      const int tau = 8 * (G == 1 ? nt + j : nt) + r, g = G == 1 ? 0 : j;
       uint32_t s, b;
-      const uint32_t word = quantise<T, ORDER>(raw[j], s, b);
+      quantise<T, ORDER>(raw[j], w[j], s, b);
       if (ORDER == kKeys) {
-        w[j] = word;
-        if (live[j] && t == 0)
+        if (live[j] && u == 0)
           *reinterpret_cast<uint32_t*>(block + k_meta_at(G) + k_meta_word_at(tau, g, G)) =
               s | b << 16;
       } else {
-        const bool odd = r & 1;
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? word : word >> 16, 4);
-        w[j] = odd ? __byte_perm(got, word, 0x7610) : __byte_perm(word, got, 0x5410);
-        const uint32_t mine = s | b << 16, meta = __shfl_xor_sync(0xffffffffu, mine, 4);
+        // Two tokens share a word: each lane of the pair gets half of the dims.
+        const bool pair = live[j] && (tau ^ 1) >= run.slot && (tau ^ 1) <= last;
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? w[j][0] : w[j][1], 2);
+        const uint32_t mine = s | b << 16, meta = __shfl_xor_sync(0xffffffffu, mine, 2);
         uint8_t* vm = block + v_meta_at(G) + v_meta_half_at(tau, g, G);
-        if (live[j] && t == 0) {
-          if (!pair) {
+        if (live[j] && !pair) {  // an end of the run: its own halves alone
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint16_t*>(codes + v_half_at(tau, g, 4 * u + c, G)) =
+                (uint16_t)(w[j][c >> 1] >> (16 * (c & 1)));
+          if (u == 0) {
             *reinterpret_cast<uint16_t*>(vm) = (uint16_t)s;
             *reinterpret_cast<uint16_t*>(vm + 4) = (uint16_t)b;
-          } else if (!odd) {
-            *reinterpret_cast<uint2*>(vm) =
-                make_uint2(__byte_perm(mine, meta, 0x5410), __byte_perm(mine, meta, 0x7632));
           }
+        } else if (pair && u == 0 && !odd) {
+          *reinterpret_cast<uint2*>(vm) =
+              make_uint2(__byte_perm(mine, meta, 0x5410), __byte_perm(mine, meta, 0x7632));
         }
-        if (live[j] && !pair) {  // an end of the run: its own halves alone
-          uint8_t* half = block + v_codes_at(G);
-          *reinterpret_cast<uint16_t*>(half + v_half_at(tau, g, 2 * t, G)) = (uint16_t)word;
-          *reinterpret_cast<uint16_t*>(half + v_half_at(tau, g, 2 * t + 1, G)) =
-              (uint16_t)(word >> 16);
-        }
+        const uint32_t even_w = odd ? got : w[j][0], odd_w = odd ? w[j][1] : got;
+        w[j][0] = __byte_perm(even_w, odd_w, 0x5410);
+        w[j][1] = __byte_perm(even_w, odd_w, 0x7632);
+        live[j] = pair;
       }
-      live[j] = pair;
     }
-    if (whole) {
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
+    const int word0 = nt * G;  // of the lane's words in the layout
+    uint8_t* dst = codes + ((word0 >> 2) * 32 + owner0) * 16 + (word0 & 3) * 4;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (live[j]) *reinterpret_cast<uint32_t*>(dst + 4 * j) = w[j];
+    for (int x = 0; x < 2; ++x) {
+      if constexpr (N == 4) {
+        if (live[0])
+          *reinterpret_cast<uint4*>(dst + x * kNext) =
+              make_uint4(w[0][x], w[1][x], w[2][x], w[3][x]);
+      } else if (live[0] && live[1]) {
+        *reinterpret_cast<uint2*>(dst + x * kNext) = make_uint2(w[0][x], w[1][x]);
+      } else {  // G = 1: one of two octets
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (live[j]) *reinterpret_cast<uint32_t*>(dst + x * kNext + 4 * j) = w[j][x];
+      }
     }
   }
 }
