@@ -2,10 +2,10 @@
 // (format: kv4.cuh).
 //
 // Two ways, by the tokens that a sequence has in the call:
-//   runs    a block takes 64 packed tokens and cuts them into runs that lie
-//           side by side in one page; a warp takes a run's keys or values in
-//           one head.  Its lanes are those of the page's layout, so it moves
-//           whole 16-byte vectors of codes.
+//   runs    a block finds the runs (tokens side by side in one page) that start
+//           among 64 or 128 packed tokens; a warp takes a run's keys or values
+//           in one head, with lanes laid out as the page's, so that it moves
+//           whole sectors of codes.
 //   tokens  a block takes 8 packed tokens, every thread 16 dims of a token's
 //           key and value.  For calls with a few tokens per sequence, whose
 //           runs would leave most lanes of a warp idle.
@@ -411,7 +411,7 @@ template <typename T, int G, Order ORDER>
 CTI_DEVICE void append_run(const T* __restrict__ rows, int stride, const Run& run,
                            uint8_t* __restrict__ block, int lane) {
   constexpr int kOctets = G == 1 ? 4 : 2;
-  constexpr int N = G == 4 ? 4 : 2;  // words of a lane's two: side by side in a vector of codes
+  constexpr int N = G == 4 ? 4 : 2;  // words that a lane has in each of two vectors of codes
   const int z = lane >> 4, r = (lane >> 1) & 7, u = lane & 1, last = run.slot + run.count - 1;
   const bool odd = r & 1;
   // The lanes of the layout whose words this one has in the end: keys, 4 r + 2 u
@@ -421,18 +421,18 @@ CTI_DEVICE void append_run(const T* __restrict__ rows, int stride, const Run& ru
   constexpr int kNext = ORDER == kKeys ? 16 : 64;  // bytes to the second
   uint8_t* codes = block + (ORDER == kKeys ? 0 : v_codes_at(G));
   for (int nt0 = (run.slot >> 3) / kOctets * kOctets; 8 * nt0 <= last; nt0 += kOctets) {
-    const int nt = nt0 + (G == 1 ? 2 * z : z);  // this lane's (first) octet
+    const int nt = nt0 + z;  // this lane's octet; G = 1: and the one after the next
     const int src = (8 * nt + r - run.slot) * stride + 16 * u;
     uint4 raw[N][2];
     bool live[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int tau = 8 * (G == 1 ? nt + j : nt) + r;
+      const int tau = 8 * (G == 1 ? nt + 2 * j : nt) + r;
       live[j] = tau >= run.slot && tau <= last;
       raw[j][0] = raw[j][1] = make_uint4(0, 0, 0, 0);
       if (live[j]) {
         const uint4* p = reinterpret_cast<const uint4*>(
-            rows + src + (G == 1 ? 8 * j * stride : 32 * j));
+            rows + src + (G == 1 ? 16 * j * stride : 32 * j));
         raw[j][0] = __ldg(p);
         raw[j][1] = __ldg(p + 1);
       }
@@ -440,7 +440,8 @@ CTI_DEVICE void append_run(const T* __restrict__ rows, int stride, const Run& ru
     uint32_t w[N][2];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int tau = 8 * (G == 1 ? nt + j : nt) + r, g = G == 1 ? 0 : j;
+      const int tau = 8 * (G == 1 ? nt + 2 * j : nt) + r, g = G == 1 ? 0 : j;
+      if (G == 1 && !__any_sync(0xffffffffu, live[j])) continue;
       uint32_t s, b;
       quantise<T, ORDER>(raw[j], w[j], s, b);
       if (ORDER == kKeys) {
@@ -480,12 +481,12 @@ CTI_DEVICE void append_run(const T* __restrict__ rows, int stride, const Run& ru
         if (live[0])
           *reinterpret_cast<uint4*>(dst + x * kNext) =
               make_uint4(w[0][x], w[1][x], w[2][x], w[3][x]);
-      } else if (live[0] && live[1]) {
-        *reinterpret_cast<uint2*>(dst + x * kNext) = make_uint2(w[0][x], w[1][x]);
-      } else {  // G = 1: one of two octets
+      } else if constexpr (G == 2) {
+        if (live[0]) *reinterpret_cast<uint2*>(dst + x * kNext) = make_uint2(w[0][x], w[1][x]);
+      } else {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          if (live[j]) *reinterpret_cast<uint32_t*>(dst + x * kNext + 4 * j) = w[j][x];
+          if (live[j]) *reinterpret_cast<uint32_t*>(dst + x * kNext + 8 * j) = w[j][x];
       }
     }
   }
@@ -659,7 +660,9 @@ struct Launch {
 Launch plan(Args& a, int G) {
   Launch l;
   l.runs = a.tokens >= (int64_t)kRunsFrom * a.num_seqs;
-  a.tile = l.runs ? kRunTokens : kTokens;
+  // Longer tiles share the way to their runs among more of them, as long as
+  // there are four blocks for each SM.
+  a.tile = !l.runs ? kTokens : a.tokens >= kSMs * 4 * kRunTokens ? kRunTokens : kRunTokens / 2;
   const int64_t tiles = ((int64_t)a.tokens + a.tile - 1) / a.tile;
   l.grid = dim3((unsigned)tiles);
   if (l.runs) {
