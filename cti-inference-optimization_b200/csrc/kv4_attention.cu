@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 
 // Query rows of a KV head, by the caller's bound, from which a sequence's rows
 // are taken in tiles of 128 on the tensor cores.
-constexpr int kTilesFrom = 33;
+constexpr int kTilesFrom = 97;
 
 // How a call is laid out over the GPU; a function of the sizes alone.
 struct Plan {

@@ -21,6 +21,7 @@
 // a bounded mbarrier wait; one that runs out records its site in the status
 // word and the roles unwind.
 #include <cfloat>
+#include <climits>
 
 #include "kv4_attention.cuh"
 
@@ -239,7 +240,8 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
       const int tok = live ? (int)a.by_group(row) : 0;
       const int head = kvh * group + (live ? row - tok * group : 0);
       const int64_t at = (int64_t)(begin + tok) * a.heads + head;
-      const int sees = !live ? 0 : a.causal ? min(first + tok + 1, limit) : limit;
+      // A row of no query sees everything: nothing is masked for it.
+      const int sees = !live ? INT_MAX : a.causal ? min(first + tok + 1, limit) : limit;
       // Queries: the row's largest magnitude, then fp16 in [2^14, 2^15) at most.
       const uint4* src =
           reinterpret_cast<const uint4*>(q + (begin + tok) * a.q_stride + (int64_t)head * D);
@@ -292,26 +294,28 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         }
         tc_fence_after();
         const uint32_t sb = lanes + 64u * b;
-        uint32_t v[2][32];
-        tmem_ld_32x32b_2x32_sync(sb, sb + 32, v[0], v[1]);
         const PageInfo pi = info[st];
         const int key0 = (rg.p0 + j) * kPage;
         const uint64_t nan_v = pi.nan_v[0] | pi.nan_v[1] | pi.nan_v[2] | pi.nan_v[3];
-        if (nan_v) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (nan_v >> (32 * c + e) & 1) v[c][e] = 0x7fffffffu;
-        }
         const int lim = min(sees - key0, pi.keys);
-        if (!__all_sync(0xffffffffu, lim >= kPage)) {
+        if (nan_v != 0 || !__all_sync(0xffffffffu, lim >= kPage)) {
+          // Scores that do not count, put back before the pass below (a short loop
+          // on its own keeps that pass's instructions few).
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[16];
+            tmem_ld_x16_sync(sb + 16 * c, x);
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * c + e >= lim) v[c][e] = __float_as_uint(-INFINITY);
+            for (int e = 0; e < 16; ++e) {
+              if (nan_v >> (16 * c + e) & 1) x[e] = 0x7fffffffu;
+              if (16 * c + e >= lim) x[e] = __float_as_uint(-INFINITY);
+            }
+            tmem_st_32x32b_x16(sb + 16 * c, x);
+          }
+          tmem_st_wait();
         }
+        uint32_t v[2][32];
+        tmem_ld_32x32b_2x32_sync(sb, sb + 32, v[0], v[1]);
         float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -501,7 +505,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             info[st].scale = __uint_as_float((uint32_t)(127 + e) << 23);
             info[st].keys = is_page ? kPage : 0;
           }
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < kVecs; ++x) {
             const int v = part * kVecs + x, nt0 = 4 * v / G;
             const uint4 w4 = *reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16);
@@ -534,7 +538,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         } else {
           uint64_t nan_bits = 0;
           uint8_t* vt = dst + Z::kKBytes;
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < kVecs; ++x) {
             const int v = part * kVecs + x, nt0 = 4 * v / G;
             const uint4 w4 =
