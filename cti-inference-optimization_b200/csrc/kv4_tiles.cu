@@ -314,16 +314,21 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
           }
           tmem_st_wait();
         }
-        uint32_t v[2][32];
-        tmem_ld_32x32b_2x32_sync(sb, sb + 32, v[0], v[1]);
+        // The scores go through registers 32 at a time, twice: short loops, whose
+        // instructions stay at hand while warps of other roles run between
+        // (unrolled, with one reading of all 64: 545 us instead of 502 for
+        // 5,500 tokens of 16 heads of 128 over 5,700 keys each).
         float mx = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t x[32];
+          tmem_ld_32x32b_x32_sync(sb + 32 * c, x);
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            mx = max3f(mx, __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
-            mx1 = max3f(mx1, __uint_as_float(v[c][e + 2]), __uint_as_float(v[c][e + 3]));
+            mx = max3f(mx, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            mx1 = max3f(mx1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
           }
+        }
         const float factor = fmaxf(down * pi.scale, 1e-37f);  // not 0: -inf stays -inf
         mx = fmaxf(mx, mx1) * factor;
         float corr = 1.0f;
@@ -355,14 +360,16 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         const float noff = m == -INFINITY ? 0.0f : -m;
         const uint64_t factor2 = f2_pack(factor, factor), noff2 = f2_pack(noff, noff);
         uint64_t sum_a = f2_pack(0.0f, 0.0f), sum_b = sum_a;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
+          uint32_t x[32];
+          tmem_ld_32x32b_x32_sync(sb + 32 * c, x);
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c][2 * e]),
-                                     __uint_as_float(v[c][2 * e + 1])),
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(x[2 * e]),
+                                     __uint_as_float(x[2 * e + 1])),
                              factor2, noff2),
                       x0, x1);
             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
