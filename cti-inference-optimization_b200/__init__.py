@@ -10,7 +10,8 @@ from . import build  # noqa: F401  (no CUDA needed)
 from ._lib import LIB_PATH, lib  # noqa: F401  (raises if the library is missing)
 from . import ops  # noqa: F401
 from .embedding import RepEncoder, flatten_slot_batch  # noqa: F401
-from .kv_cache import KV4Cache  # noqa: F401
+from .kv_cache import KV4Cache, SequenceCache  # noqa: F401
 from .moe import Expert, SMoE, TopKGate  # noqa: F401
 
-__all__ = ["SMoE", "TopKGate", "Expert", "RepEncoder", "KV4Cache", "ops", "flatten_slot_batch", "lib"]
+__all__ = ["SMoE", "TopKGate", "Expert", "RepEncoder", "KV4Cache", "SequenceCache", "ops",
+           "flatten_slot_batch", "lib"]

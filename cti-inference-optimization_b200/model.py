@@ -25,9 +25,12 @@ Attention over the packed sequences runs on this library's varlen causal
 attention kernel (``cti_varlen_attention``, head_dim 32); the reference
 builds a dense [T, T] mask instead (``get_sequence_causal_mask``,
 ``baseline/infer.py:420-427``), which does not fit at T = 278k.  There is
-no other backend: shapes the kernels do not cover raise.  This module
-is the model around the hot path; the hot path itself is the MoE layer and
-the pooling.
+no other backend: shapes the kernels do not cover raise.  A server that
+scores users as events arrive keeps their histories in a ``SequenceCache``
+(keys and values in 4 bits) and runs the new events alone
+(``predict_cached``); the reference runs whole sequences again
+(``baseline/infer.py:388-409``).  This module is the model around the hot
+path; the hot path itself is the MoE layer and the pooling.
 """
 from __future__ import annotations
 
@@ -39,6 +42,7 @@ import torch.nn as nn
 
 from . import ops
 from .embedding import RepEncoder
+from .kv_cache import KV4Cache, SequenceCache
 from .moe import SMoE
 
 
@@ -48,6 +52,17 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     (cti_varlen_attention, head_dim 32).  q, k, v [T, H, hd] bf16 CUDA
     views; cu_seqlens int32 [N+1]."""
     return ops.varlen_attention(q, k, v, cu_seqlens, max_seqlen)
+
+
+def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KV4Cache,
+                     extension: dict) -> torch.Tensor:
+    """Appends the new tokens' keys and values to one layer's 4-bit cache and
+    attends to the sequences so far (cti_kv4_append, cti_kv4_attention).
+    ``extension``: what ``SequenceCache.extend`` returned."""
+    cu, lens, table = extension["cu_seqlens"], extension["kv_lens"], extension["page_table"]
+    ops.kv4_append(cache, k, v, cu, lens, table)
+    return ops.kv4_attention(q, cache, cu, lens, table, extension["max_seqlen"],
+                             max_kv_len=extension["max_kv_len"])
 
 
 class SequenceGroups(NamedTuple):
@@ -98,8 +113,11 @@ def plan_sequence_groups(user_offsets: torch.Tensor, row_offsets: torch.Tensor,
 class TransformerEncoder(nn.Module):
     """``TransformerEncoder`` of ``baseline/infer.py:360-411`` with the MoE
     drop-in.  ``forward(x [T, D] or [1, T, D], extension)`` where
-    ``extension`` holds ``cu_seqlens`` (int32 [N+1]) and ``max_seqlen``, and
-    optionally ``mark(name)``, called after each layer's attention block
+    ``extension`` holds ``cu_seqlens`` (int32 [N+1]) and ``max_seqlen``, or is
+    what ``SequenceCache.extend`` returned (the tokens are then the new ones of
+    sequences whose histories the cache holds: their keys and values are
+    appended in 4 bits, and they attend to all of it), and optionally
+    ``mark(name)``, called after each layer's attention block
     ("attention") and MoE block ("moe") is enqueued (the benchmark records
     CUDA events there)."""
 
@@ -152,13 +170,20 @@ class TransformerEncoder(nn.Module):
         max_len = int(extension["max_seqlen"])
         T = x.shape[0]
         H, hd = self.n_heads, self.head_dim
+        cache = extension.get("cache")
+        if cache is not None and len(cache.layers) != self.num_layers:
+            raise ValueError(f"the cache has {len(cache.layers)} layers, the encoder "
+                             f"{self.num_layers}")
         mark = extension.get("mark") or (lambda name: None)
         pending = None  # the previous layer's MoE output, not yet added
         for i in range(self.num_layers):
             x, h = self._add_norm(x, pending, self.norm1[i])
             qkv = torch.nn.functional.linear(h, *self._qkv[i]).view(T, 3, H, hd)
-            a = causal_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], cu, max_len).reshape(
-                T, self.d_model)
+            if cache is None:
+                a = causal_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], cu, max_len)
+            else:
+                a = cached_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], cache.layers[i], extension)
+            a = a.reshape(T, self.d_model)
             x, h = self._add_norm(x, self.out_proj[i](a), self.norm2[i])
             mark("attention")
             moe_out, _ = self.moe[i](h.unsqueeze(0))
@@ -257,6 +282,30 @@ class CTRModel(nn.Module):
     def predict(self, batch: dict) -> torch.Tensor:
         """CTR probabilities [T] (fp32)."""
         return self._probs(batch)
+
+    def sequence_cache(self, max_seqs: int, num_pages: int, max_tokens: int) -> SequenceCache:
+        """A cache for ``predict_cached``: up to ``max_seqs`` sequences of up to
+        ``max_tokens`` tokens, ``num_pages`` pages of 64 tokens in all."""
+        enc = self.seq_encoder
+        w = self.linear[0].weight
+        return SequenceCache(enc.num_layers, max_seqs, num_pages, enc.n_heads, enc.head_dim,
+                             max_tokens, w.dtype, w.device)
+
+    @torch.no_grad()
+    def predict_cached(self, batch: dict, cache: SequenceCache, seqs) -> torch.Tensor:
+        """CTR probabilities [T] (fp32) of new tokens alone: ``batch`` is the flat
+        layout of the new tokens, ``user_offsets`` packing those of sequence
+        ``seqs[i]`` of the cache.  Equals ``predict`` over the whole sequences, at
+        the new tokens, but for the 4 bits that keys and values are held in."""
+        uo = batch["user_offsets"].tolist()
+        if len(uo) != len(seqs) + 1:
+            raise ValueError("user_offsets must hold one more entry than seqs")
+        if uo[-1] == uo[0]:
+            return torch.empty(0, dtype=torch.float32, device=cache.device)
+        x = self.rep_encoder(batch)
+        extension = cache.extend(seqs, [b - a for a, b in zip(uo[:-1], uo[1:])])
+        h, _ = self.seq_encoder(x, extension)
+        return self.head(h, want_logits=False)[1]
 
     @torch.no_grad()
     def predict_host(self, batch: dict, chunks: int = 8,

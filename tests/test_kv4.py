@@ -148,3 +148,54 @@ def test_format_is_within_half_a_step(dtype):
     # base: e |b|; scale: 15 s (1 + e) may fall short of max - min by 15 e s
     assert (off <= 0.5 * s + e * b.abs() + 16 * e * s).all()
     assert n.min() >= 0 and n.max() <= 15
+
+
+# ---------------------------------------------------------------------------
+# SequenceCache: which sequence holds which pages (host only).
+# ---------------------------------------------------------------------------
+def _sequence_cache(pages=6, seqs=4, tokens=300):
+    import cti_b200
+
+    return cti_b200.SequenceCache(2, seqs, pages, 2, 32, tokens, device="cpu")
+
+
+def test_sequence_cache_gives_pages_as_sequences_grow():
+    c = _sequence_cache()
+    e = c.extend([2, 0], [64, 1])
+    assert e["cu_seqlens"].tolist() == [0, 64, 65] and e["kv_lens"].tolist() == [64, 1]
+    assert e["page_table"].shape == (2, 1) and e["max_seqlen"] == 64 and e["max_kv_len"] == 64
+    assert e["cache"] is c and c.free_pages == 4 and (c.length(2), c.length(0)) == (64, 1)
+    f = c.extend([0, 2, 1], [63, 1, 0])
+    assert f["kv_lens"].tolist() == [64, 65, 0] and f["cu_seqlens"].tolist() == [0, 63, 64, 64]
+    t = f["page_table"]
+    assert t.shape == (3, 2) and t[0, 0] == e["page_table"][1, 0] and t[0, 1] == -1
+    assert t[1, 0] == e["page_table"][0, 0] and t[1, 1] >= 0 and t[2].tolist() == [-1, -1]
+    used = [p for p in t.flatten().tolist() if p >= 0]
+    assert len(set(used)) == len(used) == 3 and c.free_pages == 3
+    c.release([2])
+    assert c.free_pages == 5 and c.length(2) == 0
+    assert c.extend([], [])["kv_lens"].numel() == 0
+
+
+def test_sequence_cache_refuses_and_then_changes_nothing():
+    c = _sequence_cache()
+    c.extend([0, 1], [65, 64])
+    state = (c.free_pages, [c.length(i) for i in range(4)])
+    for error, seqs, new in ((RuntimeError, [2, 3], [128, 65]), (ValueError, [0], [236]),
+                             (ValueError, [0, 0], [1, 1]), (IndexError, [4], [1]),
+                             (IndexError, [-1], [1]), (ValueError, [0, 1], [1]),
+                             (ValueError, [2], [-1])):
+        with pytest.raises(error):
+            c.extend(seqs, new)
+        assert (c.free_pages, [c.length(i) for i in range(4)]) == state
+    c.extend([2], [192])
+    assert c.free_pages == 0
+    with pytest.raises(RuntimeError):
+        c.extend([3], [1])
+    for bad in ([4], [0, 0]):
+        with pytest.raises((IndexError, ValueError)):
+            c.release(bad)
+    import cti_b200
+
+    with pytest.raises(ValueError):
+        cti_b200.SequenceCache(0, 4, 4, 2, 32, 100, device="cpu")
