@@ -67,6 +67,7 @@ template <>
 struct Type16<__nv_bfloat16> {
   static constexpr uint32_t kMagic = 0x41804180u;  // 16.0 twice; the code goes to bits 3..6
   static constexpr int kShift = 3;
+  static constexpr uint32_t kTopBits = 0xffff0000u;  // of a float, that T holds exactly
   CTI_DEVICE static float to_float(uint32_t h) { return __uint_as_float(h << 16); }
   CTI_DEVICE static float low(uint32_t w) { return __uint_as_float(w << 16); }
   CTI_DEVICE static float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
@@ -77,6 +78,7 @@ template <>
 struct Type16<__half> {
   static constexpr uint32_t kMagic = 0x4c004c00u;  // 16.0 twice; the code goes to bits 6..9
   static constexpr int kShift = 6;
+  static constexpr uint32_t kTopBits = 0xffffe000u;  // in T's normal range
   CTI_DEVICE static float to_float(uint32_t h) {
     return __half2float(__ushort_as_half((unsigned short)h));
   }

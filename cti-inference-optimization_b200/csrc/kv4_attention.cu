@@ -9,7 +9,7 @@
 // Calls with many rows per sequence go to the tensor-core tiles of
 // kv4_tiles.cu; the rest of this file is for single tokens and a few.
 //
-// A warp takes a tile of 8, 16 or 32 rows (the query heads of one KV head,
+// A warp takes a tile of 4 to 32 rows (the query heads of one KV head,
 // token by token) and a range of the sequence's pages.  One bulk copy brings a
 // page's block of the KV head (2560 G bytes) into the warp's own ring in
 // shared memory; nothing else of the cache is read.  Per page, with keys and
@@ -28,8 +28,11 @@
 //   P^T = 2^(S^T scale log2e - m), against the row's exponent offset m, which
 //     is raised (and O, l rescaled) only when a score exceeds it by 2^8.
 //   O^T += V^T P^T with V = (16 + n) s + b by one 16-bit fused multiply-add
-//     per two values; P and V are rounded to 16 bits once each, as 16-bit
-//     attention does.  P^T becomes an operand by a transposition of 8 x 8.
+//     per two values, rounded to T once.  P enters as two numbers of T, so its
+//     rounding is left out: the error is V's rounding and the output's, 1.4
+//     times that of the output's alone (1.7 with one P).  With up to 4 rows the
+//     second part takes the columns that would lie idle, else instructions of
+//     its own.  P^T becomes an operand by a transposition of 8 x 8.
 // Where a block's warps share a row tile, they join their O, m and l in
 // shared memory; where a sequence is also split over blocks, they go to the
 // workspace and a second kernel joins them.
@@ -118,14 +121,18 @@ CTI_DEVICE uint32_t k_codes(uint32_t w, int j) {
   return (j < 2 ? w : w >> 8) & (j & 1 ? 0x00f000f0u : 0x000f000fu);
 }
 
-template <typename T, int G, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
+// ROWS: of a tile, 4, 8, 16 or 32.
+template <typename T, int G, int ROWS>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
     kv4_attention_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pages, const Args a,
                          T* __restrict__ out) {
   using Y = Type16<T>;
   using M = Mma<T>;
   constexpr int D = 32 * G;
-  constexpr int ROWS = 8 * NT;
+  constexpr int NT = (ROWS + 7) / 8;  // tiles of 8 columns
+  // With 4 rows the other 4 columns are the same rows again, for the second
+  // part of P.
+  constexpr bool kDup = ROWS == 4;
   constexpr int S = slots(G);
   constexpr int W = kWarps;
   constexpr int kSlot = slot_bytes(G);
@@ -220,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     float sl[NT][2];  // of rows 2 t and 2 t + 1, for scores in units of the row's scale
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int row = row0 + 8 * n + r8;
+      const int row = row0 + 8 * n + (kDup ? r8 & 3 : r8);
       const int i = (int)a.by_group(row), h = kvh * group + row - i * group;
       uint4 v[G];
       float most_q = 0.0f;
@@ -276,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = min(row0 + 8 * n + 2 * t4 + e, row_last);
+        const int row = min(row0 + 8 * n + (kDup ? 2 * t4 & 3 : 2 * t4) + e, row_last);
         sees[n][e] = a.causal ? min(first + (int)a.by_group(row) + 1, limit) : limit;
       }
 
@@ -291,6 +298,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
       m[n][0] = m[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.0f;
     }
+
+    const uint64_t part_x = t4 < 2 ? 0 : f2_pack(1.0f, 1.0f);
+    const uint64_t part_top = t4 < 2 ? f2_pack(1.0f, 1.0f) : f2_pack(-1.0f, -1.0f);
 
     int done = 0;
     for (; done < np; ++done) {
@@ -468,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
             vw[v] = *reinterpret_cast<const uint4*>(
                 vblk + ((2 * (kk / kTiles) + v) * 32 + lane) * 16);
         }
-        uint32_t pb[NT][2];
+        uint32_t pb[NT][2], pl[NT][2];  // P^T, and what its rounding left
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float(&x)[4] = sc[n][kk];
@@ -480,8 +490,23 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
           f2_unpack(f2_add(f2_pack(l[n][0], l[n][1]),
                            f2_add(f2_pack(x[0], x[1]), f2_pack(x[2], x[3]))),
                     l[n][0], l[n][1]);
-          pb[n][0] = transpose8(Y::pack(x[0], x[1]));
-          pb[n][1] = transpose8(Y::pack(x[2], x[3]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if constexpr (kDup) {
+              // The upper bits of p in columns 0..3, the rest in 4..7.
+              const uint64_t top = f2_pack(
+                  __uint_as_float(__float_as_uint(x[2 * e]) & Y::kTopBits),
+                  __uint_as_float(__float_as_uint(x[2 * e + 1]) & Y::kTopBits));
+              float y0, y1;
+              f2_unpack(f2_fma(f2_pack(x[2 * e], x[2 * e + 1]), part_x, f2_mul(top, part_top)),
+                        y0, y1);
+              pb[n][e] = transpose8(Y::pack(y0, y1));
+            } else {
+              const uint32_t p = Y::pack(x[2 * e], x[2 * e + 1]);
+              pb[n][e] = transpose8(p);
+              pl[n][e] = transpose8(Y::pack(x[2 * e] - Y::low(p), x[2 * e + 1] - Y::high(p)));
+            }
+          }
         }
         uint2 meta[2][G];
 #pragma unroll
@@ -512,7 +537,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
                 fma2<T>(code_pair<T>(w1, 2 * j), meta[1][g].x, meta[1][g].y),
                 fma2<T>(code_pair<T>(w1, 2 * j + 1), meta[1][g].x, meta[1][g].y)};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) M::run(o[n][2 * g + j], av, pb[n][0], pb[n][1]);
+            for (int n = 0; n < NT; ++n) {
+              M::run(o[n][2 * g + j], av, pb[n][0], pb[n][1]);
+              if (!kDup) M::run(o[n][2 * g + j], av, pl[n][0], pl[n][1]);
+            }
           }
         }
       }
@@ -526,6 +554,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
     count += H * np;
 
     // ---- join and store: lane 4 r + t has dims 4 r .. + 3 of every group ----
+    if (kDup) {
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][i][e] += __shfl_xor_sync(0xffffffffu, o[0][i][e], 2);
+    }
+    const bool holds = !kDup || t4 < 2;  // rows of its own
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -539,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
       float* mine = reinterpret_cast<float*>(ring);
       static_assert((ROWS * D + 2 * ROWS) * 4 <= S * kSlot, "room for the rows");
       __syncwarp();
-      if (warp != 0) {
+      if (warp != 0 && holds) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -556,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
           }
       }
       __syncthreads();
-      if (warp == 0) {
+      if (warp == 0 && holds) {
         for (int w = 1; w < W; ++w) {
           const float* src = reinterpret_cast<const float*>(ring + (size_t)w * S * kSlot);
 #pragma unroll
@@ -583,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, NT))
         }
       }
     }
-    if (!shared || warp == 0) {
+    if ((!shared || warp == 0) && holds) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -689,7 +724,7 @@ constexpr int kTilesFrom = 97;
 // How a call is laid out over the GPU; a function of the sizes alone.
 struct Plan {
   int big;             // 128-row tiles of a block (kv4_tiles.cu), 1 or 2; 0: warps as here
-  int row_tiles;       // of 8 rows, that a warp takes: 1, 2 or 4
+  int rows;            // that a warp takes: 4, 8, 16 or 32
   bool shared;         // a block's warps share a tile's pages
   int splits, chunk;   // blocks that share them, and the pages of each
   int64_t tiles;       // row tiles of a sequence
@@ -714,10 +749,10 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
     p.chunk = (int)((pages + p.splits - 1) / p.splits);
     return p;
   }
-  p.row_tiles = rows <= 8 ? 1 : rows <= 16 || G == 4 ? 2 : 4;
-  p.tiles = (rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles);
+  p.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || G == 4 ? 16 : 32;
+  p.tiles = (rows + p.rows - 1) / p.rows;
   const double units = (double)num_seqs * kv_heads * (double)p.tiles;
-  const double room = (double)kSMs * blocks_per_sm(G, p.row_tiles) * kWarps;  // warps at once
+  const double room = (double)kSMs * blocks_per_sm(G, (p.rows + 7) / 8) * kWarps;  // warps at once
   p.splits = 1;
   p.chunk = 0;
   if (units >= room && pages <= 8) {
@@ -747,18 +782,18 @@ size_t workspace_o_bytes(const Plan& p, int64_t tokens, int heads, int head_dim)
   return p.splits > 1 ? align256((size_t)p.splits * tokens * heads * head_dim * sizeof(float)) : 0;
 }
 
-template <typename T, int G, int NT>
+template <typename T, int G, int ROWS>
 int launch(const void* q, const void* pages, const Args& a, const Plan& p, void* out,
            cudaStream_t s) {
   static uint64_t configured = 0;
-  if (ensure_smem_limit(kv4_attention_kernel<T, G, NT>, (int)smem_bytes(G), configured) !=
+  if (ensure_smem_limit(kv4_attention_kernel<T, G, ROWS>, (int)smem_bytes(G), configured) !=
       cudaSuccess)
     return CTI_ERR_CUDA;
   const int64_t units = (int64_t)a.num_seqs * a.kv_heads;
   const int per = p.shared ? 1 : kWarps;
   const dim3 grid((unsigned)((units + per - 1) / per),
                   (unsigned)(p.tiles < 65535 ? p.tiles : 65535), (unsigned)p.splits);
-  if (launch_dependent(kv4_attention_kernel<T, G, NT>, grid, dim3(kThreads), smem_bytes(G), s,
+  if (launch_dependent(kv4_attention_kernel<T, G, ROWS>, grid, dim3(kThreads), smem_bytes(G), s,
                        static_cast<const T*>(q), static_cast<const uint8_t*>(pages), a,
                        static_cast<T*>(out)) != cudaSuccess)
     return CTI_ERR_CUDA;
@@ -780,13 +815,14 @@ int launch_shape(const void* q, const void* pages, const Args& a, const Plan& p,
   int rc;
   if (p.big) {
     rc = launch_tiles(q, pages, a, dtype, 32 * G, p.big, p.tiles, p.splits, out, s);
-  } else if constexpr (G == 4) {
-    rc = p.row_tiles == 1 ? launch<T, G, 1>(q, pages, a, p, out, s)
-                          : launch<T, G, 2>(q, pages, a, p, out, s);
+  } else if (p.rows == 4) {
+    rc = launch<T, G, 4>(q, pages, a, p, out, s);
+  } else if (p.rows == 8) {
+    rc = launch<T, G, 8>(q, pages, a, p, out, s);
+  } else if (G == 4 || p.rows == 16) {
+    rc = launch<T, G, 16>(q, pages, a, p, out, s);
   } else {
-    rc = p.row_tiles == 1   ? launch<T, G, 1>(q, pages, a, p, out, s)
-         : p.row_tiles == 2 ? launch<T, G, 2>(q, pages, a, p, out, s)
-                            : launch<T, G, 4>(q, pages, a, p, out, s);
+    rc = launch<T, G, G == 4 ? 16 : 32>(q, pages, a, p, out, s);
   }
   if (rc != CTI_OK || p.splits == 1) return rc;
   return launch_join<T, G>(a, p.splits, out, s);

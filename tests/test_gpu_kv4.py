@@ -373,7 +373,10 @@ def test_strided_queries_tables_and_shared_pages(cuda_device):
     lens = torch.tensor([140, 140], dtype=torch.int32, device=dev)
     cu = torch.tensor([0, 3, 6], dtype=torch.int32, device=dev)
     twice = ops.kv4_attention(torch.cat([qkv[:3, 0]] * 2), s.cache, cu, lens, table, max_new=3)
-    assert torch.equal(twice[:3], twice[3:]) and torch.equal(twice[:3], out[:3])
+    assert torch.equal(twice[:3], twice[3:])
+    # Another bound of the new tokens may take another variant, which sums in another order: it is
+    # held to the same bound as the first call.
+    s.compare(torch.cat([twice[:3], out[3:]]))
 
 
 def test_results_repeat_and_survive_streams_and_graphs(cuda_device):
