@@ -14,10 +14,12 @@
 //          swizzled layout of the matrix operands.  Two tiles share the work.
 //   1 warp issues S = Q K^T (M 128, N 64), 1 warp O += P V with P from TMEM and
 //          V as an MN-major operand.
-// Keys are rounded to fp16 (11 bits, as the queries hold 8 or 11) after a
-// scaling by a power of two, common to a page, that is 1 unless the page's
-// magnitudes are all below 2^-3 or come near 2^15; the scores are scaled back.  P and
-// V are rounded to the tensors' type, as 16-bit attention does.  Every wait is
+// All operands are fp16, whatever T: keys and values are unpacked to 11 bits
+// after a scaling by a power of two, common to a page, that is 1 unless the
+// page's magnitudes are all below 2^-3 or come near 2^15, and P is rounded to
+// 11 bits, so that in bf16 the output's own rounding is nearly all of the
+// error.  The scores take the keys' scaling back; the values' enters P's
+// exponents (m follows score + scaling) and is taken off the sum l.  Every wait is
 // a bounded mbarrier wait; one that runs out records its site in the status
 // word and the roles unwind.
 #include <cfloat>
@@ -51,18 +53,20 @@ struct Shape {
   static constexpr uint32_t kTileCols = 128 + D;
   static_assert(TILES * kTileCols <= kTmemCols, "TMEM budget");
   static constexpr int kInfoBytes = kStages * 48;
+  static constexpr int kMetaBytes = 512 * G;  // scales and bases as fp16, by unpacking warp
   static constexpr int kBarBytes = 320;
   static constexpr size_t kSmem =
       1024 + (size_t)TILES * kQBytes + (size_t)kStages * 2 * kKBytes +
-                                  (size_t)kRaw * block_bytes(G) + kInfoBytes + kBarBytes;
+                                  (size_t)kRaw * block_bytes(G) + kInfoBytes + kMetaBytes + kBarBytes;
   static_assert(kSmem <= (TILES == 2 ? 232448 : 115000), "shared memory");
 };
 
 // What the unpacking warps tell the softmax about a page.
 struct alignas(16) PageInfo {
-  float scale;        // of its scores
+  float scale;        // of its scores: 2^(keys' exponent)
   int keys;           // 64, or 0: not a page
-  int pad[2];
+  float v_exponent;   // its values are held as v 2^-v_exponent
+  float v_down;       // 2^-v_exponent
   uint64_t nan_v[4];  // bit per key: a value that is not finite (pages that some rows see in part)
 };
 
@@ -137,7 +141,8 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
   uint8_t* sKV = smem + TILES * Z::kQBytes;  // [S] x {K, V}
   uint8_t* sRaw = sKV + (size_t)S * 2 * Z::kKBytes;  // [R] page blocks
   PageInfo* info = reinterpret_cast<PageInfo*>(sRaw + (size_t)R * block_bytes(G));
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(info + S);  // [S] (unpacking warps)
+  uint32_t* sMeta = reinterpret_cast<uint32_t*>(info + S);
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(sMeta + Z::kMetaBytes / 4);  // [S] (unpacking warps)
   uint64_t* kv_empty = kv_full + S;                           // [S] PV of every tile done
   uint64_t* q_full = kv_empty + S;                            // [TILES] (4 softmax warps)
   uint64_t* q_empty = q_full + TILES;                         // [TILES] last S done
@@ -330,7 +335,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
           }
         }
         const float factor = fmaxf(down * pi.scale, 1e-37f);  // not 0: -inf stays -inf
-        mx = fmaxf(mx, mx1) * factor;
+        mx = fmaf(fmaxf(mx, mx1), factor, pi.v_exponent);
         float corr = 1.0f;
         if (mx - m > kSlack) {
           corr = ex2_approx(m - mx);
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             }
           }
         }
-        const float noff = m == -INFINITY ? 0.0f : -m;
+        const float noff = m == -INFINITY ? 0.0f : pi.v_exponent - m;
         const uint64_t factor2 = f2_pack(factor, factor), noff2 = f2_pack(noff, noff);
         uint64_t sum_a = f2_pack(0.0f, 0.0f), sum_b = sum_a;
 #pragma unroll 1
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             if (e & 1) sum_b = f2_add(sum_b, f2_pack(p0, p1));
             else sum_a = f2_add(sum_a, f2_pack(p0, p1));
-            pk[e] = Y::pack(p0, p1);
+            pk[e] = Type16<__half>::pack(p0, p1);
           }
           tmem_st_32x32b_x16(sb + 16 * c, pk);
         }
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         if (lane == 0) mbar_arrive(&p_full[2 * i + b]);
         float s0, s1;
         f2_unpack(f2_add(sum_a, sum_b), s0, s1);
-        l += s0 + s1;
+        l = fmaf(s0 + s1, pi.v_down, l);
       }
       if (!ok) break;
       // ---- the rows ----
@@ -491,23 +496,59 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
                             mbar_wait(&kv_empty[st], (uint32_t)((g / S) & 1) ^ 1u, a.status,
                                       0x721, abort_flag));
         if (!ok) break;
-        if (keys) {
-          // The page's scaling, from a bound of its magnitudes, 31 max s + max
-          // |b| (at most 8 times the largest): every key warp finds the same.
-          const uint32_t* km = reinterpret_cast<const uint32_t*>(blk + k_meta_at(G));
-          uint32_t top_sb = 0;  // max s in the low half, max |b| in the high one
+        // The part's scales and bases: words of (s, b) of a key, or pairs of words
+        // (s of two tokens, b of both).  A bound of the page's magnitudes, 31 max
+        // s + max |b| (at most 8 times the largest), gives its scaling; all warps
+        // of the part find the same.
+        const uint32_t* raw_meta = reinterpret_cast<const uint32_t*>(
+            blk + (keys ? k_meta_at(G) : v_meta_at(G)));
+        uint32_t top2 = 0;
 #pragma unroll
-          for (int x = 0; x < 2 * G; ++x) {
-            uint32_t w = km[32 * x + lane] & 0x7fff7fffu;
-            if (!whole && (32 * x + lane) / G >= most) w = 0;
-            top_sb = max2<T>(top_sb, w);
+        for (int x = 0; x < 2 * G; ++x) {
+          const int i = 32 * x + lane;
+          uint32_t w = raw_meta[i] & 0x7fff7fffu;
+          if (!whole) {
+            if (keys ? i / G >= most : 2 * (i / (2 * G)) >= most) w = 0;
+            else if (!keys && 2 * (i / (2 * G)) + 1 >= most) w &= 0xffffu;
           }
-          const float most_k = fminf(fmaf(31.0f, Y::low(top_sb), Y::high(top_sb)), FLT_MAX);
-          const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most_k));
-          int e = 0;
-          if (top != 0 && (top < 0x3e000000u || top >= 0x47000000u))  // [2^-3, 2^15)
-            e = max(-100, min((int)(top >> 23) - 127, 100));
-          const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+          top2 = max2<T>(top2, w);
+        }
+        // Keys: s in the low half, |b| in the high one.  Values: a lane has s's
+        // (even) or b's (odd).
+        const float t0 = Y::low(top2), t1 = Y::high(top2);
+        const bool has_s = keys || (lane & 1) == 0, has_b = keys || (lane & 1) != 0;
+        const uint32_t top_s = __reduce_max_sync(
+            0xffffffffu, has_s ? __float_as_uint(keys ? t0 : fmaxf(t0, t1)) : 0u);
+        const uint32_t top_b = __reduce_max_sync(
+            0xffffffffu, has_b ? __float_as_uint(keys ? t1 : fmaxf(t0, t1)) : 0u);
+        const float top = fminf(fmaf(31.0f, __uint_as_float(top_s), __uint_as_float(top_b)), FLT_MAX);
+        int e = 0;
+        if (top > 0.0f && (top < 0.125f || top >= 32768.0f))
+          e = max(-100, min((int)(__float_as_uint(top) >> 23) - 127, 100));
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        // This warp's own, scaled and as fp16.
+        uint32_t* meta = sMeta + (warp - Z::kSoftmaxWarps) * (32 * kVecs);
+        uint64_t nan_bits = 0;
+#pragma unroll
+        for (int x = 0; x < kVecs; ++x) {
+          const int i = 32 * (part * kVecs + x) + lane;
+          uint32_t w = raw_meta[i];
+          if (!keys && !whole) {
+            // Behind the last key: zero.  Not finite: zero, and the softmax is told.
+            const int tau = 2 * (i / (2 * G));
+            constexpr uint32_t inf = Inf16<T>::kBits;
+            uint32_t n = ((w & inf) == inf ? 1u : 0u) | ((w >> 16 & inf) == inf ? 2u : 0u);
+            n |= __shfl_xor_sync(0xffffffffu, n, 1);  // the other of s and b
+            n &= (tau < most ? 1u : 0u) | (tau + 1 < most ? 2u : 0u);
+            w &= ((n & 1) || tau >= most ? 0u : 0xffffu) |
+                 ((n & 2) || tau + 1 >= most ? 0u : 0xffff0000u);
+            nan_bits |= (uint64_t)n << tau;
+          }
+          meta[32 * x + lane] =
+              Type16<__half>::pack(Y::low(w) * down, Y::high(w) * down);
+        }
+        __syncwarp();
+        if (keys) {
           if (part == 0 && lane == 0) {
             info[st].scale = __uint_as_float((uint32_t)(127 + e) << 23);
             info[st].keys = is_page ? kPage : 0;
@@ -517,22 +558,21 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             const int v = part * kVecs + x, nt0 = 4 * v / G;
             const uint4 w4 = *reinterpret_cast<const uint4*>(blk + (v * 32 + lane) * 16);
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-            const uint32_t* mv = km + (8 * nt0 + hi) * G;
-            uint32_t meta[4];
+            const uint32_t* mv = meta + 32 * x + hi * G;
+            uint32_t sb[4];
             if constexpr (G == 4) {
               const uint4 m4 = *reinterpret_cast<const uint4*>(mv);
-              meta[0] = m4.x, meta[1] = m4.y, meta[2] = m4.z, meta[3] = m4.w;
+              sb[0] = m4.x, sb[1] = m4.y, sb[2] = m4.z, sb[3] = m4.w;
             } else {
 #pragma unroll
-              for (int y = 0; y < 4; ++y) meta[y] = mv[8 * (y / G) * G + y % G];
+              for (int y = 0; y < 4; ++y) sb[y] = mv[8 * (y / G) * G + y % G];
             }
             uint8_t* to = dst + nt0 * 8 * kRow;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const int nt = y / G, gr = y % G;  // nt: octets past nt0
-              const uint32_t sb =
-                  Type16<__half>::pack(Y::low(meta[y]) * down, Y::high(meta[y]) * down);
-              const uint32_t s2 = __byte_perm(sb, sb, 0x1010), b2 = __byte_perm(sb, sb, 0x3232);
+              const uint32_t s2 = __byte_perm(sb[y], sb[y], 0x1010);
+              const uint32_t b2 = __byte_perm(sb[y], sb[y], 0x3232);
               uint32_t o[4];
 #pragma unroll
               for (int p = 0; p < 4; ++p)
@@ -543,7 +583,6 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             }
           }
         } else {
-          uint64_t nan_bits = 0;
           uint8_t* vt = dst + Z::kKBytes;
 #pragma unroll 1
           for (int x = 0; x < kVecs; ++x) {
@@ -551,43 +590,28 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             const uint4 w4 =
                 *reinterpret_cast<const uint4*>(blk + v_codes_at(G) + (v * 32 + lane) * 16);
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-            const uint2* mv =
-                reinterpret_cast<const uint2*>(blk + v_meta_at(G)) + (4 * nt0 + lo) * G;
-            uint2 metas[4];
+            const uint2* mv = reinterpret_cast<const uint2*>(meta + 32 * x) + lo * G;
+            uint2 sb[4];
             if constexpr (G == 1) {
 #pragma unroll
-              for (int y = 0; y < 4; ++y) metas[y] = mv[4 * y];
+              for (int y = 0; y < 4; ++y) sb[y] = mv[4 * y];
             } else {
 #pragma unroll
               for (int y = 0; y < 4; y += 2) {
                 const uint4 m4 =
                     *reinterpret_cast<const uint4*>(mv + 4 * (y / G) * G + y % G);
-                metas[y] = make_uint2(m4.x, m4.y);
-                metas[y + 1] = make_uint2(m4.z, m4.w);
+                sb[y] = make_uint2(m4.x, m4.y);
+                sb[y + 1] = make_uint2(m4.z, m4.w);
               }
             }
             uint8_t* to = vt + nt0 * 8 * kRow;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const int nt = y / G, gr = y % G;
-              uint2 meta = metas[y];
-              if (!whole) {
-                // Behind the last key: zero.  Not finite: zero, and the softmax is told.
-                const int tau = 8 * (nt0 + nt) + 2 * lo;
-                constexpr uint32_t inf = Inf16<T>::kBits;
-                const bool n0 =
-                    tau < most && ((meta.x & inf) == inf || (meta.y & inf) == inf);
-                const bool n1 = tau + 1 < most &&
-                                ((meta.x >> 16 & inf) == inf || (meta.y >> 16 & inf) == inf);
-                const uint32_t keep = (n0 || tau >= most ? 0u : 0xffffu) |
-                                      (n1 || tau + 1 >= most ? 0u : 0xffff0000u);
-                meta.x &= keep;
-                meta.y &= keep;
-                nan_bits |= (uint64_t)(n0 ? 1 : 0) << tau | (uint64_t)(n1 ? 2 : 0) << tau;
-              }
               uint32_t o[4];
 #pragma unroll
-              for (int p = 0; p < 4; ++p) o[p] = fma2<T>(code_pair<T>(w[y], p), meta.x, meta.y);
+              for (int p = 0; p < 4; ++p)
+                o[p] = fma2<__half>(code_pair<__half>(w[y], p), sb[y].x, sb[y].y);
               uint8_t* row = to + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow;
               *reinterpret_cast<uint2*>(row + (at_v0 ^ 64 * (gr & 1))) =
                   make_uint2(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410));
@@ -603,6 +627,10 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
           if (lane == 0) {
             info[st].nan_v[part] = nan_bits;
             if (kEach == 2) info[st].nan_v[part + 2] = 0;
+            if (part == 0) {
+              info[st].v_exponent = (float)e;
+              info[st].v_down = down;
+            }
           }
         }
         fence_proxy_async_smem();
@@ -664,9 +692,8 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
   } else {
     // ---------------- PV issuer ----------------
     if (lane == 0) {
-      constexpr uint32_t type = sizeof(T) == 2 && Type16<T>::kShift == 3 ? 1u : 0u;  // bf16, fp16
-      constexpr uint32_t id_pv = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) |
-                                 ((D >> 3) << 17) | ((kTile >> 4) << 24);  // V MN-major
+      // fp16 operands, fp32 sums; V MN-major
+      constexpr uint32_t id_pv = (1u << 4) | (1u << 16) | ((D >> 3) << 17) | ((kTile >> 4) << 24);
       const uint32_t kv_addr = smem_u32(sKV);
       int it = 0, g = 0;
       bool ok = true, any = false;

@@ -39,7 +39,9 @@ def attention(q, k, v, new, total, causal, scale):
 
     With e = eps / 2 of the type, u = 2^-24 of fp32, A = sum p |v|:
       p's and v's rounding: 2 e A; the output's: e |out|;
-      p below the type's normals: half its smallest step for each key, over a sum l >= 1;
+      p below the type's normals, or those of fp16 (the type may be bf16 and p, v held in fp16):
+      half the smallest step, 2^-25, for each key, over a sum l >= 1; v below them, after a common
+      factor that is not 1 only where some are large: 2^-25 max(1, max |v|);
       a score is off by at most d: 2 d A in the weights and their sum (first order; d << 1).
     d, for a score q . k with k = (16 + n) s + b:
       - q (16 + n) s and q b may be summed apart, in fp32, over up to head_dim + 8 terms.  In a
@@ -52,7 +54,7 @@ def attention(q, k, v, new, total, causal, scale):
         2^-20 max(1, max |k|) sum |q|."""
     dtype = q.dtype
     e, u = rounding(dtype), 2.0 ** -24
-    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    tiny = 2.0 ** -25
     H, D = q.shape[1], q.shape[2]
     group = H // k.shape[1]
     out = torch.zeros(q.shape, dtype=torch.float64)
@@ -88,7 +90,7 @@ def attention(q, k, v, new, total, causal, scale):
         few = torch.einsum("hnl,lhd->nhd", seen.double(), vz.abs())
         out[n0:n0 + n] = o
         tol[n0:n0 + n] = (e * o.abs() + 2 * e * A + 2 * dmax.T[..., None] * A + 2.0 ** -20 * A +
-                          tiny * few + tiny) * 1.01
+                          tiny * few + tiny * max(1.0, float(vz.abs().max()) if L else 0.0)) * 1.01
         n0, t0 = n0 + n, t0 + L
     return out, tol
 
