@@ -502,26 +502,35 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         // of the part find the same.
         const uint32_t* raw_meta = reinterpret_cast<const uint32_t*>(
             blk + (keys ? k_meta_at(G) : v_meta_at(G)));
-        uint32_t top2 = 0;
+        uint32_t most_s = 0, most_b = 0;  // of keys: both in most_s
 #pragma unroll
-        for (int x = 0; x < 2 * G; ++x) {
-          const int i = 32 * x + lane;
-          uint32_t w = raw_meta[i] & 0x7fff7fffu;
-          if (!whole) {
-            if (keys ? i / G >= most : 2 * (i / (2 * G)) >= most) w = 0;
-            else if (!keys && 2 * (i / (2 * G)) + 1 >= most) w &= 0xffffu;
+        for (int x = 0; x < (G + 1) / 2; ++x) {
+          constexpr int kWords = G == 1 ? 2 : 4;  // side by side, of a lane
+          const int i = (32 * x + lane) * kWords;
+          uint32_t w[4] = {0, 0, 0, 0};
+          if constexpr (G == 1) {
+            const uint2 m2 = *reinterpret_cast<const uint2*>(raw_meta + i);
+            w[0] = m2.x, w[1] = m2.y;
+          } else {
+            const uint4 m4 = *reinterpret_cast<const uint4*>(raw_meta + i);
+            w[0] = m4.x, w[1] = m4.y, w[2] = m4.z, w[3] = m4.w;
           }
-          top2 = max2<T>(top2, w);
+#pragma unroll
+          for (int y = 0; y < kWords; ++y) {
+            w[y] &= 0x7fff7fffu;
+            if (!whole) {
+              const int tau = keys ? (i + y) / G : (i + y) / (2 * G) * 2;
+              if (tau >= most) w[y] = 0;
+              else if (!keys && tau + 1 >= most) w[y] &= 0xffffu;
+            }
+            if (keys || (y & 1) == 0) most_s = max2<T>(most_s, w[y]);
+            else most_b = max2<T>(most_b, w[y]);
+          }
         }
-        // Keys: s in the low half, |b| in the high one.  Values: a lane has s's
-        // (even) or b's (odd).
-        const float t0 = Y::low(top2), t1 = Y::high(top2);
-        const bool has_s = keys || (lane & 1) == 0, has_b = keys || (lane & 1) != 0;
-        const uint32_t top_s = __reduce_max_sync(
-            0xffffffffu, has_s ? __float_as_uint(keys ? t0 : fmaxf(t0, t1)) : 0u);
-        const uint32_t top_b = __reduce_max_sync(
-            0xffffffffu, has_b ? __float_as_uint(keys ? t1 : fmaxf(t0, t1)) : 0u);
-        const float top = fminf(fmaf(31.0f, __uint_as_float(top_s), __uint_as_float(top_b)), FLT_MAX);
+        const float top_s = keys ? Y::low(most_s) : fmaxf(Y::low(most_s), Y::high(most_s));
+        const float top_b = keys ? Y::high(most_s) : fmaxf(Y::low(most_b), Y::high(most_b));
+        const float top = __uint_as_float(__reduce_max_sync(
+            0xffffffffu, __float_as_uint(fminf(fmaf(31.0f, top_s, top_b), FLT_MAX))));
         int e = 0;
         if (top > 0.0f && (top < 0.125f || top >= 32768.0f))
           e = max(-100, min((int)(__float_as_uint(top) >> 23) - 127, 100));
