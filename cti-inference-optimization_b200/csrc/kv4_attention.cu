@@ -36,6 +36,13 @@
 // Where a block's warps share a row tile, they join their O, m and l in
 // shared memory; where a sequence is also split over blocks, they go to the
 // workspace and a second kernel joins them.
+//
+// Bound by instructions, the logic pipe's first (a shift or a three-input logic
+// operation takes two cycles of a quarter of an SM): about 1,050 a page and KV
+// head for head_dim 128, 400 for 32, and 490 for a warp's queries and rows.
+// One token, 32 heads on 8 KV heads of 128, 131,071 keys: 43.8 us, 59 % of the
+// copy bandwidth.  2,048 sequences of 136 keys on average, 8 heads of 32: 43.6
+// us, 32 %.
 #include <cfloat>
 
 #include "kv4_attention.cuh"
@@ -867,7 +874,7 @@ extern "C" int cti_kv4_attention(const void* q, int64_t q_stride, int dtype,
     return CTI_ERR_INVALID_ARG;
   if (dtype != CTI_DTYPE_BF16 && dtype != CTI_DTYPE_F16) return CTI_ERR_UNSUPPORTED;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128) return CTI_ERR_UNSUPPORTED;
-  if (tokens > INT32_MAX - 256 || heads > 65535 || tokens * heads > INT32_MAX - 64 ||
+  if (tokens > INT32_MAX - 256 || heads > 65535 || tokens * heads > INT32_MAX - 512 ||
       (int64_t)num_seqs * kv_heads > INT32_MAX || table_cols > INT32_MAX / kv4::kPage)
     return CTI_ERR_UNSUPPORTED;
   if (num_seqs == 0 || tokens == 0) return CTI_OK;

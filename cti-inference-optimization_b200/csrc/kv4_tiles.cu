@@ -16,12 +16,18 @@
 //          V as an MN-major operand.
 // All operands are fp16, whatever T: keys and values are unpacked to 11 bits
 // after a scaling by a power of two, common to a page, that is 1 unless the
-// page's magnitudes are all below 2^-3 or come near 2^15, and P is rounded to
+// page's magnitudes are all below 2^-3 or come near 2^15 (then their bound goes
+// to 2^14, so that small values beside large ones keep their bits), and P is rounded to
 // 11 bits, so that in bf16 the output's own rounding is nearly all of the
 // error.  The scores take the keys' scaling back; the values' enters P's
-// exponents (m follows score + scaling) and is taken off the sum l.  Every wait is
-// a bounded mbarrier wait; one that runs out records its site in the status
-// word and the roles unwind.
+// exponents (m follows score + scaling) and is taken off the sum l; beside
+// values 2^k above 2^15 with a weight of note, those of other pages keep k bits
+// fewer than 24 in P.  Every wait is a bounded mbarrier wait; one that runs out
+// records its site in the status word and the roles unwind.
+//
+// Bound by the unpacking for head_dim 128 (without it 554 us become 400 for
+// 5,500 tokens of 16 heads over 5,700 keys each), and by the chain S, softmax,
+// P V of a page for 32 and 64: about 1.3 us a page.
 #include <cfloat>
 #include <climits>
 
@@ -182,11 +188,13 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
     *abort_flag = 0;
     fence_barrier_init();
   }
+  // Everything read below may come from the kernel before; tensor memory too may
+  // still be that kernel's, which must not wait for ours.
+  grid_dependency_wait();
   if (warp == Z::kSoftmaxWarps + Z::kUnpackWarps) {
     tmem_alloc(tmem_slot, Z::kTmemCols);
     tmem_relinquish();
   }
-  grid_dependency_wait();  // everything read below may come from the kernel before
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -533,7 +541,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             0xffffffffu, __float_as_uint(fminf(fmaf(31.0f, top_s, top_b), FLT_MAX))));
         int e = 0;
         if (top > 0.0f && (top < 0.125f || top >= 32768.0f))
-          e = max(-100, min((int)(__float_as_uint(top) >> 23) - 127, 100));
+          e = max(-100, min((int)(__float_as_uint(top) >> 23) - 127 - 14, 100));  // to 2^14
         const float down = __uint_as_float((uint32_t)(127 - e) << 23);
         // This warp's own, scaled and as fp16.
         uint32_t* meta = sMeta + (warp - Z::kSoftmaxWarps) * (32 * kVecs);

@@ -363,8 +363,8 @@ int cti_ctr_head(const void* h_bf16, const void* W1_bf16, const float* b1, const
  *   s = T((max - min) / 15),  b = T(min - 16 s),
  *   n = clamp(round((x - b) / s) - 16, 0, 15)   (ties to even; 0 where s = 0)
  * and stand for (16 + n) s + b.  A group with a value that is not finite (or
- * whose b is not: magnitudes above 20,000 in fp16) stands for NaN as a whole.
- * head_dim 32, 64 or 128 (CTI_ERR_UNSUPPORTED otherwise).
+ * whose b is not: magnitudes above 20,000 in fp16, 1e38 in bf16) stands for
+ * NaN as a whole.  head_dim 32, 64 or 128 (CTI_ERR_UNSUPPORTED otherwise).
  *
  * pages: num_pages pages of cti_kv4_page_bytes(kv_heads, head_dim) bytes,
  * 16-byte aligned; a page holds CTI_KV4_PAGE_TOKENS tokens of every KV head.
@@ -373,7 +373,9 @@ int cti_ctr_head(const void* h_bf16, const void* W1_bf16, const float* b1, const
  * cu_seqlens int32 [num_seqs+1] (non-decreasing): the packed tokens of
  * sequence s are cu[s] .. cu[s+1] - 1; they are the LAST ones of its
  * kv_lens[s] (int32) tokens, so packed token t has position
- * kv_lens[s] - cu[s+1] + t.  Sequences may share pages that no call writes.
+ * kv_lens[s] - cu[s+1] + t.  Sequences may share pages that no call writes; a
+ * call must not write one slot twice, nor a slot that another call in flight
+ * uses.
  * A position or page outside its buffer raises CTI_ERR_BOUNDS in `status`
  * (detail: the sequence) and is left out: not written, read as zeros, or not
  * attended to.  Rows of no sequence are left as they were.
@@ -405,7 +407,10 @@ int cti_kv4_read(const void* pages, int64_t num_pages, int dtype, const int32_t*
  * head h reads KV head h / (heads / kv_heads).  q [tokens][heads][head_dim]
  * with a token stride as above; out the same, contiguous.  A row that sees
  * no key is zero.  max_new and max_kv_len: the caller's bounds of the new
- * tokens and of kv_lens; the work is split by them, results hold for any.
+ * tokens and of kv_lens; the work is split by them, results hold for any (in
+ * another order of summation).  A value that is not finite reaches only the
+ * rows that see its token, where it may spoil the whole row.  tokens * heads
+ * and num_seqs * kv_heads below 2^31 - 512 (CTI_ERR_UNSUPPORTED otherwise).
  * workspace: cti_kv4_attention_workspace_bytes(...) bytes, 256-byte aligned
  * (may be NULL where that is 0); contents do not outlive the call. */
 size_t cti_kv4_attention_workspace_bytes(int num_seqs, int64_t tokens, int max_new,

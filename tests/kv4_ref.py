@@ -40,23 +40,26 @@ def attention(q, k, v, new, total, causal, scale):
     With e = eps / 2 of the type, u = 2^-24 of fp32, A = sum p |v|:
       p's and v's rounding: 2 e A; the output's: e |out|;
       p below the type's normals, or those of fp16 (the type may be bf16 and p, v held in fp16):
-      half the smallest step, 2^-25, for each key, over a sum l >= 1; v below them, after a common
-      factor that is not 1 only where some are large: 2^-25 max(1, max |v|);
-      a score is off by at most d: 2 d A in the weights and their sum (first order; d << 1).
+      half the smallest step, 2^-25, for each key, over a sum l >= 1;
+      v's scale below fp16's normals: 31 2^-25 < 2^-20, or, after a common factor that takes a bound
+      of 8 max |v| to 2^14 at least, 31 2^-25 8 2^-14 max |v| < 2^-31 max |v|;
+      a score is off by at most d, so a weight by a factor of exp(+-2 d) with its sum: expm1(2 d) A.
     d, for a score q . k with k = (16 + n) s + b:
       - q (16 + n) s and q b may be summed apart, in fp32, over up to head_dim + 8 terms.  In a
         group with largest magnitude kmax, s <= 2 kmax / 15 and |b| <= kmax + 16 s, so 31 s + |b| <
         8 kmax: below 16 sum |q| kmax (head_dim + 8) u;
       - the sum of q over a group may be split into two numbers of the type, short by e^2 of
         itself, twice (for s and b): below 2 e^2 16 sum |q| kmax;
-      - keys rounded to 11 bits: 2^-12 sum |q| |k|; their scales may lie below fp16's normals,
-        31 2^-25 < 2^-20 for each, times a common factor where the largest key is above 1:
-        2^-20 max(1, max |k|) sum |q|."""
+      - keys rounded to 11 bits: 2^-12 sum |q| |k|, and as for v 2^-20 max(1, 2^-11 max |k|) sum |q|."""
     dtype = q.dtype
     e, u = rounding(dtype), 2.0 ** -24
     tiny = 2.0 ** -25
     H, D = q.shape[1], q.shape[2]
     group = H // k.shape[1]
+
+    def most(x):
+        return float(torch.nan_to_num(x).abs().max()) if x.numel() else 0.0
+
     out = torch.zeros(q.shape, dtype=torch.float64)
     tol = torch.zeros(q.shape, dtype=torch.float64)
     n0 = t0 = 0
@@ -70,8 +73,8 @@ def attention(q, k, v, new, total, causal, scale):
         d = torch.einsum("nhd,lhd->hnl", qs.abs(), kmax) * abs(scale) * 16 * (
             (D + 8) * u + 2 * e * e)
         d = d + abs(scale) * (2.0 ** -12 * torch.einsum("nhd,lhd->hnl", qs.abs(), ks.abs()) +
-                              2.0 ** -20 * max(1.0, float(torch.nan_to_num(ks).abs().max()) if L
-                                               else 0.0) * qs.abs().sum(-1).T[:, :, None])
+                              2.0 ** -20 * max(1.0, 2.0 ** -11 * most(ks)) *
+                              qs.abs().sum(-1).T[:, :, None])
         if causal:
             pos = L - n + torch.arange(n)
             s = s.masked_fill(torch.arange(L)[None, :] > pos[:, None], float("-inf"))
@@ -89,8 +92,8 @@ def attention(q, k, v, new, total, causal, scale):
         dmax = torch.where(seen, torch.nan_to_num(d), 0.0).amax(-1) if L else torch.zeros(H, n)
         few = torch.einsum("hnl,lhd->nhd", seen.double(), vz.abs())
         out[n0:n0 + n] = o
-        tol[n0:n0 + n] = (e * o.abs() + 2 * e * A + 2 * dmax.T[..., None] * A + 2.0 ** -20 * A +
-                          tiny * few + tiny * max(1.0, float(vz.abs().max()) if L else 0.0)) * 1.01
+        tol[n0:n0 + n] = (e * o.abs() + 2 * e * A + torch.expm1(2 * dmax.T[..., None]) * A + 2.0 ** -20 * A +
+                          tiny * few + 2.0 ** -20 * max(1.0, 2.0 ** -11 * most(vs))) * 1.01
         n0, t0 = n0 + n, t0 + L
     return out, tol
 

@@ -255,6 +255,34 @@ def test_long_sequences(cuda_device, H, Hkv, D, new, total):
     s.check(causal=False)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D,n", [(2, 2, 32, 100), (4, 2, 64, 64), (4, 1, 128, 25),
+                                       (8, 1, 32, 16), (1, 1, 128, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_about_a_hundred_rows(cuda_device, dtype, H, Hkv, D, n, causal):
+    """97 to 128 query rows of a KV head: one 128-row tile, of one page range or several."""
+    s = Setup(cuda_device, [n, 1, n - 3], [n + 40, 1, 200], H, Hkv, D, dtype, seed=n)
+    s.check(causal=causal, max_new=n)
+    s = Setup(cuda_device, [n], [2500], H, Hkv, D, dtype, seed=n + 1)
+    s.check(causal=causal, max_new=n)
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(2, 2, 32), (4, 2, 64), (2, 1, 128)])
+@pytest.mark.parametrize("n", [1, 12, 60, 150])
+def test_magnitudes_far_from_one(cuda_device, H, Hkv, D, n):
+    """Keys and values of 1e-5 to 1e5, other ones in every page: what a page is scaled by must not
+    show.  The scores' scale keeps the largest of them within a few hundred."""
+    total = 400
+    k, v = (_values(total, Hkv, D, torch.bfloat16, i).float() for i in (1, 2))
+    size = torch.tensor([1e5, 1e-3, 1.0, 3e4, 1e-5, 40.0, 1e-4])[torch.arange(total) // 64]
+    k = (k * size[:, None, None]).bfloat16()
+    v = (v * size.flip(0)[:, None, None]).bfloat16()
+    s = Setup(cuda_device, [n], [total], H, Hkv, D, torch.bfloat16, k=k, v=v)
+    s.check(scale=1e-4, max_new=n)
+    s.check(scale=-1e-4, causal=False)
+    s.check(scale=4e-6, max_new=n)
+
+
 def test_scale_and_large_scores(cuda_device):
     """Scores of hundreds: the running maximum keeps every exponential in range.  The scale enters
     the bound of a score's error."""
@@ -451,6 +479,35 @@ def test_a_step_appends_and_attends(cuda_device):
         want, tol = ref.attention(q[rows], ref.held(k[held]), ref.held(v[held]), n, done, True,
                                   D ** -0.5)
         assert ((out.double().cpu() - want).abs() <= tol).all()
+
+
+def test_pages_past_four_gigabytes(cuda_device):
+    """A cache whose bytes need more than 32 bits: the last pages hold what the first ones do."""
+    import cti_b200
+    from cti_b200 import _lib, ops
+
+    dev, H, D = cuda_device, 8, 128
+    pages = 2 ** 32 // _lib.lib.cti_kv4_page_bytes(H, D) + 60
+    c = cti_b200.KV4Cache(pages, H, D, device=dev)
+    x = _values(260, H, D, torch.bfloat16, 0).to(dev)
+    lens = torch.tensor([130, 130], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 130, 260], dtype=torch.int32, device=dev)
+    table = torch.tensor([[0, 1, 2], [pages - 1, pages - 3, pages - 2]], dtype=torch.int32,
+                         device=dev)
+    x[130:] = x[:130]
+    ops.kv4_append(c, x, x, cu, lens, table)
+    k, v = ops.kv4_read(c, cu, lens, table, 260)
+    assert torch.equal(k[:130], k[130:]) and torch.equal(v, k)
+    _check_read(k[130:], x[130:].cpu())
+    for n in (1, 130):
+        q = x[:n].repeat(2, 1, 1)
+        out = ops.kv4_attention(q, c, torch.tensor([0, n, 2 * n], dtype=torch.int32, device=dev),
+                                lens, table, n)
+        _lib.raise_on_status(dev)
+        assert torch.equal(out[:n], out[n:])
+        want, tol = ref.attention(q[:n].cpu(), ref.held(x[:130].cpu()), ref.held(x[:130].cpu()),
+                                  [n], [130], True, D ** -0.5)
+        assert ((out[:n].double().cpu() - want).abs() <= tol).all()
 
 
 def test_wrappers_refuse_wrong_tensors(cuda_device):
