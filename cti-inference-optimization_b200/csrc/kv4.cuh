@@ -117,18 +117,8 @@ CTI_DEVICE uint32_t code_pair(uint32_t w, int j) {
   return (x & (0x000f000fu << s)) | Type16<T>::kMagic;
 }
 
-// Where a packed token's key and value live.
-struct Place {
-  int64_t page;  // -1: nowhere (an index outside its buffer; the status word says so)
-  int slot;
-};
-
-// Largest s in [0, n) with cu[s] <= t (cu[0] <= t < cu[n]).  Tried first: the
-// sequence that t lies in if all are equally long, at once right for batches
-// of single tokens.
-CTI_DEVICE int sequence_of(const int32_t* __restrict__ cu, int n, int tokens, int t) {
-  const int guess = (int)((int64_t)t * n / tokens);
-  if (__ldg(cu + guess) <= t && t < __ldg(cu + guess + 1)) return guess;
+// Largest s in [0, n) with cu[s] <= t (cu[0] <= t < cu[n]).
+CTI_DEVICE int sequence_of(const int32_t* __restrict__ cu, int n, int t) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -147,18 +137,6 @@ CTI_DEVICE int64_t page_of(const int32_t* __restrict__ table, int64_t table_stri
   }
   raise_status(status, CTI_ERR_BOUNDS, s);
   return -1;
-}
-
-// The place of packed new token t: the last cu[s+1] - cu[s] of sequence s's
-// kv_lens[s] tokens are the new ones.
-CTI_DEVICE Place place_of(const int32_t* __restrict__ cu, const int32_t* __restrict__ kv_lens,
-                          const int32_t* __restrict__ table, int64_t table_stride, int table_cols,
-                          int num_seqs, int tokens, int64_t num_pages, int t,
-                          int32_t* status) {
-  const int s = sequence_of(cu, num_seqs, tokens, t);
-  const int64_t p = (int64_t)__ldg(kv_lens + s) - __ldg(cu + s + 1) + t;
-  return {page_of(table, table_stride, table_cols, num_pages, s, p, status),
-          (int)(p & (kPage - 1))};
 }
 
 }  // namespace kv4

@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
       const uint32_t slot = (count + h) % S;
       if (lane == 0) {
         mbar_arrive_expect_tx(&full[slot], kSlot);
-        bulk_load(ring + slot * kSlot, base + max(id, 0) * page_stride + (h & (H - 1)) * kSlot, kSlot,
-                  &full[slot]);
+        bulk_load(ring + slot * kSlot, base + max(id, 0) * page_stride + (h & (H - 1)) * kSlot,
+                  kSlot, &full[slot]);
       }
     };
     auto arrived = [&](int h) {

@@ -1,18 +1,19 @@
 // Writing tokens into the 4-bit key/value cache and reading them back
 // (format: kv4.cuh).
 //
-// Two ways, by the tokens that a sequence has in the call:
-//   runs    a block finds the runs (tokens side by side in one page) that start
-//           among 64 or 128 packed tokens; a warp takes a run's keys or values
-//           in one head, with lanes laid out as the page's, so that it moves
-//           whole sectors of codes.
-//   tokens  a block takes 8 packed tokens, every thread 16 dims of a token's
-//           key and value.  For calls with a few tokens per sequence, whose
-//           runs would leave most lanes of a warp idle.
+// A block takes packed tokens side by side, 32 / G of them (G = head_dim / 32)
+// or a multiple.  In a page, 16 bytes hold a word each of G groups in 4 / G
+// octets of tokens.  A warp's lanes take those four words; with them a token's
+// two halves of the group (append; 16 dims to a lane) or four quarters (read);
+// and 4 or 2 tokens side by side, whose values share sectors.  So whole sectors
+// move where tokens follow each other in a page, and nothing is lost where each is
+// of its own sequence.  (With a token's groups side by side in a warp instead,
+// sectors are written in pieces: 38 us for 25 to append 24,576 tokens of 8 heads
+// of 64, in L2.)
 // Either way moves 4 + 1.25 bytes per pair of a key's and a value's element.
-// Measured, 278,000 tokens of 8 heads of 32: 123 us to append (bound by
-// instructions, 17 for 32 values of a warp; 47 % of the copy bandwidth) and 75
-// us to read back (latency; 76 %).
+// Measured, 278,000 tokens of 8 heads of 32: 112 us to append (bound by
+// instructions, 17 for 32 values of a warp; 51 % of the copy bandwidth) and 79
+// us to read back (instructions and latency; 73 %).
 #include <cfloat>
 
 #include "kv4.cuh"
@@ -24,11 +25,8 @@ using namespace kv4;
 
 constexpr int kSMs = 148;
 constexpr int kThreads = 256;
-constexpr int kTokens = 8;      // packed tokens of a block, by tokens
-constexpr int kRunTokens = 128;  // and by runs, at most
-constexpr int64_t kMaxStride = (int64_t)1 << 24;
-// A sequence's tokens in a call, on average, from which runs are used.
-constexpr int kRunsFrom = 8;
+constexpr int kTokens = 128;  // packed tokens of a block, at most
+constexpr int64_t kMaxStride = ((int64_t)1 << 31) / kTokens;
 
 struct Args {
   const int32_t* cu;
@@ -211,8 +209,6 @@ CTI_DEVICE void quantise(const uint4 (&raw)[2], uint32_t (&word)[2], uint32_t& s
   }
 }
 
-CTI_DEVICE uint32_t twice(uint32_t h) { return __byte_perm(h, h, 0x1010); }
-
 // What a K word stands for in T.
 template <typename T>
 CTI_DEVICE uint4 k_values(uint32_t w, uint32_t meta) {
@@ -230,40 +226,115 @@ CTI_DEVICE void v_values(uint32_t w, uint32_t s, uint32_t b, uint2& even, uint2&
   odd = make_uint2(__byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
 }
 
-// Place of packed token t, page -2 where it is of no sequence.
-CTI_DEVICE Place find_place(const Args& a, int t) {
-  Place at = {-2, 0};
-  if (t < a.tokens && t >= __ldg(a.cu) && t < __ldg(a.cu + a.num_seqs))
-    at = place_of(a.cu, a.kv_lens, a.table, a.table_stride, a.table_cols, a.num_seqs, a.tokens,
-                  a.num_pages, t, a.status);
-  return at;
+// Where a packed token's key and value live.
+struct Place {
+  int64_t page;  // its offset in bytes; -1: nowhere (an index outside its buffer; the
+                 // status word says so); -2: a token of no sequence
+  int slot;
+};
+
+// The places of the block's a.tile packed tokens from t0 on.  All threads of the
+// block.
+template <int G>
+CTI_DEVICE void find_places(const Args& a, int t0, Place (&places)[kTokens]) {
+  static_assert(kTokens <= kThreads, "a thread per token");
+  const int lane = lane_id(), first = t0 + warp_id() * 32, t = first + lane;
+  if (warp_id() * 32 < a.tile) {
+    Place at = {-2, 0};
+    const bool live = warp_id() * 32 + lane < a.tile && t < a.tokens && t >= __ldg(a.cu) &&
+                      t < __ldg(a.cu + a.num_seqs);
+    // As many tokens in each sequence: no search.
+    int s = live ? (int)((int64_t)t * a.num_seqs / a.tokens) : 0;
+    if (!__all_sync(0xffffffffu, !live || (__ldg(a.cu + s) <= t && t < __ldg(a.cu + s + 1)))) {
+      // The sequence of the warp's first token, 32 borders at a time; the others'
+      // are found among the next 32.
+      int lo = 0, hi = a.num_seqs;  // cu[lo] <= first (or lo = 0), and first < cu[hi]
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, border = lo + (lane + 1) * step;
+        const uint32_t le =
+            __ballot_sync(0xffffffffu, border < hi && __ldg(a.cu + border) <= first);
+        const int last = __popc(le);
+        hi = min(hi, lo + (last + 1) * step);
+        lo += last * step;
+      }
+      const int end = __ldg(a.cu + min(lo + 1 + lane, a.num_seqs));
+      int past = 0;
+#pragma unroll
+      for (int step = 16; step > 0; step >>= 1)
+        if (__shfl_sync(0xffffffffu, end, past + step - 1) <= t) past += step;
+      const bool beyond = __shfl_sync(0xffffffffu, end, 31) <= t;  // empty sequences between
+      if (live) s = beyond ? sequence_of(a.cu, a.num_seqs, t) : lo + past;
+    }
+    if (live) {
+      const int64_t p = (int64_t)__ldg(a.kv_lens + s) - __ldg(a.cu + s + 1) + t;
+      const int64_t page =
+          page_of(a.table, a.table_stride, a.table_cols, a.num_pages, s, p, a.status);
+      at.page = page < 0 ? -1 : page * a.kv_heads * block_bytes(G);
+      at.slot = (int)(p & (kPage - 1));
+    }
+    if (warp_id() * 32 + lane < a.tile) places[warp_id() * 32 + lane] = at;
+  }
+  __syncthreads();
 }
 
-// ---------------------------------------------------------------------------
-// By tokens.
-// ---------------------------------------------------------------------------
+// What a warp does, turn by turn, and its lanes' parts in it: PARTS lanes share a
+// group of a token.
+template <int G, int PARTS>
+struct Turns {
+  static constexpr int kUnit = 32 / G;            // tokens of 4 / G octets,
+  static constexpr int kSteps = PARTS;            // which take so many turns in one head
+  static constexpr int kSide = 32 / (4 * PARTS);  // tokens of an octet in a turn
+  static constexpr int kWarps = kThreads / 32;
+  int head, tok, end;  // of the tokens, where the turns end
+  int heads;
+  CTI_DEVICE Turns(int tile, int heads_) : heads(heads_) {
+    const int lane = lane_id(), warp = warp_id();
+    head = warp / kSteps;
+    end = heads > 0 ? tile : 0;
+    tok = (lane / PARTS & 3) / G * 8 + warp % kSteps * kSide + lane / (4 * PARTS);
+    wrap();
+  }
+  CTI_DEVICE void wrap() {
+    while (head >= heads && tok < end) head -= heads, tok += kUnit;
+  }
+  CTI_DEVICE void next() {
+    head += kWarps / kSteps;
+    wrap();
+  }
+  // The same for a whole warp: its tokens are all of one unit.
+  CTI_DEVICE bool more() const { return tok < end; }
+  CTI_DEVICE static int group() { return (lane_id() / PARTS & 3) % G; }
+  CTI_DEVICE static int part() { return lane_id() % PARTS; }
+};
+
+// The heads of this block: gridDim.y blocks share a tile.
+CTI_DEVICE int2 heads_of(const Args& a) {
+  const int per = (a.kv_heads + gridDim.y - 1) / gridDim.y;
+  const int first = min(a.kv_heads, per * (int)blockIdx.y);
+  return make_int2(first, min(a.kv_heads - first, per));
+}
+
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads)
-    kv4_append_tokens_kernel(const T* __restrict__ k, const T* __restrict__ v, Args a,
-                             uint8_t* __restrict__ pages) {
+    kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, Args a,
+                      uint8_t* __restrict__ pages) {
+  using Turn = Turns<G, 2>;
   __shared__ Place places[kTokens];
-  const int t0 = blockIdx.x * kTokens;
-  if (threadIdx.x < kTokens) places[threadIdx.x] = find_place(a, t0 + threadIdx.x);
-  __syncthreads();
-  const int per = a.kv_heads * G * 2;  // 16-dim pieces of a token
-  const int total = (kTokens * per + 31) & ~31;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int tok = i / per, piece = i - tok * per;
-    const Place at = tok < kTokens ? places[tok] : Place{-1, 0};
-    const int head = piece / (2 * G), g = (piece >> 1) & (G - 1), t = 2 * (piece & 1);
-    const bool live = at.page >= 0;
+  const int t0 = blockIdx.x * a.tile;
+  find_places<G>(a, t0, places);
+  const int2 heads = heads_of(a);
+  // Offsets of 32 bits: the tile's tokens are within 2^31 elements of each other.
+  const T* kt = k + t0 * a.k_stride;
+  const T* vt = v + t0 * a.v_stride;
+  const int g = Turn::group(), part = Turn::part();
+  for (Turn i(a.tile, heads.y); i.more(); i.next()) {
+    const Place at = places[i.tok];
+    const int head = heads.x + i.head, piece = (2 * (head * G + g) + part) * 16;
     uint4 rk[2], rv[2];
     rk[0] = rk[1] = rv[0] = rv[1] = make_uint4(0, 0, 0, 0);
-    if (live) {
-      const uint4* pk =
-          reinterpret_cast<const uint4*>(k + (t0 + tok) * a.k_stride + piece * 16);
-      const uint4* pv =
-          reinterpret_cast<const uint4*>(v + (t0 + tok) * a.v_stride + piece * 16);
+    if (at.page >= 0) {
+      const uint4* pk = reinterpret_cast<const uint4*>(kt + (i.tok * (int)a.k_stride + piece));
+      const uint4* pv = reinterpret_cast<const uint4*>(vt + (i.tok * (int)a.v_stride + piece));
       rk[0] = __ldg(pk);
       rk[1] = __ldg(pk + 1);
       rv[0] = __ldg(pv);
@@ -272,18 +343,18 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t ks, kb, vs, vb, wk[2], wv[2];
     quantise<T, kKeys>(rk, wk, ks, kb);
     quantise<T, kValues>(rv, wv, vs, vb);
-    if (!live) continue;  // the loop's bound is the same for a whole warp
-    uint8_t* block = pages + (at.page * a.kv_heads + head) * (int64_t)block_bytes(G);
+    if (at.page < 0) continue;  // the loop's end is the same for a whole warp
+    uint8_t* block = pages + at.page + head * block_bytes(G);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      *reinterpret_cast<uint32_t*>(block + k_word_at(at.slot, g, t + x, G)) = wk[x];
+      *reinterpret_cast<uint32_t*>(block + k_word_at(at.slot, g, 2 * part + x, G)) = wk[x];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
         *reinterpret_cast<uint16_t*>(block + v_codes_at(G) +
-                                     v_half_at(at.slot, g, 2 * (t + x) + c, G)) =
+                                     v_half_at(at.slot, g, 4 * part + 2 * x + c, G)) =
             (uint16_t)(wv[x] >> (16 * c));
     }
-    if (t == 0) {
+    if (part == 0) {
       *reinterpret_cast<uint32_t*>(block + k_meta_at(G) + k_meta_word_at(at.slot, g, G)) =
           ks | kb << 16;
       uint8_t* vm = block + v_meta_at(G) + v_meta_half_at(at.slot, g, G);
@@ -295,335 +366,61 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads)
-    kv4_read_tokens_kernel(const uint8_t* __restrict__ pages, Args a, T* __restrict__ k,
-                           T* __restrict__ v) {
+    kv4_read_kernel(const uint8_t* __restrict__ pages, Args a, T* __restrict__ k,
+                    T* __restrict__ v) {
+  using Turn = Turns<G, 4>;
   __shared__ Place places[kTokens];
-  const int t0 = blockIdx.x * kTokens;
+  const int t0 = blockIdx.x * a.tile;
   grid_dependency_wait();
-  if (threadIdx.x < kTokens) places[threadIdx.x] = find_place(a, t0 + threadIdx.x);
-  __syncthreads();
-  const int per = a.kv_heads * G * 4;
-  const int total = kTokens * per;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int tok = i / per, piece = i - tok * per;
-    const Place at = places[tok];
-    if (at.page == -2) continue;
-    const int head = piece / (4 * G), g = (piece >> 2) & (G - 1), t = piece & 3;
-    uint4 ok = make_uint4(0, 0, 0, 0), ov = ok;
-    if (at.page >= 0) {
-      const uint8_t* block = pages + (at.page * a.kv_heads + head) * (int64_t)block_bytes(G);
-      const uint32_t wk =
-          __ldg(reinterpret_cast<const uint32_t*>(block + k_word_at(at.slot, g, t, G)));
-      const uint32_t mk = __ldg(
-          reinterpret_cast<const uint32_t*>(block + k_meta_at(G) + k_meta_word_at(at.slot, g, G)));
-      const uint8_t* vm = block + v_meta_at(G) + v_meta_half_at(at.slot, g, G);
-      const uint32_t vs = __ldg(reinterpret_cast<const uint16_t*>(vm));
-      const uint32_t vb = __ldg(reinterpret_cast<const uint16_t*>(vm + 4));
+  find_places<G>(a, t0, places);
+  const int2 heads = heads_of(a);
+  T* kt = k + t0 * a.k_stride;
+  T* vt = v + t0 * a.v_stride;
+  const int g = Turn::group(), part = Turn::part();
+  constexpr int N = 2;  // turns at once: all loads first
+  for (Turn i(a.tile, heads.y); i.more();) {
+    uint32_t wk[N], mk[N], h0[N], h1[N];
+    uint2 mv[N];
+    int64_t page[N];
+    int tok[N], piece[N];
+    bool odd[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      page[n] = -2;
+      if (!i.more()) continue;
+      const Place at = places[i.tok];
+      const int head = heads.x + i.head;
+      page[n] = at.page;
+      tok[n] = i.tok;
+      piece[n] = (4 * (head * G + g) + part) * 8;
+      odd[n] = at.slot & 1;
+      i.next();
+      if (at.page < 0) continue;
+      const uint8_t* block = pages + at.page + head * block_bytes(G);
+      wk[n] = __ldg(reinterpret_cast<const uint32_t*>(block + k_word_at(at.slot, g, part, G)));
+      mk[n] = __ldg(reinterpret_cast<const uint32_t*>(block + k_meta_at(G) +
+                                                      k_meta_word_at(at.slot, g, G)));
+      mv[n] = __ldg(reinterpret_cast<const uint2*>(block + v_meta_at(G) +
+                                                   v_meta_half_at(at.slot & ~1, g, G)));
       const uint8_t* vc = block + v_codes_at(G);
-      const uint32_t h0 =
-          __ldg(reinterpret_cast<const uint16_t*>(vc + v_half_at(at.slot, g, 2 * t, G)));
-      const uint32_t h1 =
-          __ldg(reinterpret_cast<const uint16_t*>(vc + v_half_at(at.slot, g, 2 * t + 1, G)));
-      uint2 v0, v1;
-      v_values<T>(h0 | h1 << 16, twice(vs), twice(vb), v0, v1);
-      ok = k_values<T>(wk, mk);
-      ov = make_uint4(v0.x, v0.y, v1.x, v1.y);
+      h0[n] = __ldg(reinterpret_cast<const uint16_t*>(vc + v_half_at(at.slot, g, 2 * part, G)));
+      h1[n] = __ldg(reinterpret_cast<const uint16_t*>(vc + v_half_at(at.slot, g, 2 * part + 1, G)));
     }
-    *reinterpret_cast<uint4*>(k + (t0 + tok) * a.k_stride + piece * 8) = ok;
-    *reinterpret_cast<uint4*>(v + (t0 + tok) * a.v_stride + piece * 8) = ov;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// By runs.
-// ---------------------------------------------------------------------------
-// Side by side in one page: packed tokens [start, start + count), from `slot`
-// of the page on.
-struct Run {
-  int64_t page;
-  int start, count, slot;
-};
-
-// The runs that START among the block's a.tile packed tokens from t0 on, so
-// that no run is cut at a tile's end.  All threads of the block; returns their
-// number.
-CTI_DEVICE int find_runs(const Args& a, int t0, Run (&runs)[kRunTokens]) {
-  static_assert(kRunTokens % 32 == 0 && kRunTokens <= kThreads, "a thread per token");
-  __shared__ int32_t ends[kRunTokens];  // cu[s0 + 1 + i]
-  __shared__ uint32_t starts[kRunTokens / 32];
-  __shared__ int s0_shared;
-  const int i = threadIdx.x, tile = a.tile;
-  if (i < 32) {  // the sequence of token t0, 32 borders at a time
-    int lo = 0, hi = a.num_seqs;  // cu[lo] <= t0 (or lo = 0), and t0 < cu[hi]
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 31) / 32, at = lo + (i + 1) * step;
-      const uint32_t le = __ballot_sync(0xffffffffu, at < hi && __ldg(a.cu + at) <= t0);
-      const int last = __popc(le);
-      hi = min(hi, lo + (last + 1) * step);
-      lo += last * step;
-    }
-    if (i == 0) s0_shared = lo;
-  }
-  __syncthreads();
-  const int s0 = s0_shared;
-  if (i < tile) ends[i] = __ldg(a.cu + min(s0 + 1 + i, a.num_seqs));
-  __syncthreads();
-  const int t = t0 + i;
-  Run run = {-2, t, 0, 0};
-  if (i < tile && t < a.tokens && t >= __ldg(a.cu) && t < __ldg(a.cu + a.num_seqs)) {
-    int s = s0;
-    if (ends[tile - 1] > t) {
-      int lo = -1, hi = tile - 1;  // ends[lo] <= t < ends[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (ends[mid] <= t) lo = mid;
-        else hi = mid;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (page[n] == -2) continue;
+      uint4 ok = make_uint4(0, 0, 0, 0), ov = ok;
+      if (page[n] >= 0) {
+        const uint32_t both = odd[n] ? 0x3232 : 0x1010;
+        uint2 v0, v1;
+        v_values<T>(h0[n] | h1[n] << 16, __byte_perm(mv[n].x, 0, both),
+                    __byte_perm(mv[n].y, 0, both), v0, v1);
+        ok = k_values<T>(wk[n], mk[n]);
+        ov = make_uint4(v0.x, v0.y, v1.x, v1.y);
       }
-      s += hi;
-    } else {  // more than `tile` sequences, empty ones, lie within the tile
-      s = sequence_of(a.cu, a.num_seqs, a.tokens, t);
+      *reinterpret_cast<uint4*>(kt + (tok[n] * (int)a.k_stride + piece[n])) = ok;
+      *reinterpret_cast<uint4*>(vt + (tok[n] * (int)a.v_stride + piece[n])) = ov;
     }
-    const int end = min(__ldg(a.cu + s + 1), a.tokens);
-    const int64_t pos = (int64_t)__ldg(a.kv_lens + s) - __ldg(a.cu + s + 1) + t;
-    run.slot = (int)(pos & (kPage - 1));
-    if (t == __ldg(a.cu + s) || run.slot == 0) {
-      run.count = min(kPage - run.slot, end - t);
-      run.page = page_of(a.table, a.table_stride, a.table_cols, a.num_pages, s, pos, a.status);
-    }
-  }
-  if (i < tile) {
-    const uint32_t b = __ballot_sync(0xffffffffu, run.count > 0);
-    if ((i & 31) == 0) starts[i >> 5] = b;
-  }
-  __syncthreads();
-  int count = 0, before = 0;
-  for (int w = 0; w < tile / 32; ++w) {
-    if (w == i / 32) before = count + __popc(starts[w] & ((1u << (i & 31)) - 1));
-    count += __popc(starts[w]);
-  }
-  if (run.count > 0) runs[before] = run;
-  __syncthreads();
-  return count;
-}
-
-// A run's keys (or values) of one head.  Lane 16 z + 2 r + u takes dims 16 u ..
-// + 15 of token r of an octet: for every group (G = 2, 4), or of two octets
-// (G = 1).  A step takes 2 octets (4).
-template <typename T, int G, Order ORDER>
-CTI_DEVICE void append_run(const T* __restrict__ rows, int stride, const Run& run,
-                           uint8_t* __restrict__ block, int lane) {
-  constexpr int kOctets = G == 1 ? 4 : 2;
-  constexpr int N = G == 4 ? 4 : 2;  // words that a lane has in each of two vectors of codes
-  const int z = lane >> 4, r = (lane >> 1) & 7, u = lane & 1, last = run.slot + run.count - 1;
-  const bool odd = r & 1;
-  // The lanes of the layout whose words this one has in the end: keys, 4 r + 2 u
-  // and the next; values, those of the pair of tokens r / 2 and the dims 16 u + 8
-  // (r % 2) .. + 7.
-  const int owner0 = ORDER == kKeys ? 4 * r + 2 * u : (4 * u + 2 * (r & 1)) * 4 + (r >> 1);
-  constexpr int kNext = ORDER == kKeys ? 16 : 64;  // bytes to the second
-  uint8_t* codes = block + (ORDER == kKeys ? 0 : v_codes_at(G));
-  for (int nt0 = (run.slot >> 3) / kOctets * kOctets; 8 * nt0 <= last; nt0 += kOctets) {
-    const int nt = nt0 + z;  // this lane's octet; G = 1: and the one after the next
-    const int src = (8 * nt + r - run.slot) * stride + 16 * u;
-    uint4 raw[N][2];
-    bool live[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int tau = 8 * (G == 1 ? nt + 2 * j : nt) + r;
-      live[j] = tau >= run.slot && tau <= last;
-      raw[j][0] = raw[j][1] = make_uint4(0, 0, 0, 0);
-      if (live[j]) {
-        const uint4* p = reinterpret_cast<const uint4*>(
-            rows + src + (G == 1 ? 16 * j * stride : 32 * j));
-        raw[j][0] = __ldg(p);
-        raw[j][1] = __ldg(p + 1);
-      }
-    }
-    uint32_t w[N][2];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int tau = 8 * (G == 1 ? nt + 2 * j : nt) + r, g = G == 1 ? 0 : j;
-      if (G == 1 && !__any_sync(0xffffffffu, live[j])) continue;
-      uint32_t s, b;
-      quantise<T, ORDER>(raw[j], w[j], s, b);
-      if (ORDER == kKeys) {
-        if (live[j] && u == 0)
-          *reinterpret_cast<uint32_t*>(block + k_meta_at(G) + k_meta_word_at(tau, g, G)) =
-              s | b << 16;
-      } else {
-        // Two tokens share a word: each lane of the pair gets half of the dims.
-        const bool pair = live[j] && (tau ^ 1) >= run.slot && (tau ^ 1) <= last;
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? w[j][0] : w[j][1], 2);
-        const uint32_t mine = s | b << 16, meta = __shfl_xor_sync(0xffffffffu, mine, 2);
-        uint8_t* vm = block + v_meta_at(G) + v_meta_half_at(tau, g, G);
-        if (live[j] && !pair) {  // an end of the run: its own halves alone
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint16_t*>(codes + v_half_at(tau, g, 4 * u + c, G)) =
-                (uint16_t)(w[j][c >> 1] >> (16 * (c & 1)));
-          if (u == 0) {
-            *reinterpret_cast<uint16_t*>(vm) = (uint16_t)s;
-            *reinterpret_cast<uint16_t*>(vm + 4) = (uint16_t)b;
-          }
-        } else if (pair && u == 0 && !odd) {
-          *reinterpret_cast<uint2*>(vm) =
-              make_uint2(__byte_perm(mine, meta, 0x5410), __byte_perm(mine, meta, 0x7632));
-        }
-        const uint32_t even_w = odd ? got : w[j][0], odd_w = odd ? w[j][1] : got;
-        w[j][0] = __byte_perm(even_w, odd_w, 0x5410);
-        w[j][1] = __byte_perm(even_w, odd_w, 0x7632);
-        live[j] = pair;
-      }
-    }
-    const int word0 = nt * G;  // of the lane's words in the layout
-    uint8_t* dst = codes + ((word0 >> 2) * 32 + owner0) * 16 + (word0 & 3) * 4;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if constexpr (N == 4) {
-        if (live[0])
-          *reinterpret_cast<uint4*>(dst + x * kNext) =
-              make_uint4(w[0][x], w[1][x], w[2][x], w[3][x]);
-      } else if constexpr (G == 2) {
-        if (live[0]) *reinterpret_cast<uint2*>(dst + x * kNext) = make_uint2(w[0][x], w[1][x]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (live[j]) *reinterpret_cast<uint32_t*>(dst + x * kNext + 8 * j) = w[j][x];
-      }
-    }
-  }
-}
-
-// The heads [first, end) of this block: gridDim.y blocks share a tile.
-CTI_DEVICE void head_range(const Args& a, int& first, int& end) {
-  const int per = (a.kv_heads + gridDim.y - 1) / gridDim.y;
-  first = min(a.kv_heads, per * (int)blockIdx.y);
-  end = min(a.kv_heads, first + per);
-}
-
-template <typename T, int G>
-__global__ void __launch_bounds__(kThreads, 4)
-    kv4_append_runs_kernel(const T* __restrict__ k, const T* __restrict__ v, Args a,
-                           uint8_t* __restrict__ pages) {
-  __shared__ Run runs[kRunTokens];
-  const int lane = lane_id();
-  int h0, h1;
-  head_range(a, h0, h1);
-  const int heads = h1 - h0, units = find_runs(a, blockIdx.x * a.tile, runs) * heads * 2;
-  for (int u = warp_id(); u < units; u += kThreads / 32) {
-    const int i = (u >> 1) / heads, head = h0 + (u >> 1) - i * heads;
-    const Run run = runs[i];
-    if (run.page < 0) continue;
-    uint8_t* block = pages + (run.page * a.kv_heads + head) * (int64_t)block_bytes(G);
-    if ((u & 1) == 0)
-      append_run<T, G, kKeys>(k + run.start * a.k_stride + head * (32 * G), (int)a.k_stride, run,
-                              block, lane);
-    else
-      append_run<T, G, kValues>(v + run.start * a.v_stride + head * (32 * G), (int)a.v_stride, run,
-                                block, lane);
-  }
-}
-
-template <typename T, int G>
-CTI_DEVICE void read_keys(const uint8_t* __restrict__ block, const Run& run, T* __restrict__ rows,
-                          int stride, int lane) {
-  constexpr int kOctets = 4 / G;
-  const int r = lane >> 2, t = lane & 3, last = run.slot + run.count - 1;
-  const int v0 = (run.slot >> 3) / kOctets;
-  int tau0 = v0 * kOctets * 8 + r;
-  int dst = (tau0 - run.slot) * stride + 8 * t;
-  const uint8_t* src = block + (v0 * 32 + lane) * 16;
-  const uint32_t* ms = reinterpret_cast<const uint32_t*>(block + k_meta_at(G)) + tau0 * G;
-  // Two vectors at a time, all loads first.
-  for (; tau0 - r <= last; tau0 += 16 * kOctets, dst += 16 * kOctets * stride, src += 1024, ms += 64) {
-    uint4 w4[2];
-    uint32_t meta[8];
-    bool live[8];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      w4[u] = make_uint4(0, 0, 0, 0);
-      if (tau0 - r + 8 * kOctets * u <= last) w4[u] = __ldg(reinterpret_cast<const uint4*>(src + 512 * u));
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int nt = j / G, g = j % G, tau = tau0 + 8 * nt;
-      live[j] = tau >= run.slot && tau <= last;
-      if (live[j]) meta[j] = __ldg(ms + 8 * nt * G + g);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int nt = j / G, g = j % G;
-      const uint32_t w = j % 4 == 0 ? w4[j / 4].x : j % 4 == 1 ? w4[j / 4].y
-                         : j % 4 == 2 ? w4[j / 4].z : w4[j / 4].w;
-      if (live[j])
-        *reinterpret_cast<uint4*>(rows + (dst + 8 * nt * stride) + 32 * g) =
-            k_values<T>(w, meta[j]);
-    }
-  }
-}
-
-template <typename T, int G>
-CTI_DEVICE void read_values(const uint8_t* __restrict__ block, const Run& run,
-                            T* __restrict__ rows, int stride, int lane) {
-  constexpr int kOctets = 4 / G;
-  const int c = lane >> 2, t = lane & 3, last = run.slot + run.count - 1;
-  const int v0 = (run.slot >> 3) / kOctets;
-  int tau0 = v0 * kOctets * 8 + 2 * t;  // and the token after it
-  int dst = (tau0 - run.slot) * stride + 4 * c;
-  const uint8_t* src = block + v_codes_at(G) + (v0 * 32 + lane) * 16;
-  const uint2* ms = reinterpret_cast<const uint2*>(block + v_meta_at(G)) + (tau0 >> 1) * G;
-  for (; tau0 - 2 * t <= last; tau0 += 16 * kOctets, dst += 16 * kOctets * stride, src += 1024, ms += 32) {
-    uint4 w4[2];
-    uint2 meta[8];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      w4[u] = make_uint4(0, 0, 0, 0);
-      if (tau0 - 2 * t + 8 * kOctets * u <= last) {
-        w4[u] = __ldg(reinterpret_cast<const uint4*>(src + 512 * u));
-#pragma unroll
-        for (int j = 4 * u; j < 4 * u + 4; ++j) meta[j] = __ldg(ms + 4 * (j / G) * G + j % G);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int nt = j / G, g = j % G, tau = tau0 + 8 * nt;
-      const uint32_t w = j % 4 == 0 ? w4[j / 4].x : j % 4 == 1 ? w4[j / 4].y
-                         : j % 4 == 2 ? w4[j / 4].z : w4[j / 4].w;
-      T* to = rows + (dst + 8 * nt * stride) + 32 * g;
-      uint2 even, odd;
-      v_values<T>(w, meta[j].x, meta[j].y, even, odd);
-      if (tau >= run.slot && tau <= last) *reinterpret_cast<uint2*>(to) = even;
-      if (tau + 1 >= run.slot && tau + 1 <= last) *reinterpret_cast<uint2*>(to + stride) = odd;
-    }
-  }
-}
-
-template <typename T, int G>
-__global__ void __launch_bounds__(kThreads, 4)
-    kv4_read_runs_kernel(const uint8_t* __restrict__ pages, Args a, T* __restrict__ k,
-                         T* __restrict__ v) {
-  __shared__ Run runs[kRunTokens];
-  const int lane = lane_id();
-  grid_dependency_wait();
-  int h0, h1;
-  head_range(a, h0, h1);
-  const int heads = h1 - h0, units = find_runs(a, blockIdx.x * a.tile, runs) * heads * 2;
-  for (int u = warp_id(); u < units; u += kThreads / 32) {
-    const int i = (u >> 1) / heads, head = h0 + (u >> 1) - i * heads;
-    const Run run = runs[i];
-    const int64_t stride = (u & 1) == 0 ? a.k_stride : a.v_stride;
-    T* rows = ((u & 1) == 0 ? k : v) + run.start * stride + head * (32 * G);
-    if (run.page < 0) {  // every token of it is outside: zeros
-      for (int j = lane; j < run.count * 4 * G; j += 32)
-        *reinterpret_cast<uint4*>(rows + (j / (4 * G)) * stride + (j % (4 * G)) * 8) =
-            make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    const uint8_t* block = pages + (run.page * a.kv_heads + head) * (int64_t)block_bytes(G);
-    if ((u & 1) == 0)
-      read_keys<T, G>(block, run, rows, (int)stride, lane);
-    else
-      read_values<T, G>(block, run, rows, (int)stride, lane);
   }
 }
 
@@ -637,7 +434,8 @@ int check_args(const void* k, const void* v, int dtype, int head_dim, const Args
     return CTI_ERR_INVALID_ARG;
   if (dtype != CTI_DTYPE_BF16 && dtype != CTI_DTYPE_F16) return CTI_ERR_UNSUPPORTED;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128) return CTI_ERR_UNSUPPORTED;
-  if (tokens > INT32_MAX - 256 || a.kv_heads > 65535) return CTI_ERR_UNSUPPORTED;
+  if (tokens > INT32_MAX - 256 || a.num_seqs > INT32_MAX - 256 || a.kv_heads > 65535)
+    return CTI_ERR_UNSUPPORTED;
   if (a.num_seqs == 0 || tokens == 0) {
     *empty = true;
     return CTI_OK;
@@ -648,50 +446,38 @@ int check_args(const void* k, const void* v, int dtype, int head_dim, const Args
   const int64_t row = (int64_t)a.kv_heads * head_dim;
   if ((a.k_stride | a.v_stride) % 8 != 0 || a.k_stride < row || a.v_stride < row)
     return CTI_ERR_INVALID_ARG;
-  // A page's tokens are within 2^31 elements of each other.
+  // A tile's tokens are within 2^31 elements of each other.
   if (a.k_stride > kMaxStride || a.v_stride > kMaxStride) return CTI_ERR_UNSUPPORTED;
   if (a.table_stride < a.table_cols) return CTI_ERR_INVALID_ARG;
   return CTI_OK;
 }
 
-// The way, the tile and the grid of a call.
-struct Launch {
-  bool runs;
-  dim3 grid;
-};
-Launch plan(Args& a, int G) {
-  Launch l;
-  l.runs = a.tokens >= (int64_t)kRunsFrom * a.num_seqs;
-  // Longer tiles share the way to their runs among more of them, as long as
-  // there are four blocks for each SM.
-  a.tile = !l.runs ? kTokens : a.tokens >= kSMs * 4 * kRunTokens ? kRunTokens : kRunTokens / 2;
+// The tokens of a block and the grid of a call: a turn for each warp; blocks that
+// share a tile by heads, until there are four blocks for each SM; and two tiles'
+// tokens to a block where that leaves 8 for each SM (278,000 tokens of 8 heads of 32:
+// 125 us become 115 to append, 92 become 82 to read; four: 113 and 84).
+dim3 plan(Args& a, int G) {
+  const int heads = kThreads / 64;  // that keep a block's warps busy
+  a.tile = 32 / G * (a.kv_heads >= heads ? 1 : (heads + a.kv_heads - 1) / a.kv_heads);
+  if (a.tile < kTokens && a.tokens >= (int64_t)a.tile * 2 * 8 * kSMs) a.tile *= 2;
   const int64_t tiles = ((int64_t)a.tokens + a.tile - 1) / a.tile;
-  l.grid = dim3((unsigned)tiles);
-  if (l.runs) {
-    // Blocks that share a tile by heads: at least four for each SM in all, as
-    // long as a block's warps have a run each (two runs start in a tile at
-    // the least, with keys and values apart).
-    int64_t share = (kSMs * 4 + tiles - 1) / tiles;
-    const int64_t most = a.kv_heads * G > 2 ? (a.kv_heads + 1) / 2 : 1;
-    l.grid.y = (unsigned)(share > most ? most : share);
-  }
-  return l;
+  const int64_t share = (kSMs * 4 + tiles - 1) / tiles;
+  const int64_t most = (a.kv_heads + heads - 1) / heads;
+  return dim3((unsigned)tiles, (unsigned)(share < most ? share : most));
 }
 
 template <typename T, int G>
 int launch_append(const void* k, const void* v, Args a, void* pages, cudaStream_t s) {
-  const Launch l = plan(a, G);
-  auto* kernel = l.runs ? kv4_append_runs_kernel<T, G> : kv4_append_tokens_kernel<T, G>;
-  kernel<<<l.grid, kThreads, 0, s>>>(static_cast<const T*>(k), static_cast<const T*>(v), a,
-                                     static_cast<uint8_t*>(pages));
+  const dim3 grid = plan(a, G);
+  kv4_append_kernel<T, G><<<grid, kThreads, 0, s>>>(
+      static_cast<const T*>(k), static_cast<const T*>(v), a, static_cast<uint8_t*>(pages));
   return cudaGetLastError() == cudaSuccess ? CTI_OK : CTI_ERR_CUDA;
 }
 
 template <typename T, int G>
 int launch_read(const void* pages, Args a, void* k, void* v, cudaStream_t s) {
-  const Launch l = plan(a, G);
-  auto* kernel = l.runs ? kv4_read_runs_kernel<T, G> : kv4_read_tokens_kernel<T, G>;
-  return launch_dependent(kernel, l.grid, dim3(kThreads), 0, s,
+  const dim3 grid = plan(a, G);
+  return launch_dependent(kv4_read_kernel<T, G>, grid, dim3(kThreads), 0, s,
                           static_cast<const uint8_t*>(pages), a, static_cast<T*>(k),
                           static_cast<T*>(v)) == cudaSuccess
              ? CTI_OK

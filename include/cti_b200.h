@@ -385,7 +385,8 @@ size_t cti_kv4_page_bytes(int kv_heads, int head_dim);
 
 /* Writes the packed tokens' keys and values (views [tokens][kv_heads][head_dim]
  * with token strides in elements, multiples of 8, at most 2^24; 16-byte
- * aligned bases). */
+ * aligned bases).  tokens and num_seqs at most 2^31 - 257, kv_heads 65535
+ * (CTI_ERR_UNSUPPORTED otherwise). */
 int cti_kv4_append(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int dtype,
                    const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* page_table,
                    int64_t table_stride, int table_cols, int num_seqs, int64_t tokens,
