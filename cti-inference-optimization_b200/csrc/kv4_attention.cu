@@ -9,7 +9,7 @@
 // Calls with many rows per sequence go to the tensor-core tiles of
 // kv4_tiles.cu; the rest of this file is for single tokens and a few.
 //
-// A warp takes a tile of 4 to 32 rows (the query heads of one KV head,
+// A warp takes a tile of 4, 8 or 16 rows (the query heads of one KV head,
 // token by token) and a range of the sequence's pages.  One bulk copy brings a
 // page's block of the KV head (2560 G bytes) into the warp's own ring in
 // shared memory; nothing else of the cache is read.  Per page, with keys and
@@ -65,7 +65,7 @@ __host__ __device__ constexpr int slot_bytes(int G) {
 }
 __host__ __device__ constexpr int slots(int G) { return G == 1 ? 3 : 2; }
 __host__ __device__ constexpr int blocks_per_sm(int G, int NT) {
-  return NT == 4 ? 2 : G == 4 ? (NT == 1 ? 4 : 2) : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 6 : 4;
+  return G == 4 ? (NT == 1 ? 4 : 2) : G == 2 ? (NT == 1 ? 4 : 3) : NT == 1 ? 6 : 4;
 }
 __host__ __device__ constexpr size_t smem_bytes(int G) {
   return (size_t)kWarps * slots(G) * (slot_bytes(G) + 8);
@@ -128,7 +128,7 @@ CTI_DEVICE uint32_t k_codes(uint32_t w, int j) {
   return (j < 2 ? w : w >> 8) & (j & 1 ? 0x00f000f0u : 0x000f000fu);
 }
 
-// ROWS: of a tile, 4, 8, 16 or 32.
+// ROWS: of a tile, 4, 8 or 16.
 template <typename T, int G, int ROWS>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
     kv4_attention_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pages, const Args a,
@@ -725,13 +725,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 }
 
 // Query rows of a KV head, by the caller's bound, from which a sequence's rows
-// are taken in tiles of 128 on the tensor cores.
-constexpr int kTilesFrom = 97;
+// are taken in tiles of 128 on the tensor cores: the first where the sequences' KV
+// heads fill half of the GPU, else the second.  Measured, us here and there, 2,000
+// keys, head_dim 32 / 64 / 128:
+//   96 sequences of 4 KV heads: 64 rows, 72 and 80 / 104 and 100 / 180 and 164;
+//                               96 rows, 98 and 80 / 145 and 100 / 254 and 166
+//   8 sequences:                64 rows, 20 and 22 / 24 and 24 / 32 and 34;
+//                              128 rows, 26 and 24 / 38 and 26 / 48 and 38
+//   1 sequence of 8 KV heads:  128 rows, 17 and 20 / 17 and 24 / 22 and 34
+constexpr int kTilesFrom = 65, kTilesFromFew = 97;
 
 // How a call is laid out over the GPU; a function of the sizes alone.
 struct Plan {
   int big;             // 128-row tiles of a block (kv4_tiles.cu), 1 or 2; 0: warps as here
-  int rows;            // that a warp takes: 4, 8, 16 or 32
+  int rows;            // that a warp takes: 4, 8 or 16
   bool shared;         // a block's warps share a tile's pages
   int splits, chunk;   // blocks that share them, and the pages of each
   int64_t tiles;       // row tiles of a sequence
@@ -744,32 +751,45 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   const int64_t rows = (most > 0 ? most : 1) * (heads / kv_heads);
   const int64_t pages = max_kv_len > 0 ? (max_kv_len + kPage - 1) / kPage : 1;
   Plan p = {};
-  if (rows >= kTilesFrom) {
-    // Two tiles share the unpacking of a page.  Fewer blocks than the GPU holds
-    // share the pages, eight at least.
-    p.big = rows > 128 ? 2 : 1;
+  const double sequences = (double)num_seqs * kv_heads;
+  if (rows >= (sequences >= kSMs / 2 ? kTilesFrom : kTilesFromFew)) {
+    // Two tiles share the unpacking of a page, which costs less than one of two
+    // blocks' latency hidden by the other, but for head_dim 32 (2,048 rows of 384
+    // KV heads over 2,000 keys: 1092 us with two, 1071 with one; for 64, 1235 and
+    // 1378; for 128, 1639 and 2264; 192 rows: 133 and 131, 150 and 168, 197 and
+    // 268).  Fewer blocks than the GPU holds share the pages, eight at least.
+    p.big = rows > 128 && G > 1 ? 2 : 1;
     p.tiles = (rows + 128 * p.big - 1) / (128 * p.big);
-    const double blocks = (double)num_seqs * kv_heads * (double)p.tiles;
+    const double blocks = sequences * (double)p.tiles;
     int64_t splits = (int64_t)(kSMs * (3 - p.big) / blocks);
     splits = splits > pages / 8 ? pages / 8 : splits;
     p.splits = (int)(splits < 1 ? 1 : splits > 128 ? 128 : splits);
     p.chunk = (int)((pages + p.splits - 1) / p.splits);
     return p;
   }
-  p.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || G == 4 ? 16 : 32;
+  // (96 sequences of 4 KV heads, 2,000 keys, head_dim 32 / 64 / 128: 8 rows in
+  // tiles of 4 33 us / 39 / 64, of 8 25 / 31 / 45; 16 rows in tiles of 8 35 / 41 /
+  // 68, of 16 35 / 43 / 59; 48 rows 66 / 92 / 162, 53 / 80 / 133, and, for 32 and
+  // 64, 72 / 102 in tiles of 32.)
+  p.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
   p.tiles = (rows + p.rows - 1) / p.rows;
-  const double units = (double)num_seqs * kv_heads * (double)p.tiles;
+  const double units = sequences * (double)p.tiles;
   const double room = (double)kSMs * blocks_per_sm(G, (p.rows + 7) / 8) * kWarps;  // warps at once
   p.splits = 1;
   p.chunk = 0;
-  if (units >= room && pages <= 8) {
-    // Short sequences, more tiles than warps: a warp each.
+  if (units >= room && pages <= (units >= 4 * room ? 64 : 16)) {
+    // More tiles than warps, and none so long that the last ones run alone: a
+    // warp each.  (Lengths up to 16 pages, 8 heads of 32: 600 sequences 82 us,
+    // 92 shared; 2,400 sequences 135 and 170.  Up to 64 pages: 300 sequences,
+    // less than four times the warps, 158 and 140; 2,400 sequences 446 and 511.)
     p.shared = false;
     return p;
   }
   // A block's warps share a tile; with long sequences, blocks do too, so that
   // all run at once, or, where that is more than 16 pages for a warp, in
-  // pieces of 12, small enough that sequences of any lengths balance out.
+  // pieces of 12, small enough that sequences of any lengths balance out (48
+  // sequences of 1,000 to 8,000 keys, 8 KV heads of 128: 81 us, 91 without and 85
+  // with pieces of 4; 128 of 100 to 16,000: 294, 335 and 343).
   p.shared = true;
   const double ideal = units * pages / room;
   int64_t per_warp = ideal > 16 ? 12 : (int64_t)ideal + 1;
@@ -826,10 +846,8 @@ int launch_shape(const void* q, const void* pages, const Args& a, const Plan& p,
     rc = launch<T, G, 4>(q, pages, a, p, out, s);
   } else if (p.rows == 8) {
     rc = launch<T, G, 8>(q, pages, a, p, out, s);
-  } else if (G == 4 || p.rows == 16) {
-    rc = launch<T, G, 16>(q, pages, a, p, out, s);
   } else {
-    rc = launch<T, G, G == 4 ? 16 : 32>(q, pages, a, p, out, s);
+    rc = launch<T, G, 16>(q, pages, a, p, out, s);
   }
   if (rc != CTI_OK || p.splits == 1) return rc;
   return launch_join<T, G>(a, p.splits, out, s);

@@ -17,8 +17,8 @@
 // All operands are fp16, whatever T: keys and values are unpacked to 11 bits
 // after a scaling by a power of two, common to a page, that is 1 unless the
 // page's magnitudes are all below 2^-3 or come near 2^15 (then their bound goes
-// to 2^14, so that small values beside large ones keep their bits), and P is rounded to
-// 11 bits, so that in bf16 the output's own rounding is nearly all of the
+// to 2^14, so that small values beside large ones keep their bits), and P is
+// rounded to 11 bits, so that in bf16 the output's own rounding is nearly all of the
 // error.  The scores take the keys' scaling back; the values' enters P's
 // exponents (m follows score + scaling) and is taken off the sum l; beside
 // values 2^k above 2^15 with a weight of note, those of other pages keep k bits
@@ -52,7 +52,7 @@ struct Shape {
   static constexpr int kStages = G == 4 ? (TILES == 2 ? 3 : 2) : G == 2 ? 3 : 4;
   static constexpr int kRaw = G == 4 && TILES == 1 ? 1 : 3;  // page blocks in flight
   static constexpr int kSoftmaxWarps = 4 * TILES;
-  static constexpr int kUnpackWarps = TILES == 2 && G > 1 ? 8 : 4;
+  static constexpr int kUnpackWarps = TILES == 2 ? 8 : 4;
   static constexpr int kThreads = (kSoftmaxWarps + kUnpackWarps + 2) * 32;
   static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
   // Of a tile: two S / P buffers of 64 columns, then O.
@@ -63,7 +63,7 @@ struct Shape {
   static constexpr int kBarBytes = 320;
   static constexpr size_t kSmem =
       1024 + (size_t)TILES * kQBytes + (size_t)kStages * 2 * kKBytes +
-                                  (size_t)kRaw * block_bytes(G) + kInfoBytes + kMetaBytes + kBarBytes;
+      (size_t)kRaw * block_bytes(G) + kInfoBytes + kMetaBytes + kBarBytes;
   static_assert(kSmem <= (TILES == 2 ? 232448 : 115000), "shared memory");
 };
 
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
   uint8_t* sRaw = sKV + (size_t)S * 2 * Z::kKBytes;  // [R] page blocks
   PageInfo* info = reinterpret_cast<PageInfo*>(sRaw + (size_t)R * block_bytes(G));
   uint32_t* sMeta = reinterpret_cast<uint32_t*>(info + S);
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(sMeta + Z::kMetaBytes / 4);  // [S] (unpacking warps)
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(sMeta + Z::kMetaBytes / 4);  // [S]
   uint64_t* kv_empty = kv_full + S;                           // [S] PV of every tile done
   uint64_t* q_full = kv_empty + S;                            // [TILES] (4 softmax warps)
   uint64_t* q_empty = q_full + TILES;                         // [TILES] last S done
@@ -218,8 +218,8 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
   constexpr int kRows = TILES * kTile;
   const int ntiles = (rows + kRows - 1) / kRows;
 
-  // The pages [p0, p0 + np) of this block for the rows from row0 on, and the
-  // keys that some row and that every row sees.
+  // The pages [p0, p0 + np) of this block for the rows from row0 on, the keys
+  // that some row and that every row sees.
   struct Range {
     int p0, np, most, all;
   };
@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
     bool ok = true;
     for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y, ++it) {
       const Range rg = range_of(tile);
+      if (i > 0 && tile * kRows + i * kTile >= rows) break;
       const int row = tile * kRows + i * kTile + r;
       const bool live = row < rows;
       const int tok = live ? (int)a.by_group(row) : 0;
@@ -672,12 +673,17 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
       bool ok = true, any = false;
       for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y, ++it) {
         const Range rg = range_of(tile);
-        for (int i = 0; ok && i < TILES; ++i)
-          ok = mbar_wait(&q_full[i], (uint32_t)(it & 1), a.status, 0x730, abort_flag);
+        const int tiles = TILES == 2 && rows - tile * kRows <= kTile ? 1 : TILES;
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+          ok = ok && (i >= tiles || mbar_wait(&q_full[i], (uint32_t)(it & 1), a.status, 0x730,
+                                                 abort_flag));
         for (int j = 0; ok && j < rg.np; ++j, ++g) {
           const int st = g % S, b = g & 1;
           ok = mbar_wait(&kv_full[st], (uint32_t)((g / S) & 1), a.status, 0x731, abort_flag);
-          for (int i = 0; ok && i < TILES; ++i) {
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) {
+            if (!ok || i >= tiles) break;
             // The buffer's last reader is the PV of page g - 2.
             ok = mbar_wait(&pv_done[2 * i + b], (uint32_t)((g >> 1) & 1) ^ 1u, a.status, 0x732,
                            abort_flag);
@@ -716,9 +722,12 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
       bool ok = true, any = false;
       for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y, ++it) {
         const Range rg = range_of(tile);
+        const int tiles = TILES == 2 && rows - tile * kRows <= kTile ? 1 : TILES;
         for (int j = 0; ok && j < rg.np; ++j, ++g) {
           const int st = g % S, b = g & 1;
-          for (int i = 0; ok && i < TILES; ++i) {
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) {
+            if (!ok || i >= tiles) break;
             if (j == 0)  // the last tile's O has been read
               ok = mbar_wait(&o_empty[i], (uint32_t)(it & 1) ^ 1u, a.status, 0x740, abort_flag);
             ok = ok && mbar_wait(&p_full[2 * i + b], (uint32_t)((g >> 1) & 1), a.status, 0x741,
@@ -738,9 +747,10 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             umma_commit(&kv_empty[st]);
             any = true;
           }
+          for (int i = tiles; ok && i < TILES; ++i) mbar_arrive(&kv_empty[st]);
         }
         // A tile without pages leaves O alone, but its turn counts.
-        for (int i = 0; ok && rg.np == 0 && i < TILES; ++i)
+        for (int i = 0; ok && rg.np == 0 && i < tiles; ++i)
           ok = mbar_wait(&o_empty[i], (uint32_t)(it & 1) ^ 1u, a.status, 0x742, abort_flag);
       }
       if (any) {
@@ -777,8 +787,9 @@ int launch(const void* q, const void* pages, const Args& a, int64_t y, int split
 template <typename T, int G>
 int launch_shape(const void* q, const void* pages, const Args& a, int tiles, int64_t y, int splits,
                  void* out, cudaStream_t s) {
-  return tiles == 2 ? launch<T, G, 2>(q, pages, a, y, splits, out, s)
-                    : launch<T, G, 1>(q, pages, a, y, splits, out, s);
+  if constexpr (G > 1)
+    if (tiles == 2) return launch<T, G, 2>(q, pages, a, y, splits, out, s);
+  return launch<T, G, 1>(q, pages, a, y, splits, out, s);
 }
 
 template <typename T>
