@@ -119,6 +119,31 @@ def test_pieces_of_any_size_fill_the_cache_as_one_call_does(cuda_device, dtype):
     assert torch.equal(other.pages, s.cache.pages)
 
 
+@pytest.mark.parametrize("H,D,tokens", [(9, 32, 77000), (9, 128, 19200), (3, 64, 3000),
+                                        (1, 32, 5000), (2, 128, 1500)])
+def test_many_sequences_of_any_lengths(cuda_device, H, D, tokens):
+    """Calls large and small, with runs of empty sequences and of single tokens longer than a warp
+    is wide; then the ends of the sequences alone, from odd tokens on."""
+    from cti_b200 import _lib, ops
+
+    g = torch.Generator().manual_seed(H + D)
+    lens = [0] * 40 + [1] * 70 + [0] * 33 + [2, 0, 64, 129]
+    while sum(lens) < tokens:
+        lens.append(int(torch.randint(0, 200, (), generator=g)) if len(lens) % 5 else 0)
+    lens += [0] * 35
+    s = Setup(cuda_device, lens, lens, H, H, D, torch.bfloat16, seed=D)
+    k, v = ops.kv4_read(s.cache, s.cu, s.lens, s.table, sum(lens))
+    _check_read(k, s.k)
+    _check_read(v, s.v)
+    some = [n // 2 for n in lens]
+    cu = ref.offsets(some)
+    ends = torch.tensor(lens).cumsum(0).tolist()
+    rows = torch.tensor([e - n + j for e, n in zip(ends, some) for j in range(n)])
+    ks, vs = ops.kv4_read(s.cache, cu.to(cuda_device), s.lens, s.table, sum(some))
+    _lib.raise_on_status(cuda_device)
+    assert torch.equal(ks.cpu(), k.cpu()[rows]) and torch.equal(vs.cpu(), v.cpu()[rows])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_values_on_and_next_to_the_borders_between_codes(cuda_device, dtype):
     """Groups whose values lie exactly on s (n + 1/2) + b (ties go to the even code) and one step of
@@ -234,6 +259,13 @@ def test_single_tokens(cuda_device, dtype, H, Hkv, D):
     a = s.check(max_new=1)
     b = s.check(causal=False)
     assert torch.equal(a, b)  # a sequence's last token sees all of it either way
+
+
+def test_more_sequences_than_warps(cuda_device):
+    """A warp for a sequence's head, over up to 12 pages."""
+    g = torch.Generator().manual_seed(17)
+    total = [int(torch.randint(1, 740, (), generator=g)) for _ in range(240)]
+    Setup(cuda_device, [1] * 240, total, 16, 16, 32, torch.bfloat16, seed=18).check()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
