@@ -634,8 +634,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
           if (row >= rows) continue;
           const int i = (int)a.by_group(row);
           const int64_t at = (int64_t)(begin + i) * a.heads + kvh * group + row - i * group;
+          const float inv = l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e];
           if (gridDim.z == 1) {
-            const float inv = l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e];
 #pragma unroll
             for (int g = 0; g < G; ++g)
               *reinterpret_cast<uint2*>(out + at * D + 32 * g + 4 * r8) =
@@ -651,8 +651,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
 #pragma unroll
               for (int g = 0; g < G; ++g)
                 *reinterpret_cast<float4*>(a.ws_o + ws * D + 32 * g + 4 * r8) =
-                    make_float4(o[n][2 * g][e], o[n][2 * g][2 + e], o[n][2 * g + 1][e],
-                                o[n][2 * g + 1][2 + e]);
+                    make_float4(o[n][2 * g][e] * inv, o[n][2 * g][2 + e] * inv,
+                                o[n][2 * g + 1][e] * inv, o[n][2 * g + 1][2 + e] * inv);
             }
           }
         }
@@ -666,7 +666,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
   }
 }
 
-// Joins the splits of every row: a block per row, whose warps share the splits.
+// Joins the splits of every row, each with its own O / l, m and l: a block per
+// row, whose warps share the splits.
 // Bound by latency (the rows of a call with splits are few): every warp finds
 // all weights, 32 splits at a time, then sums its own splits with independent
 // loads.
@@ -699,8 +700,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   for (int i = 0; i < 4; ++i) {
     if (32 * i >= splits) break;
     // No key of the split is seen where l is 0: its rows were not written.
-    const float w = ml[i].y == 0.0f ? 0.0f : ml[i].x == mm ? 1.0f : ex2_approx(ml[i].x - mm);
-    l += ml[i].y * w;
+    const float w =
+        ml[i].y == 0.0f ? 0.0f : ml[i].y * (ml[i].x == mm ? 1.0f : ex2_approx(ml[i].x - mm));
+    l += w;
 #pragma unroll 8
     for (int z = warp; z < min(32, splits - 32 * i); z += kJoinWarps) {
       const float wz = __shfl_sync(0xffffffffu, w, z);

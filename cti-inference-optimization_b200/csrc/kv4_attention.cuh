@@ -41,8 +41,8 @@ struct Args {
   Divisor by_group, by_kv_heads;
   int shared;          // a block's warps share a row tile; else each has its own
   int chunk;           // pages of a sequence for a block (gridDim.z > 1)
-  float* ws_o;         // [splits][tokens * heads][D]; splits > 1 only
-  float2* ws_ml;       // [splits][tokens * heads]
+  float* ws_o;         // [splits][tokens * heads][D], O / l; splits > 1 only
+  float2* ws_ml;       // [splits][tokens * heads], m and l
   int32_t* status;
 };
 

@@ -14,15 +14,16 @@
 //          swizzled layout of the matrix operands.  Two tiles share the work.
 //   1 warp issues S = Q K^T (M 128, N 64), 1 warp O += P V with P from TMEM and
 //          V as an MN-major operand.
-// All operands are fp16, whatever T: keys and values are unpacked to 11 bits
-// after a scaling by a power of two, common to a page, that is 1 unless the
-// page's magnitudes are all below 2^-3 or come near 2^15 (then their bound goes
-// to 2^14, so that small values beside large ones keep their bits), and P is
-// rounded to 11 bits, so that in bf16 the output's own rounding is nearly all of the
-// error.  The scores take the keys' scaling back; the values' enters P's
-// exponents (m follows score + scaling) and is taken off the sum l; beside
-// values 2^k above 2^15 with a weight of note, those of other pages keep k bits
-// fewer than 24 in P.  Every wait is a bounded mbarrier wait; one that runs out
+// All operands are fp16, whatever T: keys, values and P are rounded to 11 bits,
+// so that in bf16 the output's own rounding is nearly all of the error.  Keys and
+// values are scaled by powers of two first, so that a number keeps its 11 bits
+// down to 2^-25 of its page's largest (values: 2^-17).  A page's keys have a
+// scaling of their own, which its scores take back.  The values' is the one that O
+// is held in, from page to page: it is chosen with the first page (bound of the
+// magnitudes at 2^12) and again where a page's bound leaves 2^6 .. 2^15; then O is
+// multiplied by the difference, which rounds nothing (fp32 holds O while the
+// pages of a sequence's head lie within 2^80 of each other).  So P and the sum l
+// know nothing of it.  Every wait is a bounded mbarrier wait; one that runs out
 // records its site in the status word and the roles unwind.
 //
 // Bound by the unpacking for head_dim 128 (without it 554 us become 400 for
@@ -71,8 +72,7 @@ struct Shape {
 struct alignas(16) PageInfo {
   float scale;        // of its scores: 2^(keys' exponent)
   int keys;           // 64, or 0: not a page
-  float v_exponent;   // its values are held as v 2^-v_exponent
-  float v_down;       // 2^-v_exponent
+  int v_exponent;     // its values are held as v 2^-v_exponent
   uint64_t nan_v[4];  // bit per key: a value that is not finite (pages that some rows see in part)
 };
 
@@ -81,6 +81,9 @@ template <int ROW>
 CTI_DEVICE int swizzle_of(int r) {
   return ROW == 128 ? (r & 7) << 4 : (r >> 1 & 3) << 4;
 }
+
+// 2^e, for -126 <= e <= 127.
+CTI_DEVICE float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // Matrix descriptor of an operand tile, 8-row atoms stacked along its rows: K-major
 // for Q and K, MN-major (each row a key) for V.  The stride field holds an
@@ -295,6 +298,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
       if (lane == 0) mbar_arrive(&q_full[i]);
 
       float m = -INFINITY, l = 0.0f;  // m in powers of 2
+      int unit = 0;                   // O is held in units of 2^unit
       for (int j = 0; j < rg.np; ++j, ++g) {
         const int b = g & 1, st = g % S;
         // kv_full has completed once s_full has; waited for here to see the info.
@@ -344,15 +348,18 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
           }
         }
         const float factor = fmaxf(down * pi.scale, 1e-37f);  // not 0: -inf stays -inf
-        mx = fmaf(fmaxf(mx, mx1), factor, pi.v_exponent);
+        mx = fmaxf(mx, mx1) * factor;
         float corr = 1.0f;
         if (mx - m > kSlack) {
           corr = ex2_approx(m - mx);
           m = mx;
         }
-        if (__any_sync(0xffffffffu, corr != 1.0f)) {
+        const int rise = j > 0 ? pi.v_exponent - unit : 0;  // the same for the block
+        unit = pi.v_exponent;
+        if (rise != 0 || __any_sync(0xffffffffu, corr != 1.0f)) {
           l *= corr;
           if (j > 0) {
+            const float corr_o = corr * power_of_two(-max(-127, min(rise, 126)));
             // O holds the tile's pages up to g - 1: wait for their PV.
             if (!__all_sync(0xffffffffu,
                             mbar_wait(&pv_done[2 * i + (b ^ 1)], (uint32_t)(((g - 1) >> 1) & 1),
@@ -366,12 +373,12 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
               uint32_t o[16];
               tmem_ld_x16_sync(lanes + 128 + 16 * c, o);
 #pragma unroll
-              for (int d = 0; d < 16; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * corr);
+              for (int d = 0; d < 16; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * corr_o);
               tmem_st_32x32b_x16(lanes + 128 + 16 * c, o);
             }
           }
         }
-        const float noff = m == -INFINITY ? 0.0f : pi.v_exponent - m;
+        const float noff = m == -INFINITY ? 0.0f : -m;
         const uint64_t factor2 = f2_pack(factor, factor), noff2 = f2_pack(noff, noff);
         uint64_t sum_a = f2_pack(0.0f, 0.0f), sum_b = sum_a;
 #pragma unroll 1
@@ -399,7 +406,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         if (lane == 0) mbar_arrive(&p_full[2 * i + b]);
         float s0, s1;
         f2_unpack(f2_add(sum_a, sum_b), s0, s1);
-        l = fmaf(s0 + s1, pi.v_down, l);
+        l += s0 + s1;
       }
       if (!ok) break;
       // ---- the rows ----
@@ -410,7 +417,8 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
           break;
         tc_fence_after();
       }
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      // Two factors: their product may leave fp32's range.
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l, up_o = power_of_two(unit);
       const int64_t ws = (int64_t)blockIdx.z * a.tokens * a.heads + at;
 #pragma unroll 1
       for (int c = 0; c < 2 * G; ++c) {
@@ -422,6 +430,9 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
           for (int d = 0; d < 16; ++d) o[d] = 0;
         }
         if (!live) continue;
+#pragma unroll
+        for (int d = 0; d < 16; ++d)
+          o[d] = __float_as_uint(__uint_as_float(o[d]) * inv * up_o);
         if (gridDim.z == 1) {
           uint4* dst = reinterpret_cast<uint4*>(out + at * D + 16 * c);
 #pragma unroll
@@ -429,8 +440,8 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             uint32_t w[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              w[x] = Y::pack(__uint_as_float(o[8 * d + 2 * x]) * inv,
-                             __uint_as_float(o[8 * d + 2 * x + 1]) * inv);
+              w[x] = Y::pack(__uint_as_float(o[8 * d + 2 * x]),
+                             __uint_as_float(o[8 * d + 2 * x + 1]));
             dst[d] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else if (rg.np > 0) {
@@ -467,6 +478,8 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
     for (int tile = blockIdx.y; ok && tile < ntiles; tile += gridDim.y) {
       const Range rg = range_of(tile);
       int ids = 0;
+      // The values' exponent, and the largest it was (INT_MIN: no page has set it).
+      int unit = 0, unit_most = INT_MIN;
       for (int j = 0; j < rg.np; ++j, ++g) {
         if ((j & 31) == 0) {
           ids = j + lane < rg.np ? __ldg(table + rg.p0 + j + lane) : 0;
@@ -508,7 +521,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         // The part's scales and bases: words of (s, b) of a key, or pairs of words
         // (s of two tokens, b of both).  A bound of the page's magnitudes, 31 max
         // s + max |b| (at most 8 times the largest), gives its scaling; all warps
-        // of the part find the same.
+        // of the part find the same, page by page.
         const uint32_t* raw_meta = reinterpret_cast<const uint32_t*>(
             blk + (keys ? k_meta_at(G) : v_meta_at(G)));
         uint32_t most_s = 0, most_b = 0;  // of keys: both in most_s
@@ -540,10 +553,20 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         const float top_b = keys ? Y::high(most_s) : fmaxf(Y::low(most_b), Y::high(most_b));
         const float top = __uint_as_float(__reduce_max_sync(
             0xffffffffu, __float_as_uint(fminf(fmaf(31.0f, top_s, top_b), FLT_MAX))));
-        int e = 0;
-        if (top > 0.0f && (top < 0.125f || top >= 32768.0f))
-          e = max(-100, min((int)(__float_as_uint(top) >> 23) - 127 - 14, 100));  // to 2^14
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        const int top_e = (int)(__float_as_uint(top) >> 23) - 127;
+        int e;
+        if (keys) {
+          e = top > 0.0f ? max(-100, min(top_e - 14, 100)) : 0;  // to 2^14
+        } else {
+          // O in its next unit stays finite while that is not 2^80 below its largest.
+          if (top > 0.0f && (unit_most == INT_MIN || top_e - unit < 6 || top_e - unit >= 15)) {
+            unit = max(-100, min(top_e - 12, 100));
+            if (unit_most != INT_MIN) unit = max(unit, unit_most - 80);
+            unit_most = max(unit, unit_most);
+          }
+          e = unit;
+        }
+        const float down = power_of_two(-e);
         // This warp's own, scaled and as fp16.
         uint32_t* meta = sMeta + (warp - Z::kSoftmaxWarps) * (32 * kVecs);
         uint64_t nan_bits = 0;
@@ -568,7 +591,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         __syncwarp();
         if (keys) {
           if (part == 0 && lane == 0) {
-            info[st].scale = __uint_as_float((uint32_t)(127 + e) << 23);
+            info[st].scale = power_of_two(e);
             info[st].keys = is_page ? kPage : 0;
           }
 #pragma unroll 1
@@ -645,10 +668,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
           if (lane == 0) {
             info[st].nan_v[part] = nan_bits;
             if (kEach == 2) info[st].nan_v[part + 2] = 0;
-            if (part == 0) {
-              info[st].v_exponent = (float)e;
-              info[st].v_down = down;
-            }
+            if (part == 0) info[st].v_exponent = e;
           }
         }
         fence_proxy_async_smem();

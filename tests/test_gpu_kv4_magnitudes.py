@@ -1,0 +1,101 @@
+"""Attention over the 4-bit cache, for values, keys, queries and scales of all magnitudes: the error
+of each row's output as a vector, against the 64-bit form on what the cache holds.
+
+The tolerance.  With e the tensors' type's half step (finfo.eps / 2) and f = 2^-11 fp16's:
+  - up to 96 rows of a KV head (warps): the values and the output are rounded to the type;
+  - from 97 rows on (tiles): the output is rounded to the type, keys, values and weights to fp16.
+Each rounding moves a term of sum_j p_j v_j by at most its half step relative to the term, one
+term's error is independent of the next one's, and so is the terms' own sign: errors of both
+kinds add up as the roots of sums of squares, and the ratio of the two is sqrt(2) e for warps and
+sqrt(e^2 + 3 f^2) for tiles.  (A key's rounding moves a score by its half step times the root of the
+sum of q_d^2 k_d^2 scale^2, about the scores' standard deviation, which these tests keep near 1, and
+a weight as much.)  The rounding errors' mean square is a third of the half step's or less, which
+leaves a factor of sqrt(3) for rows whose terms happen to cancel more than others': 1.5 is used."""
+import math
+
+import pytest
+import torch
+
+import kv4_ref as ref
+from test_gpu_kv4 import TYPES, Setup
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [(2, 2, 32), (4, 2, 64), (2, 1, 128)]
+# New tokens of the sequence: one row, a few, and tiles of 128 rows for all SHAPES.
+TOKENS = [1, 12, 100, 150]
+
+
+def _tolerance(dtype, tiles):
+    e, f = ref.rounding(dtype), 2.0 ** -11
+    return 1.5 * math.sqrt(e * e + 3 * f * f if tiles else 2 * e * e)
+
+
+def _check(s, dtype, tiles, scale=None, causal=True, held=ref.held, **kw):
+    """The largest error of a row, relative to the row."""
+    from cti_b200 import _lib, ops
+
+    D = s.q.shape[2]
+    out = ops.kv4_attention(s.q.to(s.dev), s.cache, s.cu, s.lens, s.table, causal=causal,
+                            scale=scale, **kw)
+    _lib.raise_on_status(s.dev)
+    want, _ = ref.attention(s.q, held(s.k), held(s.v), s.new, s.total, causal,
+                            D ** -0.5 if scale is None else scale)
+    got = out.double().cpu()
+    assert torch.isfinite(got).all()
+    off = ((got - want).norm(dim=-1) / want.norm(dim=-1)).max()
+    assert off <= _tolerance(dtype, tiles), float(off)
+
+
+def _setup(dev, n, total, H, Hkv, D, dtype, size_k=1.0, size_v=1.0, size_q=1.0):
+    """size_k, size_v: of the keys and values, a number or one for each token."""
+    g = torch.Generator().manual_seed(n + total + D)
+    size_k, size_v = (torch.as_tensor(x, dtype=torch.float64).reshape(-1, 1, 1)
+                      for x in (size_k, size_v))
+    k = (torch.randn(total, Hkv, D, generator=g) * size_k).to(dtype)
+    v = (torch.randn(total, Hkv, D, generator=g) * size_v).to(dtype)
+    s = Setup(dev, [n], [total], H, Hkv, D, dtype, k=k, v=v)
+    s.q = (s.q.double() * size_q).to(dtype)
+    return s
+
+
+def _by_page(total, sizes):
+    return torch.tensor(sizes, dtype=torch.float64)[torch.arange(total) // 64 % len(sizes)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("n", TOKENS)
+@pytest.mark.parametrize("total", [400, 2500])
+def test_small_values_beside_a_larger_page_and_a_sink(cuda_device, dtype, H, Hkv, D, n, total):
+    """Values of 0.003, twice that in the first page, and a key whose value is next to nothing and
+    whose score is 6 above the others': the output is what the small weights give."""
+    s = _setup(cuda_device, n, total, H, Hkv, D, dtype,
+               size_v=torch.where(torch.arange(total) < 64, 0.006, 0.003))
+    s.k[3], s.v[3] = 6 / D ** 0.5, 1e-4
+    s.q = (s.q.float() + 1.0).to(dtype)
+    t = Setup(cuda_device, [n], [total], H, Hkv, D, dtype, k=s.k, v=s.v)
+    t.q = s.q
+    _check(t, dtype, n >= 100, max_new=n)
+    _check(t, dtype, n >= 100, max_new=n, causal=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("n", TOKENS)
+@pytest.mark.parametrize("sizes", [[0.002, 0.008], [0.008, 0.002], [700.0, 2800.0],
+                                   [0.02, 50.0, 0.5, 0.02]])
+def test_pages_of_different_magnitudes(cuda_device, dtype, H, Hkv, D, n, sizes):
+    """One range of pages (a sequence of 7) and several (of 40)."""
+    for total in (400, 2500):
+        s = _setup(cuda_device, n, total, H, Hkv, D, dtype, size_v=_by_page(total, sizes))
+        _check(s, dtype, n >= 100, max_new=n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("last", [1, 2, 3])
+def test_small_values_and_a_last_page_of_a_few_tokens(cuda_device, dtype, H, Hkv, D, last):
+    for n in (1, 100, 150):
+        s = _setup(cuda_device, n, 384 + last, H, Hkv, D, dtype, size_v=0.004)
+        _check(s, dtype, n >= 100, max_new=n)
