@@ -26,7 +26,9 @@
 //     b_g) sum(q_g), with the sums of q split into two 16-bit numbers.  So a
 //     score is exact but for fp32 sums and 2^-16 of that term.
 //   P^T = 2^(S^T scale log2e - m), against the row's exponent offset m, which
-//     is raised (and O, l rescaled) only when a score exceeds it by 2^8.
+//     is raised (and O, l rescaled) only when a score exceeds it by 2^8.  In bf16,
+//     whose values may be as large as fp32's, P is 2^20 smaller, so that O stays
+//     below the largest value for 4,096 keys and more.
 //   O^T += V^T P^T with V = (16 + n) s + b by one 16-bit fused multiply-add
 //     per two values, rounded to T once.  P enters as two numbers of T, so its
 //     rounding is left out: the error is V's rounding and the output's, 1.4
@@ -144,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
   constexpr int W = kWarps;
   constexpr int kSlot = slot_bytes(G);
   constexpr float kOffUnit = Y::kShift == 3 ? 1.0f : 0x1p14f;
+  constexpr float kPUnit = Y::kShift == 3 ? -20.0f : 0.0f;  // P's largest exponent, but for kSlack
   constexpr int H = halves(G) ? 2 : 1;  // slots that a page takes
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = warp_id(), lane = lane_id();
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
       most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 2));
       // 2^k with most_q 2^k in [2^14, 2^15)
       int k = 14 + 127 - (int)(__float_as_uint(most_q) >> 23);
-      k = most_q > 0.0f ? max(-100, min(k, 100)) : 0;
+      k = most_q > 0.0f ? max(-113, min(k, 100)) : 0;
       const float up = __uint_as_float((uint32_t)(127 + k) << 23) * (a.negate ? -1.0f : 1.0f);
       float sum_mine = 0.0f;  // of group t4's 32 dims (G = 2: t4 & 1; G = 1: the only one)
 #pragma unroll
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
       off_b[n][0] = G == 4 || t4 < G ? hi2 : t4 < 2 * G ? lo2 : 0u;
       off_b[n][1] = G == 4 ? lo2 : 0u;
       const float mine =
-          fmaxf(a.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - k) << 23), 1e-37f);
+          fmaxf(a.scale_log2 * 0x1p24f * __uint_as_float((uint32_t)(127 - k) << 23), 1e-37f);
       sl[n][0] = __shfl_sync(0xffffffffu, mine, 8 * t4);
       sl[n][1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
     }
@@ -474,7 +477,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) noff[n][e] = m[n][e] == -INFINITY ? 0.0f : -m[n][e] * sl[n][e];
+        for (int e = 0; e < 2; ++e)
+          noff[n][e] = m[n][e] == -INFINITY ? 0.0f : fmaf(-m[n][e], sl[n][e], kPUnit);
       uint4 vw[2];
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
@@ -693,19 +697,25 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
-  float l = 0.0f, o[G];
+  float l = 0.0f, o[G], w[4];
 #pragma unroll
   for (int g = 0; g < G; ++g) o[g] = 0.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (32 * i >= splits) break;
     // No key of the split is seen where l is 0: its rows were not written.
-    const float w =
-        ml[i].y == 0.0f ? 0.0f : ml[i].y * (ml[i].x == mm ? 1.0f : ex2_approx(ml[i].x - mm));
-    l += w;
+    w[i] = ml[i].y == 0.0f ? 0.0f : ml[i].y * (ml[i].x == mm ? 1.0f : ex2_approx(ml[i].x - mm));
+    l += w[i];
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  // Weights that add up to 1, so that the sum does not pass the largest value.
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (32 * i >= splits) break;
 #pragma unroll 8
     for (int z = warp; z < min(32, splits - 32 * i); z += kJoinWarps) {
-      const float wz = __shfl_sync(0xffffffffu, w, z);
+      const float wz = __shfl_sync(0xffffffffu, w[i] * inv, z);
       if (wz == 0.0f) continue;
       const float* src = a.ws_o + ((32 * i + z) * rows + row) * D + lane;
 #pragma unroll
@@ -713,16 +723,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     }
   }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-#pragma unroll
   for (int g = 0; g < G; ++g) part[warp][32 * g + lane] = o[g];
   __syncthreads();
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
     float sum = part[0][d];
 #pragma unroll
     for (int w = 1; w < kJoinWarps; ++w) sum += part[w][d];
-    reinterpret_cast<uint16_t*>(out)[row * D + d] = (uint16_t)Y::bits(sum * inv);
+    reinterpret_cast<uint16_t*>(out)[row * D + d] = (uint16_t)Y::bits(sum);
   }
 }
 

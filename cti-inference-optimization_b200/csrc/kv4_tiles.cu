@@ -274,9 +274,9 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         }
       }
       int k = 14 + 127 - (int)(__float_as_uint(most_q) >> 23);
-      k = most_q > 0.0f ? max(-100, min(k, 100)) : 0;
-      const float up = __uint_as_float((uint32_t)(127 + k) << 23) * (a.negate ? -1.0f : 1.0f);
-      const float down = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+      k = most_q > 0.0f ? max(-113, min(k, 100)) : 0;
+      const float up = power_of_two(k) * (a.negate ? -1.0f : 1.0f);
+      const float down = a.scale_log2 * power_of_two(-k);
       if (!__all_sync(0xffffffffu,
                       mbar_wait(&q_empty[i], (uint32_t)(it & 1) ^ 1u, a.status, 0x710, abort_flag)))
         break;
@@ -556,11 +556,11 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         const int top_e = (int)(__float_as_uint(top) >> 23) - 127;
         int e;
         if (keys) {
-          e = top > 0.0f ? max(-100, min(top_e - 14, 100)) : 0;  // to 2^14
+          e = top > 0.0f ? max(-116, top_e - 14) : 0;  // to 2^14
         } else {
           // O in its next unit stays finite while that is not 2^80 below its largest.
           if (top > 0.0f && (unit_most == INT_MIN || top_e - unit < 6 || top_e - unit >= 15)) {
-            unit = max(-100, min(top_e - 12, 100));
+            unit = max(-116, top_e - 12);
             if (unit_most != INT_MIN) unit = max(unit, unit_most - 80);
             unit_most = max(unit, unit_most);
           }

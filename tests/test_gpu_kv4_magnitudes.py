@@ -99,3 +99,25 @@ def test_small_values_and_a_last_page_of_a_few_tokens(cuda_device, dtype, H, Hkv
     for n in (1, 100, 150):
         s = _setup(cuda_device, n, 384 + last, H, Hkv, D, dtype, size_v=0.004)
         _check(s, dtype, n >= 100, max_new=n)
+
+
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("n", TOKENS)
+@pytest.mark.parametrize("total", [400, 2500])
+def test_values_at_the_ends_of_the_range(cuda_device, H, Hkv, D, n, total):
+    """Of bf16: values of 1e37, all of one sign, so that their weighted sum before it is divided
+    passes fp32's range; of 1e36 of both signs; and of 1e-34."""
+    for size, mean in ((1e36, 1e37), (1e36, 0.0), (1e-34, 0.0)):
+        s = _setup(cuda_device, n, total, H, Hkv, D, torch.bfloat16, size_v=size)
+        s = Setup(cuda_device, [n], [total], H, Hkv, D, torch.bfloat16, k=s.k,
+                  v=(s.v.double() + mean).bfloat16())
+        _check(s, torch.bfloat16, n >= 100, max_new=n)
+
+
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("n", TOKENS)
+@pytest.mark.parametrize("size_q,size_k", [(1e34, 1e-34), (2e37, 1e-33), (1e-34, 1e34)])
+def test_queries_at_the_ends_of_the_range(cuda_device, H, Hkv, D, n, size_q, size_k):
+    """Of bf16, whose scores are ordinary."""
+    s = _setup(cuda_device, n, 400, H, Hkv, D, torch.bfloat16, size_k=size_k, size_q=size_q)
+    _check(s, torch.bfloat16, n >= 100, scale=D ** -0.5 / (size_q * size_k), max_new=n)
