@@ -54,7 +54,7 @@ namespace {
 
 using namespace kv4;
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 
 // Warps of a block, and blocks of an SM: what registers allow.  The slots of a
 // warp's ring hold pages, or, where those are large, a page's keys or its
@@ -254,10 +254,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
       }
       most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 1));
       most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 2));
-      // 2^k with most_q 2^k in [2^14, 2^15)
-      int k = 14 + 127 - (int)(__float_as_uint(most_q) >> 23);
-      k = most_q > 0.0f ? max(-113, min(k, 100)) : 0;
-      const float up = __uint_as_float((uint32_t)(127 + k) << 23) * (a.negate ? -1.0f : 1.0f);
+      const int k = query_exponent(most_q, a);
+      const float up = power_of_two(k) * a.sign;
       float sum_mine = 0.0f;  // of group t4's 32 dims (G = 2: t4 & 1; G = 1: the only one)
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -283,8 +281,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
       const uint32_t hi2 = Y::pack(16.0f * hi, hi), lo2 = Y::pack(16.0f * lo, lo);
       off_b[n][0] = G == 4 || t4 < G ? hi2 : t4 < 2 * G ? lo2 : 0u;
       off_b[n][1] = G == 4 ? lo2 : 0u;
-      const float mine =
-          fmaxf(a.scale_log2 * 0x1p24f * __uint_as_float((uint32_t)(127 - k) << 23), 1e-37f);
+      const float mine = a.scale_m * power_of_two(min(a.scale_e + 24 - k, 128));
       sl[n][0] = __shfl_sync(0xffffffffu, mine, 8 * t4);
       sl[n][1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
     }
@@ -917,6 +914,8 @@ extern "C" int cti_kv4_attention(const void* q, int64_t q_stride, int dtype,
        workspace_bytes < cti_kv4_attention_workspace_bytes(num_seqs, tokens, max_new, max_kv_len,
                                                            heads, kv_heads, head_dim)))
     return CTI_ERR_INVALID_ARG;
+  int scale_e = 0;
+  const double scale_m = scale == 0.0f ? 1.0 : frexp(fabs((double)scale) * kLog2e, &scale_e);
   const Args a = {cu_seqlens,
                   kv_lens,
                   page_table,
@@ -927,8 +926,9 @@ extern "C" int cti_kv4_attention(const void* q, int64_t q_stride, int dtype,
                   heads,
                   kv_heads,
                   heads / kv_heads,
-                  fmaxf(fabsf(scale) * kLog2e, 1e-30f),
-                  scale < 0.0f,
+                  (float)scale_m,
+                  scale_e,
+                  scale == 0.0f ? 0.0f : copysignf(1.0f, scale),
                   causal,
                   num_pages,
                   q_stride,

@@ -33,8 +33,9 @@ struct Args {
   int num_seqs;
   int tokens;
   int heads, kv_heads, group;
-  float scale_log2;  // |scale| log2(e), at least 1e-30 so that -inf stays -inf
-  int negate;        // scale < 0: the queries' signs are flipped
+  float scale_m;     // |scale| log2(e) = scale_m 2^scale_e
+  int scale_e;
+  float sign;        // of scale, which goes to the queries: 1, -1, or 0
   int causal;
   int64_t num_pages;
   int64_t q_stride;
@@ -45,6 +46,17 @@ struct Args {
   float2* ws_ml;       // [splits][tokens * heads], m and l
   int32_t* status;
 };
+
+// 2^e, for -126 <= e <= 127; infinity for 128.
+CTI_DEVICE float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// The exponent k that queries of at most `most` are scaled by, to 2^14 .. 2^15 in fp16.  Where
+// |scale| 2^-k would leave fp32's normal numbers they stay smaller: a rounding in fp16 is
+// nothing then, even to keys of 2^127.
+CTI_DEVICE int query_exponent(float most, const Args& a) {
+  const int k = 14 + 127 - (int)(__float_as_uint(most) >> 23);
+  return most * fabsf(a.sign) > 0.0f ? max(-113, min(k, min(100, a.scale_e + 126))) : 0;
+}
 
 // Exponent bits of T: set in infinities and NaN.
 template <typename T>

@@ -82,9 +82,6 @@ CTI_DEVICE int swizzle_of(int r) {
   return ROW == 128 ? (r & 7) << 4 : (r >> 1 & 3) << 4;
 }
 
-// 2^e, for -126 <= e <= 127.
-CTI_DEVICE float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
-
 // Matrix descriptor of an operand tile, 8-row atoms stacked along its rows: K-major
 // for Q and K, MN-major (each row a key) for V.  The stride field holds an
 // atom's bytes; the leading one the bytes between the panels of a wide V.
@@ -273,10 +270,9 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             most_q = max3f(most_q, fabsf(Y::low(w[j])), fabsf(Y::high(w[j])));
         }
       }
-      int k = 14 + 127 - (int)(__float_as_uint(most_q) >> 23);
-      k = most_q > 0.0f ? max(-113, min(k, 100)) : 0;
-      const float up = power_of_two(k) * (a.negate ? -1.0f : 1.0f);
-      const float down = a.scale_log2 * power_of_two(-k);
+      const int k = query_exponent(most_q, a);
+      const float up = power_of_two(k) * a.sign;
+      const float down = a.scale_m * power_of_two(min(a.scale_e - k, 128));
       if (!__all_sync(0xffffffffu,
                       mbar_wait(&q_empty[i], (uint32_t)(it & 1) ^ 1u, a.status, 0x710, abort_flag)))
         break;
@@ -347,7 +343,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             mx1 = max3f(mx1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
           }
         }
-        const float factor = fmaxf(down * pi.scale, 1e-37f);  // not 0: -inf stays -inf
+        const float factor = fmaxf(down * pi.scale, 1e-37f);  // -inf stays -inf, and 2^37 next to 0
         mx = fmaxf(mx, mx1) * factor;
         float corr = 1.0f;
         if (mx - m > kSlack) {

@@ -121,3 +121,18 @@ def test_queries_at_the_ends_of_the_range(cuda_device, H, Hkv, D, n, size_q, siz
     """Of bf16, whose scores are ordinary."""
     s = _setup(cuda_device, n, 400, H, Hkv, D, torch.bfloat16, size_k=size_k, size_q=size_q)
     _check(s, torch.bfloat16, n >= 100, scale=D ** -0.5 / (size_q * size_k), max_new=n)
+
+
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("n", TOKENS)
+def test_scale_of_zero_and_next_to_it(cuda_device, H, Hkv, D, n):
+    """A scale of zero weighs all keys alike, whatever their size; one of 1e-36 belongs to keys, or
+    queries, of 1e36, and one of 1e-42, below fp32's normal numbers, to both."""
+    for size_q, size_k, scale in ((1e10, 1e30, 0.0), (1.0, 1e36, 1e-36), (3e30, 3e5, 1e-36),
+                                  (1e20, 1e22, 1e-42), (1e-20, 1e30, -1e-10)):
+        s = _setup(cuda_device, n, 400, H, Hkv, D, torch.bfloat16, size_k=size_k, size_q=size_q)
+        scale *= D ** -0.5
+        # fp32's numbers below 1e-38 have few bits: the scale that the call is given
+        scale = float(torch.tensor(scale, dtype=torch.float32))
+        _check(s, torch.bfloat16, n >= 100, scale=scale, max_new=n)
+        _check(s, torch.bfloat16, n >= 100, scale=scale, max_new=n, causal=False)
