@@ -12,8 +12,9 @@
 // the 16 s already taken off; that moves the grid by half a unit of T in b at
 // most, as much as the group's values were rounded by when they became T's.
 // A constant group has s = 0 and is held exactly.  A group with
-// a value that is not finite, or whose b is not, has s = b = NaN: all of it
-// reads back as NaN.
+// a value that is not finite, or whose b or 31 s + b in T is not, has s = b =
+// NaN: all of it reads back as NaN.  (So every code of a group that has no NaN
+// stands for a finite number, and p = 0 leaves out all that is masked.)
 //
 // A page holds 64 tokens of every KV head; one head's part of it is one
 // contiguous block of 2560 G bytes, G = head_dim / 32 groups:

@@ -163,7 +163,8 @@ CTI_DEVICE void quantise(const uint4 (&raw)[2], uint32_t (&word)[2], uint32_t& s
   const float s = Y::to_float(s_bits);
   b_bits = Y::bits(fmaf(-16.0f, s, lo));
   const float b = Y::to_float(b_bits);
-  if (!(s >= FLT_MIN && s <= FLT_MAX && fabsf(b) <= FLT_MAX)) {
+  const float top = Y::to_float(Y::bits(fmaf(31.0f, s, b)));  // what the last code stands for
+  if (!(s >= FLT_MIN && s <= FLT_MAX && fabsf(b) <= FLT_MAX && top <= FLT_MAX)) {
     word[0] = word[1] = 0;
     if (s < FLT_MIN) {  // below the smallest normal fp32 number: a constant group
       s_bits = 0;

@@ -363,8 +363,8 @@ int cti_ctr_head(const void* h_bf16, const void* W1_bf16, const float* b1, const
  *   s = T((max - min) / 15),  b = T(min - 16 s),
  *   n = clamp(round((x - b) / s) - 16, 0, 15)   (ties to even; 0 where s = 0)
  * and stand for (16 + n) s + b.  A group with a value that is not finite (or
- * whose b is not: magnitudes above 20,000 in fp16, 1e38 in bf16) stands for
- * NaN as a whole.  head_dim 32, 64 or 128 (CTI_ERR_UNSUPPORTED otherwise).
+ * whose b or 31 s + b is not: from magnitudes of 20,900 in fp16 and 1e38 in
+ * bf16 on where they are of both signs) stands for NaN as a whole.  head_dim 32, 64 or 128 (CTI_ERR_UNSUPPORTED otherwise).
  *
  * pages: num_pages pages of cti_kv4_page_bytes(kv_heads, head_dim) bytes,
  * 16-byte aligned; a page holds CTI_KV4_PAGE_TOKENS tokens of every KV head.

@@ -136,3 +136,34 @@ def test_scale_of_zero_and_next_to_it(cuda_device, H, Hkv, D, n):
         scale = float(torch.tensor(scale, dtype=torch.float32))
         _check(s, torch.bfloat16, n >= 100, scale=scale, max_new=n)
         _check(s, torch.bfloat16, n >= 100, scale=scale, max_new=n, causal=False)
+
+
+@pytest.mark.parametrize("dtype,lo", [(torch.float16, 2161.632), (torch.bfloat16, 1.26258875e37)])
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+def test_a_group_whose_top_code_passes_the_type(cuda_device, dtype, lo, H, Hkv, D):
+    """Values up to the type's largest: the scale's rounding can take the group's top past it.  Such
+    a group is NaN as a whole, and reaches only the rows that see its token."""
+    from cti_b200 import _lib, ops
+
+    total = 200
+    hi = torch.finfo(dtype).max
+    ramp = (lo + (hi - lo) * torch.linspace(0, 1, 32, dtype=torch.float64)).to(dtype)
+    _, s, b = ref.quantise(ramp)
+    top = (31 * s + b).to(dtype)
+    assert torch.isfinite(ramp).all() and torch.isfinite(b) and torch.isinf(top)
+    below = (ramp.double() * 0.98).to(dtype)  # held: its top is within the type
+    _, s, b = ref.quantise(below)
+    assert torch.isfinite((31 * s + b).to(dtype))
+    for n in (12, 150):
+        t = _setup(cuda_device, n, total, H, Hkv, D, dtype)
+        t.v[total - 1, 0, :32], t.k[0, 0, :32], t.v[total - n - 1, Hkv - 1, -32:] = ramp, 0, below
+        t = Setup(cuda_device, [n], [total], H, Hkv, D, dtype, k=t.k, v=t.v)
+        cu = torch.tensor([0, total], dtype=torch.int32, device=cuda_device)
+        _, v = ops.kv4_read(t.cache, cu, t.lens, t.table, total)
+        assert torch.isnan(v[total - 1, 0, :32]).all() and int(torch.isnan(v).sum()) == 32
+        assert not torch.isinf(v).any()
+        out = ops.kv4_attention(t.q.to(cuda_device), t.cache, t.cu, t.lens, t.table, max_new=n)
+        _lib.raise_on_status(cuda_device)
+        out = out.cpu()
+        assert torch.isfinite(out[:n - 1]).all()
+        assert torch.isnan(out[n - 1, :H // Hkv, :32]).all()
