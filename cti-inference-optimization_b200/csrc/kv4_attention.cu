@@ -26,9 +26,10 @@
 //     b_g) sum(q_g), with the sums of q split into two 16-bit numbers.  So a
 //     score is exact but for fp32 sums and 2^-16 of that term.
 //   P^T = 2^(S^T scale log2e - m), against the row's exponent offset m, which
-//     is raised (and O, l rescaled) only when a score exceeds it by 2^8.  In bf16,
-//     whose values may be as large as fp32's, P is 2^20 smaller, so that O stays
-//     below the largest value for 4,096 keys and more.
+//     is raised (and O, l rescaled) only when a score exceeds it by 2^8.  In fp16
+//     P is 2^7 larger, so that weights of 2^-21 of the largest keep their bits (those
+//     below 2^-32 are 0); in bf16, whose values may be as large as fp32's, it is 2^20
+//     smaller, so that O stays below the largest value for 4,096 keys and more.
 //   O^T += V^T P^T with V = (16 + n) s + b by one 16-bit fused multiply-add
 //     per two values, rounded to T once.  P enters as two numbers of T, so its
 //     rounding is left out: the error is V's rounding and the output's, 1.4
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
   constexpr int W = kWarps;
   constexpr int kSlot = slot_bytes(G);
   constexpr float kOffUnit = Y::kShift == 3 ? 1.0f : 0x1p14f;
-  constexpr float kPUnit = Y::kShift == 3 ? -20.0f : 0.0f;  // P's largest exponent, but for kSlack
+  constexpr float kPUnit = Y::kShift == 3 ? -20.0f : kPUnitFp16;  // of weights of 1
   constexpr int H = halves(G) ? 2 : 1;  // slots that a page takes
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = warp_id(), lane = lane_id();

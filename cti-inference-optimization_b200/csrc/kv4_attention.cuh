@@ -11,6 +11,9 @@ constexpr int kSMs = 148;
 // A row's exponent offset m is only raised (and O, l rescaled) when a score
 // exceeds it by this power of 2: p <= 2^kSlack.
 constexpr float kSlack = 8.0f;
+// Exponent that weights of 1 are formed with where P is fp16: 2^kSlack of it are
+// within fp16, and small weights have the most bits.
+constexpr float kPUnitFp16 = 7.0f;
 
 // x / d for 0 <= x < 2^31 by a multiplication and a shift (the round-up
 // method of Granlund and Montgomery).

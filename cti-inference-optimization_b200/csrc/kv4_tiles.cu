@@ -7,8 +7,10 @@
 //   warps 0..3 (and 4..7)  softmax of a tile, thread = row.  They lay the
 //          tile's queries out in shared memory first: fp16, each row scaled by
 //          a power of two.  Per page: the row's 64 scores from TMEM, masked;
-//          p = 2^(x - m), m raised (O and l rescaled) only when a score exceeds
-//          it by 2^8; P in 16 bits back over the scores.
+//          p = 2^(x - m + 7), m raised (O and l rescaled) only when a score
+//          exceeds it by 2^8; P in 16 bits back over the scores.  (The 7 takes p to
+//          fp16's range: weights of 2^-21 of the largest keep 11 bits, those
+//          below 2^-32 are 0.)
 //   4 or 8 warps  unpacking: half of them take a page's keys, half its values,
 //          from a ring of page blocks that bulk copies fill, to 16 bits in the
 //          swizzled layout of the matrix operands.  Two tiles share the work.
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             }
           }
         }
-        const float noff = m == -INFINITY ? 0.0f : -m;
+        const float noff = m == -INFINITY ? 0.0f : kPUnitFp16 - m;
         const uint64_t factor2 = f2_pack(factor, factor), noff2 = f2_pack(noff, noff);
         uint64_t sum_a = f2_pack(0.0f, 0.0f), sum_b = sum_a;
 #pragma unroll 1

@@ -167,3 +167,23 @@ def test_a_group_whose_top_code_passes_the_type(cuda_device, dtype, lo, H, Hkv, 
         out = out.cpu()
         assert torch.isfinite(out[:n - 1]).all()
         assert torch.isnan(out[n - 1, :H // Hkv, :32]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("n", TOKENS)
+@pytest.mark.parametrize("sink", [0, 2400])
+def test_many_small_weights_beside_one_large(cuda_device, dtype, H, Hkv, D, n, sink):
+    """A key of no value has a score 13 above the others' mean, at the sequence's start or near its
+    end: the output comes from 2,500 weights of about 2^-18.8.  fp16 holds 11 bits of a number down
+    to 2^-14, so they are rounded to 11 bits where they are formed 2^4.8 larger, or more.  The
+    queries' first 32 dims are 1, and the key has no others, so its score is the same for all rows;
+    values of 64 keep the output, of about 64 sqrt(2500) 2^-18.8 = 0.007, in fp16's normal range."""
+    total = 2500
+    s = _setup(cuda_device, n, total, H, Hkv, D, dtype, size_k=0.5, size_v=64.0)
+    s.k[sink], s.v[sink] = 0.0, 0.0
+    s.k[sink, :, :32] = 13.0 * D ** 0.5 / 32
+    s.q[..., :32] = 1.0
+    t = Setup(cuda_device, [n], [total], H, Hkv, D, dtype, k=s.k, v=s.v)
+    t.q = s.q
+    _check(t, dtype, n >= 100, max_new=n, causal=False)
