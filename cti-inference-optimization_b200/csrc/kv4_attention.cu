@@ -170,6 +170,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
   const int len = __ldg(a.kv_lens + s);
   if (begin < 0 || end > a.tokens || end < begin) {
     if (lane == 0) raise_status(a.status, CTI_ERR_INVALID_ARG, s);
+    if (gridDim.z > 1 && blockIdx.z == 0 && blockIdx.y == 0)
+      refuse_rows(a.ws_ml, max(begin, 0), min(end, a.tokens), a.heads, group, kvh);
     return;
   }
   const int n_new = end - begin;
@@ -693,6 +695,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     if (32 * i + lane < splits) ml[i] = a.ws_ml[(32 * i + lane) * rows + row];
     mm = fmaxf(mm, ml[i].x);
   }
+  if (__shfl_sync(0xffffffffu, ml[0].y, 0) < 0.0f) return;  // a refused sequence's
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
   float l = 0.0f, o[G], w[4];

@@ -61,6 +61,19 @@ CTI_DEVICE int query_exponent(float most, const Args& a) {
   return most * fabsf(a.sign) > 0.0f ? max(-113, min(k, min(100, a.scale_e + 126))) : 0;
 }
 
+// A sequence whose offsets lie outside the tokens, or fall, is refused.  Where
+// sequences are split, its rows' l of the first split says so to the join (-1;
+// no other l is negative), which leaves them as they were.  One block of a
+// sequence's KV head calls this.
+static __device__ __noinline__ void refuse_rows(float2* ws_ml, int begin, int end, int heads,
+                                                int group, int kvh) {
+#pragma unroll 1
+  for (int t = begin + (int)threadIdx.x; t < end; t += blockDim.x)
+#pragma unroll 1
+    for (int h = 0; h < group; ++h)
+      ws_ml[(int64_t)t * heads + kvh * group + h] = make_float2(-INFINITY, -1.0f);
+}
+
 // Exponent bits of T: set in infinities and NaN.
 template <typename T>
 struct Inf16;

@@ -784,6 +784,14 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
     tc_fence_after();
     tmem_dealloc(tmem, Z::kTmemCols);
   }
+  if (gridDim.z > 1 && blockIdx.z == 0 && blockIdx.y == 0) {
+    // Here, not where the offsets are first read, so that the roles' registers stay theirs.
+    const int seq = (int)a.by_kv_heads(blockIdx.x);
+    const int from = __ldg(a.cu + seq), to = __ldg(a.cu + seq + 1);
+    if (from < 0 || to > a.tokens || to < from)
+      refuse_rows(a.ws_ml, max(from, 0), min(to, a.tokens), a.heads, a.group,
+                  (int)blockIdx.x - seq * a.kv_heads);
+  }
 }
 
 template <typename T, int G, int TILES>

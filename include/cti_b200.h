@@ -378,7 +378,9 @@ int cti_ctr_head(const void* h_bf16, const void* W1_bf16, const float* b1, const
  * uses.
  * A position or page outside its buffer raises CTI_ERR_BOUNDS in `status`
  * (detail: the sequence) and is left out: not written, read as zeros, or not
- * attended to.  Rows of no sequence are left as they were.
+ * attended to.  cu_seqlens that do not lie in 0 .. tokens, or fall, are not
+ * sequences: cti_kv4_attention raises CTI_ERR_INVALID_ARG for those.  Rows of
+ * no sequence are left as they were.
  * ---------------------------------------------------------------------- */
 #define CTI_KV4_PAGE_TOKENS 64
 size_t cti_kv4_page_bytes(int kv_heads, int head_dim);

@@ -1,0 +1,56 @@
+"""How attention over the 4-bit cache is shared among warps and blocks: each page counts once and
+wholly, whatever the split; nothing of the workspace is used that the call did not write; rows of
+a sequence that is refused are left as they were."""
+import pytest
+import torch
+
+import kv4_ref as ref
+from test_gpu_kv4 import Setup
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [(2, 2, 32), (4, 2, 64), (4, 1, 128)]
+
+
+def _call(s, q, cu, lens, table, max_new, max_kv_len, fill, out=None, splits=True, causal=1):
+    """The C entry point with a workspace of `fill` bytes."""
+    from cti_b200 import _lib, ops
+
+    T, H, D = q.shape
+    c = s.cache
+    n = lens.numel()
+    need = _lib.lib.cti_kv4_attention_workspace_bytes(n, T, max_new, max_kv_len, H, c.kv_heads, D)
+    assert (need > 0) == splits
+    ws = torch.full((max(need, 256),), fill, dtype=torch.uint8, device=q.device)
+    out = torch.full_like(q, 7.0) if out is None else out
+    rc = _lib.lib.cti_kv4_attention(
+        q.data_ptr(), H * D, c.dtype_code, cu.data_ptr(), lens.data_ptr(), table.data_ptr(),
+        table.stride(0), table.shape[1], n, T, max_new, max_kv_len, H, c.kv_heads, D, D ** -0.5,
+        causal, c.pages.data_ptr(), c.num_pages, out.data_ptr(), ws.data_ptr(), need,
+        _lib.status_word(q.device).data_ptr(), torch.cuda.current_stream(q.device).cuda_stream)
+    assert rc == _lib.CTI_OK
+    assert ops.PAGE_TOKENS == 64
+    return out
+
+
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("n", [1, 9, 140])
+@pytest.mark.parametrize("fill", [0x3f, 0xff])
+def test_rows_of_a_refused_sequence_are_left_as_they_were(cuda_device, H, Hkv, D, n, fill):
+    """Offsets that pass the tokens, or start before them, with split sequences."""
+    from cti_b200 import _lib
+
+    dev = cuda_device
+    s = Setup(dev, [n, n], [4000, 4000], H, Hkv, D, torch.bfloat16, seed=n)
+    q = s.q.to(dev)
+    max_kv = 4000
+    good = _call(s, q, s.cu, s.lens, s.table, n, max_kv, fill)
+    _lib.raise_on_status(dev)
+    s.compare(good)
+    for cu, kept in (([0, n, 2 * n + 5], slice(n, 2 * n)), ([-3, n, 2 * n], slice(0, n))):
+        cu = torch.tensor(cu, dtype=torch.int32, device=dev)
+        out = _call(s, q, cu, s.lens, s.table, n, max_kv, fill)
+        assert _lib.read_status(dev)[0] == _lib.CTI_ERR_INVALID_ARG
+        assert (out[kept] == 7.0).all()
+        other = slice(0, n) if kept.start else slice(n, 2 * n)
+        assert torch.equal(out[other], good[other])
