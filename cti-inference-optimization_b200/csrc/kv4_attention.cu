@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(G, (ROWS + 7) / 8))
             if (r8 == 0)
               a.ws_ml[ws] = make_float2(m[n][e] == -INFINITY ? -INFINITY : m[n][e] * sl[n][e],
                                         l[n][e]);
-            if (np > 0 || shared) {  // else the row is empty, and not read
+            if (np > 0) {  // else the block has no pages (the first warp's come first)
 #pragma unroll
               for (int g = 0; g < G; ++g)
                 *reinterpret_cast<float4*>(a.ws_o + ws * D + 32 * g + 4 * r8) =
@@ -745,6 +745,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 //   1 sequence of 8 KV heads:  128 rows, 17 and 20 / 17 and 24 / 22 and 34
 constexpr int kTilesFrom = 65, kTilesFromFew = 97;
 
+// Bytes that the splits' outputs may take.  Calls that would need more have rows
+// enough to fill the GPU without so many splits.
+constexpr int64_t kWorkspaceMost = (int64_t)64 << 20;
+
 // How a call is laid out over the GPU; a function of the sizes alone.
 struct Plan {
   int big;             // 128-row tiles of a block (kv4_tiles.cu), 1 or 2; 0: warps as here
@@ -762,6 +766,10 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   const int64_t pages = max_kv_len > 0 ? (max_kv_len + kPage - 1) / kPage : 1;
   Plan p = {};
   const double sequences = (double)num_seqs * kv_heads;
+  const int64_t split_bytes = tokens * heads * (head_dim * (int64_t)sizeof(float) +
+                                                (int64_t)sizeof(float2));
+  int64_t most_splits = (kWorkspaceMost - 512) / split_bytes;  // but for alignment
+  most_splits = most_splits < 1 ? 1 : most_splits > 128 ? 128 : most_splits;
   if (rows >= (sequences >= kSMs / 2 ? kTilesFrom : kTilesFromFew)) {
     // Two tiles share the unpacking of a page, which costs less than one of two
     // blocks' latency hidden by the other, but for head_dim 32 (2,048 rows of 384
@@ -773,7 +781,7 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
     const double blocks = sequences * (double)p.tiles;
     int64_t splits = (int64_t)(kSMs * (3 - p.big) / blocks);
     splits = splits > pages / 8 ? pages / 8 : splits;
-    p.splits = (int)(splits < 1 ? 1 : splits > 128 ? 128 : splits);
+    p.splits = (int)(splits < 1 ? 1 : splits > most_splits ? most_splits : splits);
     p.chunk = (int)((pages + p.splits - 1) / p.splits);
     return p;
   }
@@ -805,8 +813,8 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   int64_t per_warp = ideal > 16 ? 12 : (int64_t)ideal + 1;
   p.chunk = (int)(per_warp * kWarps);
   int64_t splits = (pages + p.chunk - 1) / p.chunk;
-  if (splits > 128) {
-    splits = 128;
+  if (splits > most_splits) {
+    splits = most_splits;
     p.chunk = (int)((pages + splits - 1) / splits);
   }
   p.splits = (int)splits;

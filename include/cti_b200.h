@@ -417,7 +417,8 @@ int cti_kv4_read(const void* pages, int64_t num_pages, int dtype, const int32_t*
  * 2^80 below others of their sequence may count as 0.  tokens * heads
  * and num_seqs * kv_heads below 2^31 - 512 (CTI_ERR_UNSUPPORTED otherwise).
  * workspace: cti_kv4_attention_workspace_bytes(...) bytes, 256-byte aligned
- * (may be NULL where that is 0); contents do not outlive the call. */
+ * (64 MB at most; may be NULL where that is 0); contents do not outlive the
+ * call. */
 size_t cti_kv4_attention_workspace_bytes(int num_seqs, int64_t tokens, int max_new,
                                          int64_t max_kv_len, int heads, int kv_heads,
                                          int head_dim);

@@ -54,3 +54,19 @@ def test_rows_of_a_refused_sequence_are_left_as_they_were(cuda_device, H, Hkv, D
         assert (out[kept] == 7.0).all()
         other = slice(0, n) if kept.start else slice(n, 2 * n)
         assert torch.equal(out[other], good[other])
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(32, 8, 128), (8, 8, 32)])
+@pytest.mark.parametrize("n", [1, 8])
+def test_one_long_history_among_many_short_ones(cuda_device, H, Hkv, D, n):
+    """A bound that one sequence needs, and a table as wide: most splits have no pages, and the
+    workspace holds NaN where they would be."""
+    from cti_b200 import _lib
+
+    total = [9000] + [n + i % 90 for i in range(40)]
+    s = Setup(cuda_device, [n] * len(total), total, H, Hkv, D, torch.bfloat16, seed=D)
+    out = _call(s, s.q.to(cuda_device), s.cu, s.lens, s.table, n, 9000, 0xff)
+    _lib.raise_on_status(cuda_device)
+    s.compare(out)
+    need = _lib.lib.cti_kv4_attention_workspace_bytes(len(total), sum(s.new), n, 9000, H, Hkv, D)
+    assert need <= 64 << 20
