@@ -16,6 +16,7 @@ import math
 import pytest
 import torch
 
+import kv4_pages as pages
 import kv4_ref as ref
 from test_gpu_kv4 import TYPES, Setup
 
@@ -187,3 +188,18 @@ def test_many_small_weights_beside_one_large(cuda_device, dtype, H, Hkv, D, n, s
     t = Setup(cuda_device, [n], [total], H, Hkv, D, dtype, k=s.k, v=s.v)
     t.q = s.q
     _check(t, dtype, n >= 100, max_new=n, causal=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", [(8, 8, 32), (6, 3, 64), (8, 2, 128)])
+@pytest.mark.parametrize("new,total", pages.CALLS)
+def test_ordinary_values(cuda_device, dtype, H, Hkv, D, new, total):
+    """Numbers near 1, long and short, few rows and many, for every bound of the work."""
+    g = torch.Generator().manual_seed(sum(total) + D)
+    k, v = (torch.randn(sum(total), Hkv, D, generator=g).to(dtype) for _ in range(2))
+    s = Setup(cuda_device, new, total, H, Hkv, D, dtype, k=k, v=v)
+    for max_new in (max(new), 1, 200):
+        # Tiles may be taken from 65 rows on or from 97: the larger of both kernels' bounds.
+        tiles = dtype == torch.float16 and max_new * H // Hkv >= 65
+        _check(s, dtype, tiles, max_new=max_new)
+        _check(s, dtype, tiles, max_new=max_new, causal=False)

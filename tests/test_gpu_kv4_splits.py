@@ -4,7 +4,7 @@ a sequence that is refused are left as they were."""
 import pytest
 import torch
 
-import kv4_ref as ref
+import kv4_pages as pages
 from test_gpu_kv4 import Setup
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +70,37 @@ def test_one_long_history_among_many_short_ones(cuda_device, H, Hkv, D, n):
     s.compare(out)
     need = _lib.lib.cti_kv4_attention_workspace_bytes(len(total), sum(s.new), n, 9000, H, Hkv, D)
     assert need <= 64 << 20
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,Hkv,D", [(8, 8, 32), (4, 2, 64), (4, 1, 128), (4, 4, 128)])
+@pytest.mark.parametrize("new,total", pages.CALLS)
+def test_every_page_counts_once(cuda_device, dtype, H, Hkv, D, new, total):
+    """Whatever the bounds say of the work: no split, splits of other sizes, tiles or not."""
+    from cti_b200 import _lib, ops
+
+    s = Setup(cuda_device, new, total, H, Hkv, D, dtype, v=pages.values(total, Hkv, D, dtype))
+    q = s.q.to(cuda_device)
+    for causal in (True, False):
+        want, tol = pages.expected(s.v, H, new, total, causal)
+        for max_new in (max(new), 1, 200):
+            for max_kv_len in (None, max(total), 64, 100000):
+                out = ops.kv4_attention(q, s.cache, s.cu, s.lens, s.table, max_new, causal, 0.0,
+                                        max_kv_len)
+                off = ((out.double().cpu() - want).abs() / tol).max()
+                assert off <= 1, (causal, max_new, max_kv_len, float(off))
+    _lib.raise_on_status(cuda_device)
+
+
+def test_every_page_counts_once_with_a_warp_for_each(cuda_device):
+    """More heads of sequences than warps, up to 12 pages each."""
+    from cti_b200 import _lib, ops
+
+    total = [1 + 37 * i % 760 for i in range(450)]
+    new = [1] * len(total)
+    v = pages.values(total, 8, 32, torch.bfloat16)
+    s = Setup(cuda_device, new, total, 8, 8, 32, torch.bfloat16, v=v)
+    out = ops.kv4_attention(s.q.to(cuda_device), s.cache, s.cu, s.lens, s.table, 1, scale=0.0)
+    _lib.raise_on_status(cuda_device)
+    want, tol = pages.expected(v, 8, new, total, True)
+    assert ((out.double().cpu() - want).abs() <= tol).all()
