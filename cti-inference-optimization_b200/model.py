@@ -295,17 +295,27 @@ class CTRModel(nn.Module):
     def predict_cached(self, batch: dict, cache: SequenceCache, seqs) -> torch.Tensor:
         """CTR probabilities [T] (fp32) of new tokens alone: ``batch`` is the flat
         layout of the new tokens, ``user_offsets`` packing those of sequence
-        ``seqs[i]`` of the cache.  Equals ``predict`` over the whole sequences, at
-        the new tokens, but for the 4 bits that keys and values are held in."""
+        ``seqs[i]`` of the cache; tokens before the first offset and from the last
+        on belong to none and are not scored (NaN).  Equals ``predict`` over the
+        whole sequences, at the new tokens, but for the 4 bits that keys and values
+        are held in."""
         uo = batch["user_offsets"].tolist()
         if len(uo) != len(seqs) + 1:
             raise ValueError("user_offsets must hold one more entry than seqs")
-        if uo[-1] == uo[0]:
-            return torch.empty(0, dtype=torch.float32, device=cache.device)
-        x = self.rep_encoder(batch)
+        T = batch["_flat_row_offsets"].numel() // self.rep_encoder.slot_num - 1
+        if uo[0] < 0 or uo[-1] > T or any(b < a for a, b in zip(uo[:-1], uo[1:])):
+            raise ValueError(f"user_offsets must not fall, from 0 to {T} at most, got {uo}")
         extension = cache.extend(seqs, [b - a for a, b in zip(uo[:-1], uo[1:])])
-        h, _ = self.seq_encoder(x, extension)
-        return self.head(h, want_logits=False)[1]
+        probs = torch.full((T,), float("nan"), device=cache.device)
+        if uo[-1] == uo[0]:
+            return probs
+        x = self.rep_encoder(batch)
+        h, _ = self.seq_encoder(x[uo[0]:uo[-1]], extension)
+        scored = self.head(h, want_logits=False)[1]
+        if scored.numel() == T:
+            return scored
+        probs[uo[0]:uo[-1]] = scored
+        return probs
 
     @torch.no_grad()
     def predict_host(self, batch: dict, chunks: int = 8,

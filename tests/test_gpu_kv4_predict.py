@@ -1,0 +1,100 @@
+"""predict_cached: it scores the tokens that user_offsets name, for the sequences that are named, and
+leaves the cache as it was where it raises.  Its scores are those of the model's parts called one
+after the other, bit for bit; each layer's attention is held to the 64-bit form elsewhere."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+LENS = [40, 100, 17]
+
+
+@pytest.fixture(scope="module")
+def setting(cuda_device):
+    from cti_b200 import synth
+    from cti_b200.model import build_ctr_model
+
+    bb = synth.bag_batch(batch=sum(LENS) + 20, seed=4, vocab_hi=2e4)
+    model = build_ctr_model(bb.vocab.tolist(), num_layers=2, num_experts=8, dim_ff=256)
+    synth.init_ctr_model(model)
+    with torch.no_grad():
+        model.rep_encoder.emb.weight = torch.nn.Parameter(
+            synth.embedding_table(bb.total_rows, 64, seed=1), requires_grad=False)
+        # Larger weights than a model starts with: histories matter.
+        for layer in model.seq_encoder.qkv_proj:
+            layer.weight.mul_(8)
+    model.to(cuda_device).prepare_for_inference()
+    return model, bb
+
+
+def _batch(bb, ranges, user_offsets):
+    """The flat layout of some token ranges."""
+    offs = bb.row_offsets.view(bb.features, -1)
+    vals, ro, vo, start = [], [], [], 0
+    for f in range(bb.features):
+        base = int(bb.val_offsets[f])
+        pieces = [bb.values[base + int(offs[f, a]):base + int(offs[f, b])] for a, b in ranges]
+        counts = torch.cat([offs[f, a + 1:b + 1] - offs[f, a:b] for a, b in ranges])
+        ro.append(torch.cat([torch.zeros(1, dtype=torch.int64), torch.cumsum(counts, 0)]))
+        vals.append(torch.cat(pieces))
+        vo.append(start)
+        start += vals[-1].numel()
+    return {"_flat_values": torch.cat(vals), "_flat_row_offsets": torch.cat(ro),
+            "_val_offsets": torch.tensor(vo), "user_offsets": torch.tensor(user_offsets)}
+
+
+def _cache(model, **kw):
+    return model.sequence_cache(**{**dict(max_seqs=8, num_pages=10, max_tokens=256), **kw})
+
+
+def _histories(model, bb, cache):
+    """Sequences 5, 0 and 7 with LENS tokens."""
+    cu = [0, 40, 140, 157]
+    return model.predict_cached(_batch(bb, [(0, 157)], cu), cache, [5, 0, 7])
+
+
+def _state(c):
+    return (c.free_pages, [c.length(i) for i in range(c.max_seqs)])
+
+
+def _by_parts(model, batch, cache, seqs, new):
+    x = model.rep_encoder(batch)
+    h, _ = model.seq_encoder(x[:sum(new)], cache.extend(seqs, new))
+    return model.head(h, want_logits=False)[1]
+
+
+def test_scores_are_the_parts_and_depend_on_the_history(setting):
+    from cti_b200 import _lib
+
+    model, bb = setting
+    a, b = _cache(model), _cache(model)
+    first = _histories(model, bb, a)
+    assert torch.equal(first, _by_parts(model, _batch(bb, [(0, 157)], [0]), b, [5, 0, 7], LENS))
+    batch = _batch(bb, [(157, 163)], [0, 1, 4, 6])
+    second = model.predict_cached(batch, a, [7, 5, 0])
+    assert torch.equal(second, _by_parts(model, batch, b, [7, 5, 0], [1, 3, 2]))
+    assert [a.length(s) for s in (5, 0, 7)] == [43, 102, 18]
+    # Other histories, or none, give other scores, for every token.
+    none = model.predict_cached(batch, _cache(model), [7, 5, 0])
+    c = _cache(model)
+    _histories(model, bb, c)
+    other = model.predict_cached(batch, c, [0, 7, 5])
+    _lib.raise_on_status(second.device)
+    assert torch.isfinite(second).all()
+    assert (second != none).all() and (second != other).all()
+
+
+def test_offsets_that_do_not_start_at_the_first_token(setting):
+    """Tokens before, and behind, belong to no sequence: they are not scored."""
+    model, bb = setting
+    a, b = _cache(model), _cache(model)
+    for c in (a, b):
+        _histories(model, bb, c)
+    want = model.predict_cached(_batch(bb, [(159, 164)], [0, 1, 3, 5]), a, [7, 5, 0])
+    got = model.predict_cached(_batch(bb, [(157, 167)], [2, 3, 5, 7]), b, [7, 5, 0])
+    assert got.shape == (10,) and torch.equal(got[2:7], want)
+    assert torch.isnan(got[:2]).all() and torch.isnan(got[7:]).all()
+    assert _state(a) == _state(b)
+    # ... and the keys and values are those tokens'.
+    batch = _batch(bb, [(170, 172)], [0, 1, 2])
+    assert torch.equal(model.predict_cached(batch, a, [5, 0]), model.predict_cached(batch, b, [5, 0]))
