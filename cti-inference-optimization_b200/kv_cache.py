@@ -56,10 +56,11 @@ class SequenceCache:
     ``extend`` makes room for new tokens of some sequences and returns what
     ``TransformerEncoder.forward`` takes as its ``extension``: the forward of
     those tokens appends their keys and values and attends to the sequences'
-    histories.  ``release`` gives a sequence's pages back.  The book-keeping is
-    on the host; ``extend`` copies three small tensors to the device and does
-    not wait for it.  Use one stream for the forwards of one cache, or order
-    them: a released page may be given to the next sequence at once."""
+    histories.  ``undo`` takes an extension back whose forward did not run.
+    ``release`` gives a sequence's pages back.  The book-keeping is on the host;
+    ``extend`` copies three small tensors to the device and does not wait for it.
+    Use one stream for the forwards of one cache, or order them: a page that was
+    given back may go to the next sequence at once."""
 
     def __init__(self, num_layers: int, max_seqs: int, num_pages: int, kv_heads: int,
                  head_dim: int, max_tokens: int, dtype: torch.dtype = torch.bfloat16,
@@ -72,6 +73,8 @@ class SequenceCache:
         self.max_tokens = int(max_tokens)
         self._pages: list[list[int]] = [[] for _ in range(self.max_seqs)]
         self._lens = [0] * self.max_seqs
+        self._last = [0] * self.max_seqs  # the last change of each sequence
+        self._changes = 0
         self._free = list(range(int(num_pages) - 1, -1, -1))
 
     @property
@@ -107,9 +110,12 @@ class SequenceCache:
         need = [-(-t // PAGE_TOKENS) - len(self._pages[s]) for s, t in zip(seqs, totals)]
         if sum(need) > len(self._free):
             raise RuntimeError(f"{sum(need)} pages are needed, {len(self._free)} are free")
+        before = [(s, self._lens[s], len(self._pages[s]), self._last[s]) for s in seqs]
+        self._changes += 1
         for s, t, n in zip(seqs, totals, need):
             self._pages[s] += [self._free.pop() for _ in range(n)]
             self._lens[s] = t
+            self._last[s] = self._changes
         cols = max([len(self._pages[s]) for s in seqs], default=0)
         cu = [0]
         for n in new:
@@ -122,11 +128,29 @@ class SequenceCache:
         n = len(seqs)
         return {"cache": self, "cu_seqlens": flat[:n + 1], "kv_lens": flat[n + 1:2 * n + 1],
                 "page_table": flat[2 * n + 1:].view(n, cols), "max_seqlen": max(new, default=0),
-                "max_kv_len": max(totals, default=0)}
+                "max_kv_len": max(totals, default=0), "tokens": cu[-1],
+                "undo": (self._changes, before)}
+
+    def undo(self, extension: dict) -> None:
+        """Takes back what ``extend`` returned as ``extension``: its sequences have
+        the lengths and pages that they had before.  For a forward that raised;
+        raises ValueError, and changes nothing, where one of the sequences was
+        extended or released since, or the extension taken back."""
+        if extension["cache"] is not self:
+            raise ValueError("the extension is of another cache")
+        change, before = extension["undo"]
+        if any(self._last[s] != change for s, *_ in before):
+            raise ValueError("the extension is not the last change of its sequences")
+        for s, length, pages, last in reversed(before):
+            while len(self._pages[s]) > pages:
+                self._free.append(self._pages[s].pop())
+            self._lens[s], self._last[s] = length, last
 
     def release(self, seqs: Sequence[int]) -> None:
         """Forgets the sequences and frees their pages."""
+        self._changes += 1
         for s in self._check(seqs):
             self._free += reversed(self._pages[s])
             self._pages[s] = []
             self._lens[s] = 0
+            self._last[s] = self._changes

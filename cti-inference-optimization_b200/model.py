@@ -154,6 +154,17 @@ class TransformerEncoder(nn.Module):
         self._qkv = [(l.weight[perm].contiguous(), l.bias[perm].contiguous()) for l in self.qkv_proj]
         self._prepared = (w0.device, w0.dtype)
 
+    def check_cache(self, cache: SequenceCache) -> None:
+        """Raises ValueError where the encoder cannot run on ``cache``."""
+        w = self.qkv_proj[0].weight
+        for what, has, needs in (
+                ("layers", len(cache.layers), self.num_layers),
+                ("heads", cache.layers[0].kv_heads, self.n_heads),
+                ("head_dim", cache.layers[0].head_dim, self.head_dim),
+                ("dtype", cache.layers[0].dtype, w.dtype), ("device", cache.device, w.device)):
+            if has != needs:
+                raise ValueError(f"the cache's {what}: {has}, the encoder's: {needs}")
+
     def _add_norm(self, x, r, norm):
         """(x + r, norm(x + r)) on the fused sm_100a kernel (bf16 rows; the
         kernel raises for widths it does not cover)."""
@@ -171,9 +182,10 @@ class TransformerEncoder(nn.Module):
         T = x.shape[0]
         H, hd = self.n_heads, self.head_dim
         cache = extension.get("cache")
-        if cache is not None and len(cache.layers) != self.num_layers:
-            raise ValueError(f"the cache has {len(cache.layers)} layers, the encoder "
-                             f"{self.num_layers}")
+        if cache is not None:
+            self.check_cache(cache)
+            if T < extension["tokens"]:
+                raise ValueError(f"the extension holds {extension['tokens']} tokens, x {T}")
         mark = extension.get("mark") or (lambda name: None)
         pending = None  # the previous layer's MoE output, not yet added
         for i in range(self.num_layers):
@@ -298,20 +310,25 @@ class CTRModel(nn.Module):
         ``seqs[i]`` of the cache; tokens before the first offset and from the last
         on belong to none and are not scored (NaN).  Equals ``predict`` over the
         whole sequences, at the new tokens, but for the 4 bits that keys and values
-        are held in."""
+        are held in.  Where it raises, the cache is as it was before the call."""
         uo = batch["user_offsets"].tolist()
         if len(uo) != len(seqs) + 1:
             raise ValueError("user_offsets must hold one more entry than seqs")
         T = batch["_flat_row_offsets"].numel() // self.rep_encoder.slot_num - 1
         if uo[0] < 0 or uo[-1] > T or any(b < a for a, b in zip(uo[:-1], uo[1:])):
             raise ValueError(f"user_offsets must not fall, from 0 to {T} at most, got {uo}")
+        self.seq_encoder.check_cache(cache)
         extension = cache.extend(seqs, [b - a for a, b in zip(uo[:-1], uo[1:])])
         probs = torch.full((T,), float("nan"), device=cache.device)
         if uo[-1] == uo[0]:
             return probs
-        x = self.rep_encoder(batch)
-        h, _ = self.seq_encoder(x[uo[0]:uo[-1]], extension)
-        scored = self.head(h, want_logits=False)[1]
+        try:
+            x = self.rep_encoder(batch)
+            h, _ = self.seq_encoder(x[uo[0]:uo[-1]], extension)
+            scored = self.head(h, want_logits=False)[1]
+        except BaseException:
+            cache.undo(extension)
+            raise
         if scored.numel() == T:
             return scored
         probs[uo[0]:uo[-1]] = scored

@@ -98,3 +98,66 @@ def test_offsets_that_do_not_start_at_the_first_token(setting):
     # ... and the keys and values are those tokens'.
     batch = _batch(bb, [(170, 172)], [0, 1, 2])
     assert torch.equal(model.predict_cached(batch, a, [5, 0]), model.predict_cached(batch, b, [5, 0]))
+
+
+def test_a_forward_that_raises_leaves_the_cache_as_it_was(setting, monkeypatch):
+    model, bb = setting
+    a, b = _cache(model), _cache(model)
+    for c in (a, b):
+        _histories(model, bb, c)
+    state = _state(a)
+    batch = _batch(bb, [(157, 177)], [0, 19, 20])
+    for where in ("seq_encoder.moe.1", "seq_encoder.out_proj.0", "rep_encoder"):
+        module = model.get_submodule(where)
+
+        def fails(*args, **kw):
+            raise RuntimeError("out of memory")
+
+        monkeypatch.setattr(module, "forward", fails)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            model.predict_cached(batch, a, [0, 5])
+        monkeypatch.undo()
+        assert _state(a) == state
+    monkeypatch.setattr(model, "head", fails)
+    with pytest.raises(RuntimeError):
+        model.predict_cached(batch, a, [0, 5])
+    monkeypatch.undo()
+    assert _state(a) == state
+    want = model.predict_cached(batch, b, [0, 5])
+    assert torch.equal(model.predict_cached(batch, a, [0, 5]), want)
+    assert _state(a) == _state(b) != state
+
+
+def test_wrong_calls_are_refused_and_change_nothing(setting):
+    import cti_b200
+
+    model, bb = setting
+    enc, dev = model.seq_encoder, model.linear[0].weight.device
+    c = _cache(model)
+    _histories(model, bb, c)
+    state = _state(c)
+    for offsets, seqs, error in (([0, 1, 7], [5, 0], ValueError),   # past the batch's tokens
+                                 ([0, 3, 2], [5, 0], ValueError), ([0, 3, 0], [5, 0], ValueError),
+                                 ([-1, 1, 2], [5, 0], ValueError), ([0, 6], [5, 0], ValueError),
+                                 ([0, 3, 6], [5, 5], ValueError), ([0, 0, 0], [5, 9], IndexError),
+                                 ([0, 3, 6], [5, 8], IndexError)):
+        with pytest.raises(error):
+            model.predict_cached(_batch(bb, [(157, 163)], offsets), c, seqs)
+        assert _state(c) == state
+    batch = _batch(bb, [(157, 163)], [0, 3, 6])
+    args = dict(num_layers=enc.num_layers, max_seqs=8, num_pages=10, kv_heads=enc.n_heads,
+                head_dim=enc.head_dim, max_tokens=256, device=dev)
+    for kw in (dict(num_layers=enc.num_layers + 1), dict(kv_heads=2 * enc.n_heads),
+               dict(kv_heads=max(1, enc.n_heads // 2)), dict(head_dim=128 if enc.head_dim < 128 else 64),
+               dict(dtype=torch.float16), dict(device="cpu")):
+        other = cti_b200.SequenceCache(**{**args, **kw})
+        with pytest.raises(ValueError):
+            model.predict_cached(batch, other, [5, 0])
+        assert _state(other) == (10, [0] * 8)
+    e = c.extend([5], [3])
+    with pytest.raises(ValueError):  # fewer tokens than the extension holds
+        enc(torch.zeros(2, enc.d_model, dtype=torch.bfloat16, device=dev), e)
+    c.undo(e)
+    assert _state(c) == state
+    assert model.predict_cached(_batch(bb, [(157, 163)], [0, 0, 0]), c, [5, 0]).shape == (6,)
+    assert _state(c) == state
