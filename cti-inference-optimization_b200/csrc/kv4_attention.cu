@@ -763,7 +763,9 @@ Plan plan(int num_seqs, int64_t tokens, int max_new, int64_t max_kv_len, int hea
   const int G = head_dim / kGroup;
   const int64_t most = max_new < tokens ? max_new : tokens;
   const int64_t rows = (most > 0 ? most : 1) * (heads / kv_heads);
-  const int64_t pages = max_kv_len > 0 ? (max_kv_len + kPage - 1) / kPage : 1;
+  // No table reaches further, whatever the bound: pages, and a split's first, are ints.
+  const int64_t len = max_kv_len < INT32_MAX ? max_kv_len : INT32_MAX;
+  const int64_t pages = len > 0 ? (len + kPage - 1) / kPage : 1;
   Plan p = {};
   const double sequences = (double)num_seqs * kv_heads;
   const int64_t split_bytes = tokens * heads * (head_dim * (int64_t)sizeof(float) +

@@ -517,7 +517,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
         _kv4_rows(out, "out", cache, H)
         if out.size(0) != T or not out.is_contiguous():
             raise ValueError("out must be contiguous, of q's shape")
-    max_new, max_kv_len = int(max_new), int(max_kv_len)
+    # Bounds may be as large as one likes: the C entry point takes 32 and 64 bits.
+    max_new, max_kv_len = min(int(max_new), T), min(int(max_kv_len), 2 ** 62)
     need = _kv4_workspace_bytes(n, T, max_new, max_kv_len, H, Hkv, hd)
     ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     pages = cache.pages

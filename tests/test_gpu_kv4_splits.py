@@ -104,3 +104,25 @@ def test_every_page_counts_once_with_a_warp_for_each(cuda_device):
     _lib.raise_on_status(cuda_device)
     want, tol = pages.expected(v, 8, new, total, True)
     assert ((out.double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(8, 8, 32), (4, 1, 128)])
+@pytest.mark.parametrize("n", [1, 9, 140])
+def test_bounds_far_past_any_table(cuda_device, H, Hkv, D, n):
+    """max_kv_len and max_new only steer how work is split, also where a split's pages would pass
+    32 bits."""
+    from cti_b200 import _lib, ops
+
+    s = Setup(cuda_device, [n, 2], [3000, 70], H, Hkv, D, torch.bfloat16,
+              v=pages.values([3000, 70], Hkv, D, torch.bfloat16))
+    q = s.q.to(cuda_device)
+    want, tol = pages.expected(s.v, H, s.new, s.total, True)
+    for max_new in (n, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        for max_kv_len in (2 ** 31, 2 ** 37 + 64, 2 ** 40, 2 ** 45 - 1, 2 ** 62, 2 ** 63 - 1, 2 ** 80):
+            out = ops.kv4_attention(q, s.cache, s.cu, s.lens, s.table, max_new, True, 0.0,
+                                    max_kv_len)
+            assert ((out.double().cpu() - want).abs() <= tol).all()
+    _lib.raise_on_status(cuda_device)
+    out = _call(s, q, s.cu, s.lens, s.table, 2 ** 31 - 1, 2 ** 63 - 1, 0xff)
+    _lib.raise_on_status(cuda_device)
+    s.compare(out, causal=True)

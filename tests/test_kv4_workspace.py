@@ -27,3 +27,11 @@ def test_long_sequences_are_still_split():
         assert 0 < _bytes(n, n, 1, 131072, heads, kv_heads, head_dim) <= LIMIT
     assert _bytes(1, 256, 256, 131072, 32, 8, 128) > 0
     assert _bytes(2048, 2048, 1, 100, 8, 8, 32) == 0
+
+
+def test_bounds_past_any_table_are_as_good_as_the_widest():
+    """A table holds 2^31 keys of a sequence at most."""
+    for sizes in ((1, 1, 1), (3, 300, 100), (48, 48, 1)):
+        widest = _bytes(*sizes, 2 ** 31 - 1, 32, 8, 128)
+        for bound in (2 ** 31, 2 ** 37 + 64, 2 ** 40, 2 ** 62, 2 ** 63 - 1):
+            assert _bytes(*sizes, bound, 32, 8, 128) == widest
