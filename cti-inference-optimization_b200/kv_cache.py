@@ -101,6 +101,9 @@ class SequenceCache:
         """Makes room for ``new[i]`` tokens at the end of sequence ``seqs[i]``.
         Raises, and changes nothing, where the pages do not suffice or a
         sequence would pass ``max_tokens``."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("extend cannot be captured into a graph: extend first, then capture "
+                               "the forward of what it returned")
         seqs, new = self._check(seqs), [int(n) for n in new]
         if len(new) != len(seqs) or any(n < 0 for n in new):
             raise ValueError("new must hold a count for each sequence")

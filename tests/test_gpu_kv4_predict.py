@@ -161,3 +161,31 @@ def test_wrong_calls_are_refused_and_change_nothing(setting):
     assert _state(c) == state
     assert model.predict_cached(_batch(bb, [(157, 163)], [0, 0, 0]), c, [5, 0]).shape == (6,)
     assert _state(c) == state
+
+
+def test_extend_is_refused_inside_a_capture(setting):
+    """Its book-keeping would happen once, for every replay; the forward itself can be captured, with
+    the extension's tensors as its inputs."""
+    from cti_b200 import _lib
+
+    model, bb = setting
+    c = _cache(model)
+    _histories(model, bb, c)
+    state = _state(c)
+    enc, dev = model.seq_encoder, c.device
+    x = torch.randn(4, enc.d_model, device=dev).bfloat16()
+    e = c.extend([5, 0], [1, 3])
+    want, _ = enc(x, e)  # warm-up too; the tokens are appended anew by each run, to their places
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(RuntimeError, match="captured"):
+            c.extend([7], [1])
+        got, _ = enc(x, e)
+    for _ in range(2):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        assert torch.equal(got, want)
+    _lib.raise_on_status(dev)
+    assert c.length(7) == state[1][7] and c.length(5) == state[1][5] + 1
