@@ -203,3 +203,26 @@ def test_ordinary_values(cuda_device, dtype, H, Hkv, D, new, total):
         tiles = dtype == torch.float16 and max_new * H // Hkv >= 65
         _check(s, dtype, tiles, max_new=max_new)
         _check(s, dtype, tiles, max_new=max_new, causal=False)
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(4, 2, 64), (2, 1, 128)])
+@pytest.mark.parametrize("n", TOKENS)
+def test_groups_of_different_magnitudes(cuda_device, H, Hkv, D, n):
+    """Values of 1e-5 in one group of dims beside values near 1: their own part of the output is as
+    good as the others'.  So are scores that come from keys of 1e-5 where the queries' dims are
+    1e5, beside keys near 1."""
+    from cti_b200 import _lib, ops
+
+    total = 700
+    size = torch.ones(D, dtype=torch.float64)
+    size[32:64] = 1e-5
+    g = torch.Generator().manual_seed(n + D)
+    k, v = ((torch.randn(total, Hkv, D, generator=g) * size).bfloat16() for _ in range(2))
+    s = Setup(cuda_device, [n], [total], H, Hkv, D, torch.bfloat16, k=k, v=v)
+    s.q = (s.q.double() / size * 0.7).bfloat16()
+    out = ops.kv4_attention(s.q.to(cuda_device), s.cache, s.cu, s.lens, s.table, n)
+    _lib.raise_on_status(cuda_device)
+    want, _ = ref.attention(s.q, ref.held(k), ref.held(v), [n], [total], True, D ** -0.5)
+    off = (out.double().cpu() - want).unflatten(-1, (-1, 32)).norm(dim=-1)
+    off = (off / want.unflatten(-1, (-1, 32)).norm(dim=-1)).max()
+    assert off <= _tolerance(torch.bfloat16, n >= 100), float(off)
