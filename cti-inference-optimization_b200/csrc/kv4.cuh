@@ -38,6 +38,7 @@
 namespace cti {
 namespace kv4 {
 
+constexpr int kSMs = 148;
 constexpr int kPage = 64;   // tokens in a page
 constexpr int kGroup = 32;  // values that share a scale and a base
 
@@ -60,6 +61,8 @@ CTI_DEVICE int k_meta_word_at(int tau, int g, int G) { return (tau * G + g) * 4;
 CTI_DEVICE int v_meta_half_at(int tau, int g, int G) {  // s; b is 4 bytes further
   return ((tau >> 1) * G + g) * 8 + (tau & 1) * 2;
 }
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The two 16-bit types.
 template <typename T>

@@ -97,20 +97,6 @@ struct Mma<__half> {
   }
 };
 
-CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-          "r"(smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
-
-CTI_DEVICE float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 // Word i of a lane's vectors of codes (i is known when the code is compiled).
 template <int N>
 CTI_DEVICE uint32_t word_of(const uint4 (&v)[N], int i) {
@@ -880,8 +866,6 @@ int launch_dim(const void* q, const void* pages, const Args& a, const Plan& p, i
          : head_dim == 64 ? launch_shape<T, 2>(q, pages, a, p, dtype, out, s)
                           : launch_shape<T, 4>(q, pages, a, p, dtype, out, s);
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
 }  // namespace cti

@@ -7,7 +7,6 @@
 namespace cti {
 namespace kv4 {
 
-constexpr int kSMs = 148;
 // A row's exponent offset m is only raised (and O, l rescaled) when a score
 // exceeds it by this power of 2: p <= 2^kSlack.
 constexpr float kSlack = 8.0f;
@@ -72,6 +71,20 @@ static __device__ __noinline__ void refuse_rows(float2* ws_ml, int begin, int en
 #pragma unroll 1
     for (int h = 0; h < group; ++h)
       ws_ml[(int64_t)t * heads + kvh * group + h] = make_float2(-INFINITY, -1.0f);
+}
+
+CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+CTI_DEVICE float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // Exponent bits of T: set in infinities and NaN.

@@ -23,7 +23,6 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kSMs = 148;
 constexpr int kThreads = 256;
 constexpr int kTokens = 128;  // packed tokens of a block, at most
 constexpr int64_t kMaxStride = ((int64_t)1 << 31) / kTokens;
@@ -424,8 +423,6 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The checks that both entry points share.  CTI_OK with *empty set: nothing to do.
 int check_args(const void* k, const void* v, int dtype, int head_dim, const Args& a,

@@ -94,14 +94,6 @@ CTI_DEVICE uint64_t tile_desc(uint32_t saddr, uint32_t panel = 8 * ROW) {
          (uint64_t)1 << 46 | (uint64_t)(ROW == 128 ? 2 : 4) << 61;
 }
 
-CTI_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-          "r"(smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
-
 // The larger of both halves of two numbers of T that are not negative; a NaN
 // counts nothing.
 template <typename T>
@@ -111,12 +103,6 @@ CTI_DEVICE uint32_t max2(uint32_t a, uint32_t b) {
     asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   else
     asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-
-CTI_DEVICE float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
