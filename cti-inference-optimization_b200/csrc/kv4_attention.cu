@@ -40,11 +40,13 @@
 // shared memory; where a sequence is also split over blocks, they go to the
 // workspace and a second kernel joins them.
 //
-// Bound by instructions, the logic pipe's first (a shift or a three-input logic
-// operation takes two cycles of a quarter of an SM): about 1,050 a page and KV
-// head for head_dim 128, 400 for 32, and 490 for a warp's queries and rows.
-// One token, 32 heads on 8 KV heads of 128, 131,071 keys: 43.8 us, 59 % of the
-// copy bandwidth.  2,048 sequences of 136 keys on average, 8 heads of 32: 43.6
+// Bound by instructions and their latency: about 1,050 a page and KV head for
+// head_dim 128, 400 for 32, and 490 for a warp's queries and rows, half of them on
+// the logic pipe (a shift or a three-input logic operation takes two cycles of a
+// quarter of an SM), with 14 to 22 of 64 warps, as registers allow; 56 to 66 % of
+// the issue slots are taken.
+// One token, 32 heads on 8 KV heads of 128, 131,071 keys: 43.4 us, 60 % of the
+// copy bandwidth.  2,048 sequences of 136 keys on average, 8 heads of 32: 43.5
 // us, 32 %.
 #include <cfloat>
 

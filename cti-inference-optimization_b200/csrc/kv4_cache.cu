@@ -11,9 +11,11 @@
 // sectors are written in pieces: 38 us for 25 to append 24,576 tokens of 8 heads
 // of 64, in L2.)
 // Either way moves 4 + 1.25 bytes per pair of a key's and a value's element.
-// Measured, 278,000 tokens of 8 heads of 32: 112 us to append (bound by
-// instructions, 17 for 32 values of a warp; 51 % of the copy bandwidth) and 79
-// us to read back (instructions and latency; 73 %).
+// Measured, 278,000 tokens of 8 heads of 32: 113 us to append (51 % of the copy
+// bandwidth) and 79 us to read back (73 %).  Bound by latency: warps wait for loads
+// first (3.7 cycles an instruction when appending, 5.9 when reading), with 28 and 40 of
+// 64 warps there and 58 and 64 % of the issue slots taken; 17 instructions for 32
+// values of a warp are what appending cannot hide it with.
 #include <cfloat>
 
 #include "kv4.cuh"

@@ -22,7 +22,10 @@ class KV4Cache:
     """The pages of one layer: ``pages`` uint8 [num_pages, kv_heads, bytes] on
     ``device``, 64 tokens of every KV head per page, for keys and values of
     ``dtype`` (bfloat16 or float16) with ``head_dim`` 32, 64 or 128.  A token
-    takes 1.25 * head_dim bytes per KV head, against 4 * head_dim in 16 bits."""
+    takes 1.25 * head_dim bytes per KV head, against 4 * head_dim in 16 bits.
+    Each 32 head dims of a token share a scale and a base of ``dtype``; such a
+    group is NaN as a whole where one value is not finite, or where the base does
+    not fit: from magnitudes of 20,900 in float16 and 1e38 in bfloat16 on."""
 
     def __init__(self, num_pages: int, kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda"):

