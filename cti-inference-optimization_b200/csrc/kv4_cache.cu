@@ -75,8 +75,10 @@ CTI_DEVICE uint32_t min2_nan(uint32_t a, uint32_t b) {
 // looked at again, out of line:
 //   - an end of the group comes out below code 0 or above 15, because b's or
 //     s's rounding moved the grid;
-//   - a was rounded, which takes an |x| far below |b|, where a is -b, and -b
-//     lies on a border: then x's sign decides.
+//   - a was rounded onto a border that x - b does not lie on.  That takes an |x|
+//     below 2^-13 |b| (fp16; bf16: 2^-16), so -b is that close to the border, which is
+//     2^-8 s at most; x's side decides.  (In bf16 borders are multiples of 2^-13 of
+//     b's binade away from -b, too far, unless -b lies on one itself.)
 constexpr float kRound = 12582912.0f;  // 1.5 2^23
 constexpr uint32_t kRoundBits = 0x4b400000u;
 
@@ -188,9 +190,10 @@ CTI_DEVICE void quantise(const uint4 (&raw)[2], uint32_t (&word)[2], uint32_t& s
   float t_lo, t_hi;
   f2_unpack(f2_add(quotient(lo, hi), add2), t_lo, t_hi);
   bool again = t_lo < kRound + 16.0f || t_hi > kRound + 31.0f;
-  // -b on a border: -b / s = a whole number and a half
+  // -b next to a border: -b / s next to a whole number and a half
+  constexpr float kNear = Y::kShift == 3 ? 0.0f : 0x1.01p-8f;
   const float e0 = -b * inv, e1 = fmaf(fmaf(-s, e0, -b), inv, e0);
-  if (fabsf(e1 - ((e1 + kRound) - kRound)) == 0.5f) {
+  if (0.5f - fabsf(e1 - ((e1 + kRound) - kRound)) <= kNear) {
     float least = INFINITY;
 #pragma unroll
     for (int i = 0; i < 16; ++i) least = fminf(least, x[i] == 0.0f ? INFINITY : fabsf(x[i]));
