@@ -60,6 +60,12 @@ class RepEncoder(nn.Module):
         self.register_buffer("table_row_base", torch.tensor(base, dtype=torch.int64), persistent=False)
         self.register_buffer("vocab", torch.tensor(sizes, dtype=torch.int64), persistent=False)
 
+    def tokens(self, batch: dict) -> int:
+        """The tokens of a batch in either layout, without running anything."""
+        if "_flat_values" not in batch:
+            return batch[1][1].numel() - 1
+        return batch["_flat_row_offsets"].numel() // self.slot_num - 1
+
     def pool(self, batch: dict, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The [B, slot_num*emb_dim] sum-pooled embeddings (slot-major columns)."""
         dev = self.emb.weight.device

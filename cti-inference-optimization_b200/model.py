@@ -314,7 +314,7 @@ class CTRModel(nn.Module):
         uo = batch["user_offsets"].tolist()
         if len(uo) != len(seqs) + 1:
             raise ValueError("user_offsets must hold one more entry than seqs")
-        T = batch["_flat_row_offsets"].numel() // self.rep_encoder.slot_num - 1
+        T = self.rep_encoder.tokens(batch)
         if uo[0] < 0 or uo[-1] > T or any(b < a for a, b in zip(uo[:-1], uo[1:])):
             raise ValueError(f"user_offsets must not fall, from 0 to {T} at most, got {uo}")
         self.seq_encoder.check_cache(cache)

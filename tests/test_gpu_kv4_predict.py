@@ -189,3 +189,19 @@ def test_extend_is_refused_inside_a_capture(setting):
         assert torch.equal(got, want)
     _lib.raise_on_status(dev)
     assert c.length(7) == state[1][7] and c.length(5) == state[1][5] + 1
+
+
+def test_batches_by_slot_are_scored_as_flat_ones(setting):
+    """The pooling takes a batch as one (values, offsets) pair for each slot, too."""
+    model, bb = setting
+    a, b = _cache(model), _cache(model)
+    flat = _batch(bb, [(0, 30)], [4, 20, 27])
+    vo = flat["_val_offsets"].tolist() + [flat["_flat_values"].numel()]
+    slots = {i + 1: (flat["_flat_values"][vo[i]:vo[i + 1]],
+                     flat["_flat_row_offsets"].view(bb.features, -1)[i])
+             for i in range(bb.features)}
+    slots["user_offsets"] = flat["user_offsets"]
+    want = model.predict_cached(flat, a, [2, 1])
+    got = model.predict_cached(slots, b, [2, 1])
+    assert torch.equal(got[4:27], want[4:27]) and got.shape == want.shape == (30,)
+    assert _state(a) == _state(b)
