@@ -16,8 +16,15 @@
 //          swizzled layout of the matrix operands.  Two tiles share the work.
 //   1 warp issues S = Q K^T (M 128, N 64), 1 warp O += P V with P from TMEM and
 //          V as an MN-major operand.
-// All operands are fp16, whatever T: keys, values and P are rounded to 11 bits,
-// so that in bf16 the output's own rounding is nearly all of the error.  Keys and
+// All operands are fp16, whatever T.  In bf16 keys, values and P are rounded to 11
+// bits, so that the output's own rounding is nearly all of the error.  In fp16, where
+// each of these would count as much as the output's, keys and values are two numbers
+// each, (16 + n) s' + b and (16 + n) s'' with s' the upper 7 bits of s: both
+// exact, but for groups of one sign, whose first number is rounded.  That leaves
+// P's rounding and the output's: an error of 0.00029 instead of 0.00048 (keys with
+// channels of their own size), for twice the matrix instructions and a half more
+// unpacking (5,600 tokens of 16 heads over 5,700 keys: head_dim 32 298 us, 268
+// with one number; 64: 345 and 331; 128: 600 and 436).  Keys and
 // values are scaled by powers of two first, so that a number keeps its 11 bits
 // down to 2^-25 of its page's largest (values: 2^-17).  A page's keys have a
 // scaling of their own, which its scores take back.  The values' is the one that O
@@ -43,8 +50,10 @@ using namespace kv4;
 
 constexpr int kTile = 128;
 
-template <int G, int TILES>
+template <typename T, int G, int TILES>
 struct Shape {
+  // Keys and values as two numbers each.
+  static constexpr bool kTwo = Type16<T>::kShift != 3;
   static constexpr int D = 32 * G;
   static constexpr int kRow = D >= 64 ? 128 : 64;  // bytes of an operand row: one swizzle span
   static constexpr int kPanels = D > 64 ? 2 : 1;   // that a row of D takes
@@ -52,10 +61,16 @@ struct Shape {
   static constexpr int kQBytes = kPanels * kQPanel;
   static constexpr int kKVPanel = kPage * kRow;
   static constexpr int kKBytes = kPanels * kKVPanel;
-  static constexpr int kStages = G == 4 ? (TILES == 2 ? 3 : 2) : G == 2 ? 3 : 4;
-  static constexpr int kRaw = G == 4 && TILES == 1 ? 1 : 3;  // page blocks in flight
+  static constexpr int kVAt = (kTwo ? 2 : 1) * kKBytes;  // of a stage: keys, then values
+  static constexpr int kStageBytes = 2 * kVAt;
+  // Of an SM.  (One tile of two numbers and 64 dims, 96 sequences of 100 rows over 2,000
+  // keys: 126 us, two blocks with fewer stages 128; 2 sequences: 22 and 26.)
+  static constexpr int kBlocks = TILES == 2 || (kTwo && G >= 2) ? 1 : 2;
+  static constexpr int kStages =
+      G == 4 ? (kTwo || TILES == 1 ? 2 : 3) : G == 2 ? 3 : 4;
+  static constexpr int kRaw = G == 4 && kBlocks == 2 ? 1 : 3;  // page blocks in flight
   static constexpr int kSoftmaxWarps = 4 * TILES;
-  static constexpr int kUnpackWarps = TILES == 2 ? 8 : 4;
+  static constexpr int kUnpackWarps = kBlocks == 1 ? 8 : 4;
   static constexpr int kThreads = (kSoftmaxWarps + kUnpackWarps + 2) * 32;
   static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
   // Of a tile: two S / P buffers of 64 columns, then O.
@@ -65,9 +80,9 @@ struct Shape {
   static constexpr int kMetaBytes = 512 * G;  // scales and bases as fp16, by unpacking warp
   static constexpr int kBarBytes = 320;
   static constexpr size_t kSmem =
-      1024 + (size_t)TILES * kQBytes + (size_t)kStages * 2 * kKBytes +
+      1024 + (size_t)TILES * kQBytes + (size_t)kStages * kStageBytes +
       (size_t)kRaw * block_bytes(G) + kInfoBytes + kMetaBytes + kBarBytes;
-  static_assert(kSmem <= (TILES == 2 ? 232448 : 115000), "shared memory");
+  static_assert(kSmem <= (kBlocks == 1 ? 232448 : 115000), "shared memory");
 };
 
 // What the unpacking warps tell the softmax about a page.
@@ -106,6 +121,23 @@ CTI_DEVICE uint32_t max2(uint32_t a, uint32_t b) {
   return d;
 }
 
+// A scale of fp16 as two: its upper 7 bits, and the other 4.  A sum (16 + n) top + b
+// of a group whose values are not of one sign is a multiple of s 2^-7 or more and
+// below 16 s, so 11 bits hold it; (16 + n) rest has 9.
+struct TwoScales {
+  uint32_t top, rest;
+  CTI_DEVICE explicit TwoScales(uint32_t s) : top(s & 0xfff0fff0u) {
+    const __half2 d = __hsub2_rn(*reinterpret_cast<__half2*>(&s), *reinterpret_cast<__half2*>(&top));
+    rest = *reinterpret_cast<const uint32_t*>(&d);
+  }
+};
+
+// a b of both halves in fp16.
+CTI_DEVICE uint32_t mul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2_rn(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // 16 TMEM columns and their wait in one statement, as the 32-column form.
 CTI_DEVICE void tmem_ld_x16_sync(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -120,11 +152,11 @@ CTI_DEVICE void tmem_ld_x16_sync(uint32_t taddr, uint32_t (&r)[16]) {
 }
 
 template <typename T, int G, int TILES>
-__global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
+__global__ void __launch_bounds__(Shape<T, G, TILES>::kThreads, Shape<T, G, TILES>::kBlocks)
     kv4_tiles_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pages, const Args a,
                      T* __restrict__ out) {
   using Y = Type16<T>;
-  using Z = Shape<G, TILES>;
+  using Z = Shape<T, G, TILES>;
   constexpr int D = Z::D;
   constexpr int S = Z::kStages, R = Z::kRaw;
   constexpr int kRow = Z::kRow;
@@ -133,7 +165,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + TILES * Z::kQBytes;  // [S] x {K, V}
-  uint8_t* sRaw = sKV + (size_t)S * 2 * Z::kKBytes;  // [R] page blocks
+  uint8_t* sRaw = sKV + (size_t)S * Z::kStageBytes;  // [R] page blocks
   PageInfo* info = reinterpret_cast<PageInfo*>(sRaw + (size_t)R * block_bytes(G));
   uint32_t* sMeta = reinterpret_cast<uint32_t*>(info + S);
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(sMeta + Z::kMetaBytes / 4);  // [S]
@@ -494,7 +526,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
         const int most = is_page ? rg.most - key0 : 0;  // keys of the page that some row sees
         const bool whole = is_page && key0 + kPage <= rg.all;
         const int st = g % S;
-        uint8_t* dst = sKV + (size_t)st * 2 * Z::kKBytes;
+        uint8_t* dst = sKV + (size_t)st * Z::kStageBytes;
         const uint8_t* blk = sRaw + (g % R) * block_bytes(G);
         ok = __all_sync(0xffffffffu,
                         mbar_wait(&raw_full[g % R], (uint32_t)((g / R) & 1), a.status, 0x720,
@@ -598,17 +630,29 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
               const int nt = y / G, gr = y % G;  // nt: octets past nt0
               const uint32_t s2 = __byte_perm(sb[y], sb[y], 0x1010);
               const uint32_t b2 = __byte_perm(sb[y], sb[y], 0x3232);
+              uint8_t* row = to + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow + (at_k ^ 64 * (gr & 1));
               uint32_t o[4];
+              if constexpr (Z::kTwo) {
+                const TwoScales two(s2);
+                uint32_t rest[4];
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
-                o[p] = fma2<__half>(code_pair<__half>(w[y], p), s2, b2);
-              *reinterpret_cast<uint4*>(to + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow +
-                                        (at_k ^ 64 * (gr & 1))) =
-                  make_uint4(o[0], o[1], o[2], o[3]);
+                for (int p = 0; p < 4; ++p) {
+                  const uint32_t c = code_pair<__half>(w[y], p);
+                  o[p] = fma2<__half>(c, two.top, b2);
+                  rest[p] = mul2(c, two.rest);
+                }
+                *reinterpret_cast<uint4*>(row + Z::kKBytes) =
+                    make_uint4(rest[0], rest[1], rest[2], rest[3]);
+              } else {
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                  o[p] = fma2<__half>(code_pair<__half>(w[y], p), s2, b2);
+              }
+              *reinterpret_cast<uint4*>(row) = make_uint4(o[0], o[1], o[2], o[3]);
             }
           }
         } else {
-          uint8_t* vt = dst + Z::kKBytes;
+          uint8_t* vt = dst + Z::kVAt;
 #pragma unroll 1
           for (int x = 0; x < kVecs; ++x) {
             const int v = part * kVecs + x, nt0 = 4 * v / G;
@@ -634,10 +678,26 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             for (int y = 0; y < 4; ++y) {
               const int nt = y / G, gr = y % G;
               uint32_t o[4];
-#pragma unroll
-              for (int p = 0; p < 4; ++p)
-                o[p] = fma2<__half>(code_pair<__half>(w[y], p), sb[y].x, sb[y].y);
               uint8_t* row = to + (gr >> 1) * Z::kKVPanel + nt * 8 * kRow;
+              if constexpr (Z::kTwo) {
+                const TwoScales two(sb[y].x);
+                uint32_t rest[4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                  const uint32_t c = code_pair<__half>(w[y], p);
+                  o[p] = fma2<__half>(c, two.top, sb[y].y);
+                  rest[p] = mul2(c, two.rest);
+                }
+                uint8_t* low = row + Z::kKBytes;
+                *reinterpret_cast<uint2*>(low + (at_v0 ^ 64 * (gr & 1))) = make_uint2(
+                    __byte_perm(rest[0], rest[1], 0x5410), __byte_perm(rest[2], rest[3], 0x5410));
+                *reinterpret_cast<uint2*>(low + (at_v1 ^ 64 * (gr & 1))) = make_uint2(
+                    __byte_perm(rest[0], rest[1], 0x7632), __byte_perm(rest[2], rest[3], 0x7632));
+              } else {
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                  o[p] = fma2<__half>(code_pair<__half>(w[y], p), sb[y].x, sb[y].y);
+              }
               *reinterpret_cast<uint2*>(row + (at_v0 ^ 64 * (gr & 1))) =
                   make_uint2(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410));
               *reinterpret_cast<uint2*>(row + (at_v1 ^ 64 * (gr & 1))) =
@@ -693,13 +753,17 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
                            abort_flag);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t qa = q_addr + i * Z::kQBytes, ka = kv_addr + st * 2 * Z::kKBytes;
+            const uint32_t qa = q_addr + i * Z::kQBytes, ka = kv_addr + st * Z::kStageBytes;
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const int panel = kk * 32 / kRow, off = kk * 32 % kRow;
               umma_bf16(tmem + i * Z::kTileCols + 64u * b,
                         tile_desc<kRow>(qa + panel * Z::kQPanel + off),
                         tile_desc<kRow>(ka + panel * Z::kKVPanel + off), id_s, kk != 0 ? 1u : 0u);
+              if (Z::kTwo)
+                umma_bf16(tmem + i * Z::kTileCols + 64u * b,
+                          tile_desc<kRow>(qa + panel * Z::kQPanel + off),
+                          tile_desc<kRow>(ka + Z::kKBytes + panel * Z::kKVPanel + off), id_s, 1u);
             }
             umma_commit(&s_full[2 * i + b]);
             any = true;
@@ -740,13 +804,16 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
             tc_fence_after();
             const uint32_t pbuf = tmem + i * Z::kTileCols + 64u * b;
             const uint32_t ocol = tmem + i * Z::kTileCols + 128u;
-            const uint32_t va = kv_addr + st * 2 * Z::kKBytes + Z::kKBytes;
+            const uint32_t va = kv_addr + st * Z::kStageBytes + Z::kVAt;
 #pragma unroll
-            for (int kk = 0; kk < kPage / 16; ++kk)
-              umma_bf16_ts(ocol, pbuf + kk * 8,
-                           tile_desc<kRow>(va + kk * 16 * kRow,
-                                           Z::kPanels == 2 ? Z::kKVPanel : 8 * kRow),
-                           id_pv, j == 0 && kk == 0 ? 0u : 1u);
+            for (int kk = 0; kk < kPage / 16; ++kk) {
+              constexpr uint32_t panel = Z::kPanels == 2 ? Z::kKVPanel : 8 * kRow;
+              umma_bf16_ts(ocol, pbuf + kk * 8, tile_desc<kRow>(va + kk * 16 * kRow, panel), id_pv,
+                           j == 0 && kk == 0 ? 0u : 1u);
+              if (Z::kTwo)
+                umma_bf16_ts(ocol, pbuf + kk * 8,
+                             tile_desc<kRow>(va + Z::kKBytes + kk * 16 * kRow, panel), id_pv, 1u);
+            }
             umma_commit(&pv_done[2 * i + b]);
             umma_commit(&kv_empty[st]);
             any = true;
@@ -783,7 +850,7 @@ __global__ void __launch_bounds__(Shape<G, TILES>::kThreads, TILES == 2 ? 1 : 2)
 template <typename T, int G, int TILES>
 int launch(const void* q, const void* pages, const Args& a, int64_t y, int splits, void* out,
            cudaStream_t s) {
-  using Z = Shape<G, TILES>;
+  using Z = Shape<T, G, TILES>;
   static uint64_t configured = 0;
   if (ensure_smem_limit(kv4_tiles_kernel<T, G, TILES>, (int)Z::kSmem, configured) != cudaSuccess)
     return CTI_ERR_CUDA;

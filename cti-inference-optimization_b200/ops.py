@@ -500,8 +500,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
     by them, results hold for any.  Returns a contiguous [tokens, heads,
     head_dim]; a token that sees no key is zero, and rows of no sequence are
     not written.  Relative error of a row: 0.0022 in bfloat16 and 0.0003 in
-    float16 for few tokens, 0.0017 and 0.0005 where they are taken in tiles of
-    128 rows (keys, values and weights in 11 bits each)."""
+    float16 for few tokens, 0.0017 and 0.0003 where they are taken in tiles of
+    128 rows."""
     seqs = _kv4_index(cache, cu_seqlens, kv_lens, page_table)
     hd, Hkv = cache.head_dim, cache.kv_heads
     H = q.shape[1] if q.dim() == 3 else 0

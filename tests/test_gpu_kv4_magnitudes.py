@@ -226,3 +226,26 @@ def test_groups_of_different_magnitudes(cuda_device, H, Hkv, D, n):
     off = (out.double().cpu() - want).unflatten(-1, (-1, 32)).norm(dim=-1)
     off = (off / want.unflatten(-1, (-1, 32)).norm(dim=-1)).max()
     assert off <= _tolerance(torch.bfloat16, n >= 100), float(off)
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(4, 4, 32), (16, 4, 64), (8, 2, 128)])
+@pytest.mark.parametrize("n", [16, 110, 300])
+@pytest.mark.parametrize("causal", [True, False])
+def test_fp16_is_rounded_twice_whatever_the_rows(cuda_device, H, Hkv, D, n, causal):
+    """Keys with channels of their own size and offset, as projections give them.  Two roundings to
+    fp16 count, whichever kernel runs: the output's and one of values and weights.  A rounding's
+    mean square is a third of the half step's at most, so over all rows of a head the error is
+    below sqrt(2 / 3) 2^-11 of the output."""
+    from cti_b200 import _lib, ops
+
+    total = 1500
+    g = torch.Generator().manual_seed(n + D)
+    k = torch.randn(total, Hkv, D, generator=g) * torch.exp(0.5 * torch.randn(Hkv, D, generator=g))
+    k = (k + 0.7 * torch.randn(Hkv, D, generator=g)).half()
+    v = torch.randn(total, Hkv, D, generator=g).half()
+    s = Setup(cuda_device, [n], [total], H, Hkv, D, torch.float16, k=k, v=v)
+    out = ops.kv4_attention(s.q.to(cuda_device), s.cache, s.cu, s.lens, s.table, n, causal=causal)
+    _lib.raise_on_status(cuda_device)
+    want, _ = ref.attention(s.q, ref.held(k), ref.held(v), [n], [total], causal, D ** -0.5)
+    off = (out.double().cpu() - want).norm(dim=(0, 2)) / want.norm(dim=(0, 2))
+    assert off.max() <= math.sqrt(2 / 3) * 2.0 ** -11, off.tolist()
