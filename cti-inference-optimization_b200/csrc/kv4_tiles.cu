@@ -31,7 +31,7 @@
 // is held in, from page to page: it is chosen with the first page (bound of the
 // magnitudes at 2^12) and again where a page's bound leaves 2^6 .. 2^15; then O is
 // multiplied by the difference, which rounds nothing (fp32 holds O while the
-// pages of a sequence's head lie within 2^80 of each other).  So P and the sum l
+// pages of a sequence's head lie within 2^64 of each other).  So P and the sum l
 // know nothing of it.  Every wait is a bounded mbarrier wait; one that runs out
 // records its site in the status word and the roles unwind.
 //
@@ -574,10 +574,10 @@ __global__ void __launch_bounds__(Shape<T, G, TILES>::kThreads, Shape<T, G, TILE
         if (keys) {
           e = top > 0.0f ? max(-116, top_e - 14) : 0;  // to 2^14
         } else {
-          // O in its next unit stays finite while that is not 2^80 below its largest.
+          // O, below 2^30 for each key, stays finite in a unit 2^64 below its largest.
           if (top > 0.0f && (unit_most == INT_MIN || top_e - unit < 6 || top_e - unit >= 15)) {
             unit = max(-116, top_e - 12);
-            if (unit_most != INT_MIN) unit = max(unit, unit_most - 80);
+            if (unit_most != INT_MIN) unit = max(unit, unit_most - 64);
             unit_most = max(unit, unit_most);
           }
           e = unit;

@@ -414,7 +414,7 @@ int cti_kv4_read(const void* pages, int64_t num_pages, int dtype, const int32_t*
  * another order of summation).  A value that is not finite reaches only the
  * rows that see its token, where it may spoil the whole row.  In bf16, |scale|
  * times a query's magnitudes may be up to 1e34; values of one head that are
- * 2^80 below others of their sequence may count as 0.  tokens * heads
+ * 2^64 below others of their sequence may count as 0.  tokens * heads
  * and num_seqs * kv_heads below 2^31 - 512 (CTI_ERR_UNSUPPORTED otherwise).
  * workspace: cti_kv4_attention_workspace_bytes(...) bytes, 256-byte aligned
  * (64 MB at most; may be NULL where that is 0); contents do not outlive the

@@ -249,3 +249,23 @@ def test_fp16_is_rounded_twice_whatever_the_rows(cuda_device, H, Hkv, D, n, caus
     want, _ = ref.attention(s.q, ref.held(k), ref.held(v), [n], [total], causal, D ** -0.5)
     off = (out.double().cpu() - want).norm(dim=(0, 2)) / want.norm(dim=(0, 2))
     assert off.max() <= math.sqrt(2 / 3) * 2.0 ** -11, off.tolist()
+
+
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("n", TOKENS)
+@pytest.mark.parametrize("where", [0, 3, 6])
+@pytest.mark.parametrize("size", [1e15, 1e-15])
+def test_a_page_of_other_magnitude_and_no_weight(cuda_device, H, Hkv, D, n, where, size):
+    """One page's values are 1e15, or all others' are, and its keys' scores lie 150 below the
+    others': it takes part in no output, and must not take the others' bits, whether it comes
+    first, in between or last."""
+    total = 448
+    mine = torch.arange(total) // 64 == where
+    s = _setup(cuda_device, n, total, H, Hkv, D, torch.bfloat16, size_k=0.7,
+               size_v=torch.where(mine, size, 1.0) if size > 1 else torch.where(mine, 1.0, 1e15))
+    s.k[mine] = 0.0
+    s.k[mine, :, :32] = -150.0 * D ** 0.5 / 32
+    s.q[..., :32] = 1.0
+    t = Setup(cuda_device, [n], [total], H, Hkv, D, torch.bfloat16, k=s.k, v=s.v)
+    t.q = s.q
+    _check(t, torch.bfloat16, n >= 100, max_new=n, causal=False)
