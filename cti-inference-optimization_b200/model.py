@@ -316,23 +316,23 @@ class CTRModel(nn.Module):
             raise ValueError("user_offsets must hold one more entry than seqs")
         T = self.rep_encoder.tokens(batch)
         if uo[0] < 0 or uo[-1] > T or any(b < a for a, b in zip(uo[:-1], uo[1:])):
-            raise ValueError(f"user_offsets must not fall, from 0 to {T} at most, got {uo}")
+            raise ValueError(f"user_offsets must not fall, from 0 to {T} at most")
         self.seq_encoder.check_cache(cache)
         extension = cache.extend(seqs, [b - a for a, b in zip(uo[:-1], uo[1:])])
-        probs = torch.full((T,), float("nan"), device=cache.device)
-        if uo[-1] == uo[0]:
-            return probs
         try:
-            x = self.rep_encoder(batch)
-            h, _ = self.seq_encoder(x[uo[0]:uo[-1]], extension)
-            scored = self.head(h, want_logits=False)[1]
+            if extension["tokens"]:
+                x = self.rep_encoder(batch)
+                h, _ = self.seq_encoder(x[uo[0]:uo[-1]], extension)
+                scored = self.head(h, want_logits=False)[1]
+                if scored.numel() == T:
+                    return scored
+            probs = torch.full((T,), float("nan"), dtype=torch.float32, device=cache.device)
+            if extension["tokens"]:
+                probs[uo[0]:uo[-1]] = scored
+            return probs
         except BaseException:
             cache.undo(extension)
             raise
-        if scored.numel() == T:
-            return scored
-        probs[uo[0]:uo[-1]] = scored
-        return probs
 
     @torch.no_grad()
     def predict_host(self, batch: dict, chunks: int = 8,
