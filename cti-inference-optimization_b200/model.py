@@ -184,7 +184,7 @@ class TransformerEncoder(nn.Module):
         cache = extension.get("cache")
         if cache is not None:
             self.check_cache(cache)
-            if T < extension["tokens"]:
+            if T < extension.get("tokens", 0):
                 raise ValueError(f"the extension holds {extension['tokens']} tokens, x {T}")
         mark = extension.get("mark") or (lambda name: None)
         pending = None  # the previous layer's MoE output, not yet added
